@@ -152,14 +152,17 @@ LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 BORDERS = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)
 
 
+def _power(E):
+    """2^(E - 127), exactly: E is the exponent field of a 32-bit number."""
+    return (E.to(torch.int32) << 23).view(torch.float32)
+
+
 def _quantise(x):
     """[..., D] -> codes [..., D / 2] and scale bytes [..., D / 32], uint8.
     Dividing by a power of two is exact in 32 bits."""
     b = x.float().unflatten(-1, (-1, 32))
-    _, e = torch.frexp(b.abs().amax(-1))  # amax = m 2^e, 0.5 <= m < 1: floor(log2) = e - 1
-    E = (e - 1 - 2 + 127).clamp(min=1)
-    E = torch.where(b.abs().amax(-1) > 0, E, torch.ones_like(E))
-    v = torch.ldexp(b, (127 - E).unsqueeze(-1)).flatten(-2)
+    E = ((b.abs().amax(-1).view(torch.int32) >> 23) - 2).clamp(min=1)
+    v = (b / _power(E).unsqueeze(-1)).flatten(-2)
     a = v.abs()
     # Borders below even codes are passed only from above, below odd ones at them.
     code = (a > 0.25).to(torch.uint8)
@@ -179,7 +182,7 @@ def _values(codes, scales):
     lut = torch.tensor(LEVELS + tuple(-v for v in LEVELS), dtype=torch.float32, device=codes.device)
     both = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)
     v = lut[both.int()].unflatten(-1, (-1, 32))
-    return torch.ldexp(v, (scales.int() - 127).unsqueeze(-1)).flatten(-2)
+    return (v * _power(scales).unsqueeze(-1)).flatten(-2)
 
 
 def _page_views(pages, D):
