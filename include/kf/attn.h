@@ -62,6 +62,11 @@ enum kf_status {
 #define KF_ATTN_OUT_BF16 4 /* O is written as bf16 (RNE of the fp32 result)     */
 #define KF_ATTN_LSE 8      /* row_max receives LSE = Mi + ln(Li) (natural log;
                               -inf for a row without keys); row_sumexp unused */
+/* kf_attn_packed, kf_qk_norm_rope, kf_kv4_* and kf_attn_decode_kv4 flags. */
+#define KF_BF16 16         /* 16-bit inputs (and the cache's 16-bit side) are bf16,
+                              not fp16                                          */
+#define KF_ROPE_INTERLEAVED 32 /* kf_qk_norm_rope: pairs (2i, 2i + 1), not
+                              (i, i + rot / 2)                                  */
 
 /* Which kernels kf_attn_fwd runs for a shape (see kf_attn_plan). */
 enum kf_path {
@@ -259,6 +264,114 @@ int kf_attn_decode_paged(const void* Q, const void* K_pages, const void* V_pages
                          int B, int q_len, int H_q, int H_kv, int D,
                          int page_size, int max_pages_per_seq, int num_pages, int flags,
                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention over packed sequences: the tokens of all sequences one after the
+ * other, as the projections write them.  No counterpart in the reference.
+ *
+ * Q [tokens_q, H_q, D], K and V [tokens_kv, H_kv, D], fp16 (bf16 with
+ *   KF_BF16), D = 64, 128 or 256.  `strides`: NULL (contiguous), or six host
+ *   values, token and head strides of Q, K and V in elements, multiples of 8;
+ *   the D channels of a head are contiguous.
+ * q_starts, kv_starts: device int [n_seqs + 1], not decreasing: sequence b has
+ *   the queries q_starts[b] .. q_starts[b + 1] - 1 and the keys kv_starts[b] ..
+ *   kv_starts[b + 1] - 1; either may be empty.  The same array for prompts;
+ *   more keys than queries for a chunk of a prompt over its context (see
+ *   kf_kv4_read).  Values outside the tensors are clamped to them.
+ * flags & KF_ATTN_CAUSAL: query i of n sees keys j <= i + (keys of its
+ *   sequence) - n, as in kf_attn_fwd_ex.  A row that sees no key gets O = 0,
+ *   Mi = -inf, Li = 0 (LSE = -inf).
+ * O [tokens_q, H_q, D] contiguous, fp32 or by KF_ATTN_OUT_F16 / _BF16; row_max,
+ *   row_sumexp [tokens_q, H_q], optional, as in kf_attn_fwd_ex (KF_ATTN_LSE).
+ *   Rows of tokens outside the sequences are left as they were.
+ * No workspace. */
+int kf_attn_packed(const void* Q, const void* K, const void* V, void* O,
+                   float* row_max, float* row_sumexp, const int64_t* strides,
+                   const int* q_starts, const int* kv_starts,
+                   int n_seqs, int tokens_q, int tokens_kv, int H_q, int H_kv, int D,
+                   int flags, void* stream);
+
+/* RMS norm of every query and key head, then rotary positions, in one pass.
+ * No counterpart in the reference.
+ *
+ * Q, Q_out [tokens, H_q, D], K, K_out [tokens, H_kv, D], fp16 (bf16 with
+ *   KF_BF16), D = 16, 64, 128 or 256; `strides`: NULL (contiguous), or eight
+ *   host values, token and head strides of Q, K, Q_out and K_out in elements,
+ *   multiples of 8.  Q_out may be Q and K_out may be K, with the same strides;
+ *   outputs that overlap anything else give undefined rows.
+ * q_weight, k_weight: [D] of the same type, or NULL: Q or K is not normed.
+ *   With one, x -> x / sqrt(mean(x^2) + eps) * weight over the D channels.
+ * The first `rot` channels (a multiple of 16, 0 to D) of a head are turned by
+ *   the angles positions[token] * freqs[i], i < rot / 2 (device double, radians
+ *   per position, whatever context scaling they include), in the pairs
+ *   (i, i + rot / 2) or, with KF_ROPE_INTERLEAVED, (2i, 2i + 1), and multiplied
+ *   by `scale`; the others keep their normed values.
+ * positions: device int [tokens].  positions and freqs may be NULL if rot is 0.
+ * Computed in fp32 (the angles in fp64) and rounded once. */
+int kf_qk_norm_rope(const void* Q, const void* K, void* Q_out, void* K_out,
+                    const int64_t* strides, const void* q_weight, const void* k_weight,
+                    const int* positions, const double* freqs,
+                    int tokens, int H_q, int H_kv, int D, int rot, float eps, float scale,
+                    int flags, void* stream);
+
+/* A paged K/V cache in 4 bits.  No counterpart in the reference.
+ *
+ * Format: the microscaling one with 4-bit elements.  Every block of 32
+ * consecutive channels of a row has one scale byte E (1 .. 254), scale
+ * 2^(E - 127), and 32 codes (a sign bit over 0, .5, 1, 1.5, 2, 3, 4, 6).  E is
+ * the exponent field of the block's largest magnitude as fp32, less 2, at
+ * least 1; a channel is rounded to the nearest code, ties to the even code,
+ * magnitudes above 6 scales to 6.  A block with an infinity or a NaN gets E = 255
+ * and reads back as NaN.
+ * K_pages, V_pages: [num_pages, H_kv, kf_kv4_page_bytes(page_size, D)] bytes;
+ *   per page and head the codes of its rows [page_size][D / 2] (channel 2i in
+ *   the low half of byte i), then their scales [page_size][D / 32].  D = 64,
+ *   128 or 256; page_size a power of two in [16, 2^20].
+ * block_table: device int [n_seqs, max_pages_per_seq], as in
+ *   kf_attn_decode_paged. */
+size_t kf_kv4_page_bytes(int page_size, int D);  /* 0 for an invalid size */
+
+/* Quantise the new tokens' K and V into the cache.  K, V [tokens, H_kv, D] fp16
+ * (bf16 with KF_BF16), packed by seq_starts (device int [n_seqs + 1], as in
+ * kf_attn_packed); `strides`: NULL or four host values, token and head strides
+ * of K and V.  kv_lens: device int [n_seqs], the keys of each sequence with the
+ * new tokens: sequence b's packed tokens become its last ones.  A token whose
+ * page id is outside [0, num_pages), or whose place is outside the table, is
+ * not written; nor is one outside the sequences.  Two sequences of a call that
+ * write the same row of the same page leave an undefined row. */
+int kf_kv4_append(const void* K, const void* V, const int64_t* strides,
+                  void* K_pages, void* V_pages, const int* block_table,
+                  const int* seq_starts, const int* kv_lens,
+                  int n_seqs, int tokens, int H_kv, int D,
+                  int page_size, int max_pages_per_seq, int num_pages,
+                  int flags, void* stream);
+
+/* Read rows back: K, V [tokens, H_kv, D] contiguous, fp16 (bf16 with KF_BF16),
+ * exactly the values the codes stand for (fp16 cannot hold all of a cache
+ * written from bf16: beyond its range the nearest, by the conversion).
+ * Sequence b's packed tokens (seq_starts) are its last ones of kv_lens[b], so
+ * seq_starts = the running sum of kv_lens reads whole contexts, for
+ * kf_attn_packed with these as kv_starts.  Tokens of no valid page get zeros;
+ * rows outside the sequences are left as they were. */
+int kf_kv4_read(const void* K_pages, const void* V_pages, const int* block_table,
+                const int* seq_starts, const int* kv_lens, void* K, void* V,
+                int n_seqs, int tokens, int H_kv, int D,
+                int page_size, int max_pages_per_seq, int num_pages,
+                int flags, void* stream);
+
+/* Decode over the 4-bit cache: kf_attn_decode_paged's call and results for
+ * pages in the format above.  Q [B, H_q, q_len, D] fp16 (bf16 with KF_BF16);
+ * (H_q / H_kv) * q_len <= 32, else KF_ERR_SIZE; D = 64, 128 or 256.  The
+ * workspace (256-byte aligned, no initialisation, not shared by calls that can
+ * run concurrently) is required.  With KF_BF16 the softmax weights are rounded
+ * to bf16 before they meet V, else to fp16; V itself is exact. */
+size_t kf_attn_decode_kv4_workspace_bytes(int B, int q_len, int H_q, int H_kv, int D,
+                                          int page_size, int max_pages_per_seq);
+int kf_attn_decode_kv4(const void* Q, const void* K_pages, const void* V_pages,
+                       const int* block_table, const int* kv_lens,
+                       void* O, float* row_max, float* row_sumexp,
+                       int B, int q_len, int H_q, int H_kv, int D,
+                       int page_size, int max_pages_per_seq, int num_pages, int flags,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* The reference launcher's contract (tests/test_flash_attn.cu:52-113):
  * q_len = kv_len = S, scratch allocated and freed by the call, stream

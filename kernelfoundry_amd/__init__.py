@@ -23,6 +23,10 @@ Interface, mirroring the reference harness (sviraaj/kernelfoundry):
   [num_pages, H_kv, page_size, D] and a per-sequence block table).
 * ``plan(B, q_len, kv_len, H_q, H_kv, D, num_cus=None)`` -- which kernels run,
   sized for the current device's compute units (or ``num_cus``).
+* ``attn_packed``, ``qk_norm_rope`` / ``rope_freqs``, ``kv4_append`` /
+  ``kv4_read``, ``attn_decode_kv4`` -- what a server runs beside these: packed
+  prompts, head norms with rotary positions, a paged cache in 4 bits and the
+  decode over it (serve.py; no reference counterpart).
 """
 from __future__ import annotations
 
@@ -41,6 +45,8 @@ __all__ = [
     "PATH_NAMES", "attn_fwd_ex_ptr", "attn_decode_paged", "attn_decode_paged_ptr",
     "paged_workspace_bytes", "workspace_bytes_lens",
     "workspace_bytes_least", "kernel_names",
+    "KF_BF16", "KF_ROPE_INTERLEAVED", "attn_packed", "rope_freqs", "qk_norm_rope", "kv4_page_bytes",
+    "kv4_append", "kv4_read", "kv4_workspace_bytes", "attn_decode_kv4",
 ]
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -155,6 +161,21 @@ def load_library(path: str = LIB_PATH):
     lib.kf_attn_decode_paged.restype = i
     lib.kf_attn_decode_paged_workspace_bytes.argtypes = [i] * 7
     lib.kf_attn_decode_paged_workspace_bytes.restype = sz
+    i64s, f = ctypes.POINTER(ctypes.c_int64), ctypes.c_float
+    lib.kf_attn_packed.argtypes = [p] * 6 + [i64s, p, p] + [i] * 7 + [p]
+    lib.kf_attn_packed.restype = i
+    lib.kf_qk_norm_rope.argtypes = [p] * 4 + [i64s] + [p] * 4 + [i] * 5 + [f, f, i, p]
+    lib.kf_qk_norm_rope.restype = i
+    lib.kf_kv4_page_bytes.argtypes = [i] * 2
+    lib.kf_kv4_page_bytes.restype = sz
+    lib.kf_kv4_append.argtypes = [p, p, i64s] + [p] * 5 + [i] * 8 + [p]
+    lib.kf_kv4_append.restype = i
+    lib.kf_kv4_read.argtypes = [p] * 7 + [i] * 8 + [p]
+    lib.kf_kv4_read.restype = i
+    lib.kf_attn_decode_kv4_workspace_bytes.argtypes = [i] * 7
+    lib.kf_attn_decode_kv4_workspace_bytes.restype = sz
+    lib.kf_attn_decode_kv4.argtypes = [p] * 8 + [i] * 9 + [p, sz, p]
+    lib.kf_attn_decode_kv4.restype = i
     lib.kf_launch_flash_attn.argtypes = [p, p, p, p] + [i] * 5 + [p]
     lib.kf_launch_flash_attn.restype = i
     lib.kf_status_string.argtypes = [i]
@@ -447,3 +468,7 @@ def attn_decode_paged(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, re
     if return_lse:
         return out, Mi
     return (out, Mi, Li) if return_stats else out
+
+
+from .serve import (KF_BF16, KF_ROPE_INTERLEAVED, attn_decode_kv4, attn_packed,  # noqa: E402
+                    kv4_append, kv4_page_bytes, kv4_read, kv4_workspace_bytes, qk_norm_rope, rope_freqs)

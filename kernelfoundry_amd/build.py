@@ -10,6 +10,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_DIR)
@@ -19,6 +20,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libkf_attn.so")
 INCLUDE = os.path.join(REPO, "include")
 
 ARCH = "gfx950"
+SOURCES = ("attn_capi.hip", "serve_capi.hip")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # Packed-fp32 VALU ops are kept out of every code object (-packed-fp32-ops).
@@ -51,10 +53,16 @@ def run(cmd, verbose=False):
 def build_library(verbose=False, extra_flags=()):
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
-    cmd = [HIPCC, *DEVICE_FLAGS, *extra_flags, "-shared", "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}",
-           os.path.join(CSRC, "attn_capi.hip"), "-o", tmp]
-    run(cmd, verbose)
+    flags = [*DEVICE_FLAGS, *extra_flags, "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}"]
+    objects = [os.path.join(LIB_DIR, os.path.splitext(s)[0] + ".o") for s in SOURCES]
+    # The translation units side by side.
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        list(pool.map(lambda so: run([HIPCC, *flags, "-c", os.path.join(CSRC, so[0]), "-o", so[1]], verbose),
+                      zip(SOURCES, objects)))
+    run([HIPCC, f"--offload-arch={ARCH}", "-shared", *objects, "-o", tmp], verbose)
     os.replace(tmp, LIB_PATH)
+    for o in objects:
+        os.remove(o)
     return LIB_PATH
 
 

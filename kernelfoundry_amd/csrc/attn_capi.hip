@@ -15,6 +15,7 @@
 #include <numeric>
 
 #include "attn_kernels.h"
+#include "capi_internal.h"
 #include "kf/attn.h"
 
 namespace {
@@ -159,14 +160,11 @@ constexpr int kRaggedEvenRounds(int D) { return D == 16 ? 5 : 1; }
 constexpr int kRaggedMergeMaxWaves = 8192;
 constexpr int kCausalShortKeys = 768;
 constexpr int kCausalWide2Keys = 1024;
-constexpr size_t kWsAlign = 256;
-
 thread_local int g_last_hip_error = 0;
 
-struct DeviceShape {
-    int cus;
-    int xcds;
-};
+}  // namespace
+
+namespace kf_capi {
 
 // CU and XCD counts of the device current on the calling thread, cached per
 // device; the MI355X defaults when no device is visible.
@@ -193,7 +191,29 @@ DeviceShape current_device_shape() {
     return {cus, xcds};
 }
 
-inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+int hip_fail(hipError_t e) {
+    g_last_hip_error = (int)e;
+    return KF_ERR_HIP;
+}
+
+int paged_geometry(int page_size, int max_pages_per_seq, int num_pages, int* shift, int* cap) {
+    if (max_pages_per_seq <= 0 || num_pages <= 0) return KF_ERR_SIZE;
+    if (page_size < 16 || page_size > (1 << 20) || (page_size & (page_size - 1)) != 0)
+        return KF_ERR_SIZE;
+    const long long c = (long long)page_size * max_pages_per_seq;
+    if (c > INT_MAX) return KF_ERR_SIZE;
+    int sh = 0;
+    while ((1 << sh) < page_size) ++sh;
+    *shift = sh;
+    *cap = (int)c;
+    return KF_OK;
+}
+
+}  // namespace kf_capi
+
+namespace {
+
+using namespace kf_capi;
 
 bool supported_head_dim(int D) { return D == 16 || D == 64 || D == 128 || D == 256; }
 
@@ -584,13 +604,6 @@ size_t best_ws_bytes(const Plan& pl, bool lens) {
     return (lens || pl.ragged_even) && pl.ragged_bytes > pl.ws_bytes ? pl.ragged_bytes : pl.ws_bytes;
 }
 
-inline bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
-
-int hip_fail(hipError_t e) {
-    g_last_hip_error = (int)e;
-    return KF_ERR_HIP;
-}
-
 template <int D, int NW, int KS = 1>
 void launch_prefill(const Plan& pl, const kf::AttnParams& prm, bool mask, hipStream_t stream) {
     if constexpr (D >= 256 && NW == 4 && KS == 1) {
@@ -782,14 +795,20 @@ hipError_t launch_merge(const Plan& pl, const kf::AttnParams& prm, hipStream_t s
     return hipGetLastError();
 }
 
+// The merge of the ragged decode's partials, prm.merge_waves waves per KV head.
+template <int D>
+hipError_t launch_ragged_merge(int n_groups, const kf::AttnParams& prm, hipStream_t stream) {
+    constexpr int kWaves = kf::kRaggedMergeWaves;
+    const long long blocks = ((long long)n_groups * prm.merge_waves + kWaves - 1) / kWaves;
+    kf::kf_attn_ragged_merge_kernel<D><<<dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream>>>(prm);
+    return hipGetLastError();
+}
+
 // The ragged decode and its merge (one wave per query row and column block).
 template <int D>
 hipError_t launch_ragged(const Plan& pl, const kf::AttnParams& params, hipStream_t stream) {
     kf::AttnParams prm = params;
-    // A wave per item of a head of many partials, up to kRaggedMergeMaxWaves in
-    // all; then as many as cover the rows of one of few.
-    const int items = pl.R * kf::RaggedMerge<D>::kNCB, few = (pl.R * (D / 4) + 63) / 64;
-    prm.merge_waves = std::max(few, std::min(items, kRaggedMergeMaxWaves / pl.n_groups));
+    prm.merge_waves = ragged_merge_waves(pl.R, pl.n_groups, D);
     const dim3 grid(pl.ragged_wgs), block(kf::RaggedCfg<D>::kThreads);
     if (prm.block_table)
         kf::kf_attn_decode_ragged_kernel<D, true><<<grid, block, 0, stream>>>(prm);
@@ -797,10 +816,7 @@ hipError_t launch_ragged(const Plan& pl, const kf::AttnParams& params, hipStream
         kf::kf_attn_decode_ragged_kernel<D, false><<<grid, block, 0, stream>>>(prm);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    constexpr int kWaves = kf::kRaggedMergeWaves;
-    const long long blocks = ((long long)pl.n_groups * prm.merge_waves + kWaves - 1) / kWaves;
-    kf::kf_attn_ragged_merge_kernel<D><<<dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream>>>(prm);
-    return hipGetLastError();
+    return launch_ragged_merge<D>(pl.n_groups, prm, stream);
 }
 
 template <int D>
@@ -966,22 +982,6 @@ void* static_scratch(hipError_t* err) {
     return addr[dev];
 }
 
-// Paged geometry: page_size a power of two in [16, 2^20], positive counts,
-// key capacity max_pages_per_seq * page_size within int.  Returns the
-// status and, on success, log2(page_size) and the capacity.
-int paged_geometry(int page_size, int max_pages_per_seq, int num_pages, int* shift, int* cap) {
-    if (max_pages_per_seq <= 0 || num_pages <= 0) return KF_ERR_SIZE;
-    if (page_size < 16 || page_size > (1 << 20) || (page_size & (page_size - 1)) != 0)
-        return KF_ERR_SIZE;
-    const long long c = (long long)page_size * max_pages_per_seq;
-    if (c > INT_MAX) return KF_ERR_SIZE;
-    int sh = 0;
-    while ((1 << sh) < page_size) ++sh;
-    *shift = sh;
-    *cap = (int)c;
-    return KF_OK;
-}
-
 int describe_plan(int B, int q_len, int kv_len, int H_q, int H_kv, int D, const DeviceShape& dev,
                   kf_attn_plan_t* plan) {
     if (!plan) return KF_ERR_NULL;
@@ -1003,6 +1003,25 @@ int describe_plan(int B, int q_len, int kv_len, int H_q, int H_kv, int D, const 
 }
 
 }  // namespace
+
+namespace kf_capi {
+
+int ragged_merge_waves(int R, int n_groups, int D) {
+    // A wave per item of a head of many partials, up to kRaggedMergeMaxWaves in
+    // all; then as many as cover the rows of one of few.
+    const int cw = std::min(D / 4, kf::kRaggedMergeCols), items = R * (D / 4 / cw), few = (R * (D / 4) + 63) / 64;
+    return std::max(few, std::min(items, kRaggedMergeMaxWaves / n_groups));
+}
+
+hipError_t merge_ragged(int D, int n_groups, const kf::AttnParams& prm, hipStream_t stream) {
+    switch (D) {
+        case 64: return launch_ragged_merge<64>(n_groups, prm, stream);
+        case 128: return launch_ragged_merge<128>(n_groups, prm, stream);
+        default: return launch_ragged_merge<256>(n_groups, prm, stream);
+    }
+}
+
+}  // namespace kf_capi
 
 extern "C" {
 

@@ -1,0 +1,358 @@
+"""What a server runs beside the attention forward, on torch GPU tensors:
+packed prompts, head norms with rotary positions, and a paged K/V cache in 4
+bits with the decode that reads it (include/kf/attn.h: kf_attn_packed,
+kf_qk_norm_rope, kf_kv4_append, kf_kv4_read, kf_attn_decode_kv4).
+
+    freqs, scale = rope_freqs(128, scaling="yarn", factor=4.0, original_len=8192, device="cuda")
+    Q, K = qk_norm_rope(Q, K, positions, freqs, q_weight=wq, k_weight=wk, scale=scale)
+    kv4_append(K, V, K_pages, V_pages, block_table, seq_starts, kv_lens)
+    O = attn_packed(Q, K, V, seq_starts, causal=True)                          # prompts
+    O = attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens)             # a step
+    K, V = kv4_read(K_pages, V_pages, block_table, kv_starts, kv_lens, total, 128)
+    O = attn_packed(Q, K, V, seq_starts, kv_starts=kv_starts, causal=True)     # a later chunk
+
+The entries run asynchronously on ``stream`` (default: torch's current one)
+and check their arguments on the host only; what device arrays hold
+(sequence starts, key counts, page ids) is bounded by the kernels.  They have
+no backward pass: an input that requires grad is refused while torch records
+gradients.  None of them has a counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import (KF_ATTN_CAUSAL, KF_ERR_HIP, KF_OK, KfError, _new, _out_flags, _output, _raw_stream,
+               _workspace, load_library, status_string)
+
+KF_BF16 = 16
+KF_ROPE_INTERLEAVED = 32
+
+_STRIDES = {n: ctypes.c_int64 * n for n in (4, 6, 8)}
+
+
+def _check(torch, named):
+    """The tensors' device after checking that all are on one GPU."""
+    first = named[0][1]
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError(f"{named[0][0]} must be a GPU tensor")
+    grad = torch.is_grad_enabled()
+    for name, t in named:
+        if t.device != device:
+            raise ValueError(f"{name} must be on {device}")
+        if grad and t.requires_grad:
+            raise ValueError(f"{name} requires grad, but there is no backward pass: call under torch.no_grad()")
+    return device
+
+
+def _half_flag(torch, named):
+    """KF_BF16 or 0 by the one 16-bit type of the tensors."""
+    dtype = named[0][1].dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"{named[0][0]} must be float16 or bfloat16")
+    for name, t in named:
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, as {named[0][0]} is")
+    return KF_BF16 if dtype == torch.bfloat16 else 0
+
+
+def _heads3(name, t):
+    """A [tokens, heads, D] tensor's token and head strides: D contiguous."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, D]")
+    s = t.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8:
+        raise ValueError(f"{name}: the channels must be contiguous, and token and head strides multiples of 8")
+    return s[0], s[1]
+
+
+def _ints(torch, name, t, device, shape):
+    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}")
+    return t.data_ptr()
+
+
+def _starts(torch, name, t, device):
+    if t.dim() != 1 or t.shape[0] < 2:
+        raise ValueError(f"{name} must be [sequences + 1]")
+    return _ints(torch, name, t, device, (t.shape[0],))
+
+
+def _launch(torch, device, call):
+    """call() with `device` current: its streams are the current device's."""
+    if device.index == torch.cuda.current_device():
+        st = call()
+    else:
+        with torch.cuda.device(device):
+            st = call()
+    if st != KF_OK:
+        msg = status_string(st)
+        if st == KF_ERR_HIP:
+            msg += f" (hipError_t {load_library().kf_last_hip_error()})"
+        raise KfError(st, msg)
+
+
+def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, stream=None,
+                out_dtype=None, return_lse=False):
+    """Attention over packed sequences.
+
+    Q [T, H_q, D], K and V [T_kv, H_kv, D], float16 or bfloat16, D = 64, 128 or
+    256; views with other token and head strides (multiples of 8), as those of
+    a fused projection, are read in place.  ``seq_starts`` int32 [N + 1]: sequence b
+    has the tokens seq_starts[b] .. seq_starts[b + 1] - 1, none or more;
+    ``kv_starts`` the same for the keys (default: seq_starts).  ``causal`` is
+    aligned to the last key: query i of n sees keys j <= i + keys - n.
+    Returns O [T, H_q, D] (fp32, or ``out_dtype``), or (O, LSE [T, H_q]) with
+    ``return_lse``; a row without keys gets O = 0, LSE = -inf.  Rows outside
+    the sequences are not written.
+    """
+    import torch
+
+    named = (("Q", Q), ("K", K), ("V", V))
+    device = _check(torch, named)
+    flags = _out_flags(torch, out_dtype, return_lse) | _half_flag(torch, named)
+    strides = [s for name, t in named for s in _heads3(name, t)]
+    T, H_q, D = Q.shape
+    T_kv, H_kv, Dk = K.shape
+    if V.shape != K.shape or Dk != D:
+        raise ValueError("K and V must be [T_kv, H_kv, D], with Q's D")
+    if kv_starts is None:
+        kv_starts = seq_starts
+    starts = _starts(torch, "seq_starts", seq_starts, device)
+    if kv_starts.shape != seq_starts.shape:
+        raise ValueError("kv_starts and seq_starts must have one length")
+    kstarts = _ints(torch, "kv_starts", kv_starts, device, tuple(kv_starts.shape))
+    out = _output(torch, out, (T, H_q, D), out_dtype, device, stream)
+    lse = _new(torch, (T, H_q), torch.float32, device, stream) if return_lse else None
+    if causal:
+        flags |= KF_ATTN_CAUSAL
+    _launch(torch, device, lambda: load_library().kf_attn_packed(
+        Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, None,
+        _STRIDES[6](*strides), starts, kstarts, seq_starts.shape[0] - 1, T, T_kv, H_q, H_kv, D, flags,
+        _raw_stream(torch, stream, device)))
+    return (out, lse) if return_lse else out
+
+
+def rope_freqs(rot, base=10000.0, *, scaling=None, factor=1.0, original_len=None, beta_fast=32.0,
+               beta_slow=1.0, device=None):
+    """Rotary frequencies [rot / 2] (float64, radians per position) and the
+    factor that rotated channels are multiplied by, for qk_norm_rope.
+
+    f_i = base ** (-2 i / rot), and for contexts ``factor`` times as long as
+    those trained on, with ``scaling``:
+    "linear"  f_i / factor (positions interpolated);
+    "ntk"     base * factor ** (rot / (rot - 2)): the lowest frequency
+              interpolated, the highest kept;
+    "yarn"    by the turns f_i makes over ``original_len`` positions: kept from
+              beta_fast turns on, interpolated up to beta_slow, in between
+              linearly mixed; the rotated channels times 1 + ln(factor) / 10.
+    """
+    import torch
+
+    if rot <= 0 or rot % 2:
+        raise ValueError("rot must be a positive even number of channels")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError('scaling must be None, "linear", "ntk" or "yarn"')
+    if scaling is not None and factor < 1.0:
+        raise ValueError("factor must be at least 1")
+    if scaling == "ntk":
+        if rot < 4:
+            raise ValueError('scaling "ntk" needs rot >= 4')
+        base = base * factor ** (rot / (rot - 2))
+    i = torch.arange(rot // 2, dtype=torch.float64)
+    freqs = float(base) ** (-2.0 * i / rot)
+    scale = 1.0
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "yarn":
+        if not original_len or original_len <= 0:
+            raise ValueError('scaling "yarn" needs original_len')
+        if beta_fast <= beta_slow:
+            raise ValueError("beta_fast must be above beta_slow")
+        turns = original_len * freqs / (2.0 * math.pi)
+        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
+        freqs = freqs * keep + freqs / factor * (1.0 - keep)
+        scale = 1.0 + 0.1 * math.log(factor)
+    return freqs.to(device) if device is not None else freqs, scale
+
+
+def qk_norm_rope(Q, K, positions, freqs, out=None, *, q_weight=None, k_weight=None, eps=1e-6,
+                 interleaved=False, scale=1.0, stream=None):
+    """RMS norm of every query and key head, then rotary positions.
+
+    Q [T, H_q, D], K [T, H_kv, D], float16 or bfloat16, D = 16, 64, 128 or 256,
+    with any token and head strides (multiples of 8).  ``q_weight`` /
+    ``k_weight`` [D] of the same type: x / sqrt(mean(x^2) + eps) * weight
+    (None: not normed).  The first 2 * len(freqs) channels (a multiple of 16)
+    are turned by positions[t] * freqs[i] (int32 [T]; float64, see rope_freqs) in the
+    pairs (i, i + len(freqs)), or (2 i, 2 i + 1) with ``interleaved``, and
+    multiplied by ``scale``.  ``positions`` and ``freqs`` None: no rotation.
+    Returns new contiguous tensors, or ``out``, a pair that may be (Q, K)
+    themselves.
+    """
+    import torch
+
+    named = [("Q", Q), ("K", K)]
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            if w.dim() != 1 or w.shape[0] != Q.shape[-1] or not w.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous tensor of D elements")
+            named.append((name, w))
+    device = _check(torch, named)
+    flags = _half_flag(torch, named) | (KF_ROPE_INTERLEAVED if interleaved else 0)
+    strides = [*_heads3("Q", Q), *_heads3("K", K)]
+    T, H_q, D = Q.shape
+    if K.shape[0] != T or K.shape[2] != D:
+        raise ValueError("K must be [T, H_kv, D], with Q's T and D")
+    H_kv = K.shape[1]
+    rot = pos = frq = 0
+    if freqs is not None:
+        if freqs.dtype != torch.float64 or freqs.device != device or freqs.dim() != 1 or not freqs.is_contiguous():
+            raise ValueError(f"freqs must be a contiguous float64 [rot / 2] tensor on {device}")
+        rot, frq = 2 * freqs.shape[0], freqs.data_ptr()
+        if positions is None:
+            raise ValueError("freqs without positions")
+        pos = _ints(torch, "positions", positions, device, (T,))
+    if out is None:
+        out = (_new(torch, (T, H_q, D), Q.dtype, device, stream), _new(torch, (T, H_kv, D), Q.dtype, device, stream))
+        strides += (H_q * D, D, H_kv * D, D)
+    else:
+        for name, y, x in (("out[0]", out[0], Q), ("out[1]", out[1], K)):
+            if y.shape != x.shape or y.dtype != x.dtype or y.device != device:
+                raise ValueError(f"{name} must have the shape, type and device of its input")
+            s = _heads3(name, y)
+            in_place = y.data_ptr() == x.data_ptr() and y.stride() == x.stride()
+            if not (in_place or y.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous, or its input itself")
+            strides += s
+    _launch(torch, device, lambda: load_library().kf_qk_norm_rope(
+        Q.data_ptr(), K.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), _STRIDES[8](*strides),
+        q_weight.data_ptr() if q_weight is not None else None,
+        k_weight.data_ptr() if k_weight is not None else None, pos or None, frq or None, T, H_q, H_kv, D, rot, eps,
+        scale, flags, _raw_stream(torch, stream, device)))
+    return out
+
+
+def kv4_page_bytes(page_size, D) -> int:
+    """Bytes of one KV head's page of the 4-bit cache: pools are uint8 [num_pages,
+    H_kv, kv4_page_bytes(page_size, D)] tensors."""
+    n = int(load_library().kf_kv4_page_bytes(page_size, D))
+    if n == 0:
+        raise ValueError("page_size must be a power of two in [16, 2^20] and D 64, 128 or 256")
+    return n
+
+
+def _pages(torch, K_pages, V_pages, D):
+    """num_pages, H_kv and page_size of a pair of pools."""
+    if K_pages.dim() != 3 or K_pages.shape != V_pages.shape:
+        raise ValueError("K_pages and V_pages must be [num_pages, H_kv, kv4_page_bytes(page_size, D)]")
+    for t in (K_pages, V_pages):
+        if t.dtype != torch.uint8 or not t.is_contiguous():
+            raise ValueError("K_pages and V_pages must be contiguous uint8 tensors")
+    n, H_kv, nbytes = K_pages.shape
+    page_size, rest = divmod(nbytes * 32, 17 * D) if D > 0 else (0, 1)
+    if rest:
+        raise ValueError(f"a page of {nbytes} bytes does not hold whole rows of D = {D}")
+    return n, H_kv, page_size
+
+
+def _table(torch, block_table, kv_lens, device, n_seqs):
+    if block_table.dim() != 2 or block_table.shape[0] != n_seqs:
+        raise ValueError("block_table must be [sequences, max_pages_per_seq]")
+    return (_ints(torch, "block_table", block_table, device, tuple(block_table.shape)),
+            _ints(torch, "kv_lens", kv_lens, device, (n_seqs,)))
+
+
+def kv4_append(K, V, K_pages, V_pages, block_table, seq_starts, kv_lens, *, stream=None):
+    """Quantise new tokens into a paged 4-bit cache.
+
+    K, V [T, H_kv, D] float16 or bfloat16, packed by ``seq_starts`` (int32 [N + 1]),
+    with any token and head strides (multiples of 8).  Sequence b's tokens
+    become the last of its ``kv_lens[b]`` keys (int32 [N], counted with them);
+    ``block_table`` int32 [N, max_pages].  Tokens of an invalid page are not
+    written; no two sequences may write the same row.
+    """
+    import torch
+
+    named = (("K", K), ("V", V))
+    device = _check(torch, (*named, ("K_pages", K_pages), ("V_pages", V_pages)))
+    flags = _half_flag(torch, named)
+    strides = [s for name, t in named for s in _heads3(name, t)]
+    T, H_kv, D = K.shape
+    num_pages, heads, page_size = _pages(torch, K_pages, V_pages, D)
+    if V.shape != K.shape or heads != H_kv:
+        raise ValueError("K and V must be [T, H_kv, D], with the pools' H_kv")
+    starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
+    table, lens = _table(torch, block_table, kv_lens, device, n)
+    _launch(torch, device, lambda: load_library().kf_kv4_append(
+        K.data_ptr(), V.data_ptr(), _STRIDES[4](*strides), K_pages.data_ptr(), V_pages.data_ptr(), table, starts,
+        lens, n, T, H_kv, D, page_size, block_table.shape[1], num_pages, flags, _raw_stream(torch, stream, device)))
+
+
+def kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, total, D, out=None, *, out_dtype=None,
+             stream=None):
+    """Read the cache back: (K, V) [total, H_kv, D], float16 or ``out_dtype``
+    bfloat16, the values that the codes stand for.
+
+    Sequence b's packed rows ``seq_starts[b] .. seq_starts[b + 1] - 1`` are the last
+    of its ``kv_lens[b]`` keys: with seq_starts the running sum of kv_lens and
+    total = seq_starts[-1], whole contexts for attn_packed.  Rows of an
+    invalid page are zeros; rows outside the sequences are not written.
+    """
+    import torch
+
+    dtype = torch.float16 if out_dtype is None else out_dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("out_dtype must be float16 or bfloat16")
+    device = _check(torch, (("K_pages", K_pages), ("V_pages", V_pages)))
+    num_pages, H_kv, page_size = _pages(torch, K_pages, V_pages, D)
+    starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
+    table, lens = _table(torch, block_table, kv_lens, device, n)
+    shape = (total, H_kv, D)
+    K, V = (_output(torch, x, shape, dtype, device, stream) for x in (out or (None, None)))
+    _launch(torch, device, lambda: load_library().kf_kv4_read(
+        K_pages.data_ptr(), V_pages.data_ptr(), table, starts, lens, K.data_ptr(), V.data_ptr(), n, total, H_kv, D,
+        page_size, block_table.shape[1], num_pages, KF_BF16 if dtype == torch.bfloat16 else 0,
+        _raw_stream(torch, stream, device)))
+    return K, V
+
+
+def kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size, max_pages_per_seq) -> int:
+    """Workspace of attn_decode_kv4 (kf_attn_decode_kv4_workspace_bytes)."""
+    return int(load_library().kf_attn_decode_kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size,
+                                                                 max_pages_per_seq))
+
+
+def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, causal=False, workspace=None,
+                    stream=None, out_dtype=None, return_lse=False):
+    """Decode over the paged 4-bit cache that kv4_append writes.
+
+    Q [B, H_q, q_len, D] float16 or bfloat16, at most 32 query rows per KV head
+    (H_q / H_kv * q_len); the other arguments and the results are those of
+    attn_decode_paged: O [B, H_q, q_len, D] fp32 or ``out_dtype``, (O, LSE) with
+    ``return_lse``.  ``workspace``: a buffer of kv4_workspace_bytes to use
+    instead of a new one.
+    """
+    import torch
+
+    named = (("Q", Q),)
+    device = _check(torch, (*named, ("K_pages", K_pages), ("V_pages", V_pages)))
+    flags = _out_flags(torch, out_dtype, return_lse) | _half_flag(torch, named)
+    if Q.dim() != 4 or not Q.is_contiguous():
+        raise ValueError("Q must be a contiguous [B, H_q, q_len, D] tensor")
+    B, H_q, q_len, D = Q.shape
+    num_pages, H_kv, page_size = _pages(torch, K_pages, V_pages, D)
+    table, lens = _table(torch, block_table, kv_lens, device, B)
+    max_pages = block_table.shape[1]
+    out = _output(torch, out, (B, H_q, q_len, D), out_dtype, device, stream)
+    lse = _new(torch, (B, H_q, q_len), torch.float32, device, stream) if return_lse else None
+    need = kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size, max_pages)
+    workspace, ws_bytes = _workspace(torch, workspace, need, lambda: need, device, stream)
+    if causal:
+        flags |= KF_ATTN_CAUSAL
+    _launch(torch, device, lambda: load_library().kf_attn_decode_kv4(
+        Q.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), table, lens, out.data_ptr(),
+        lse.data_ptr() if return_lse else None, None, B, q_len, H_q, H_kv, D, page_size, max_pages, num_pages, flags,
+        workspace.data_ptr() if workspace is not None else None, ws_bytes, _raw_stream(torch, stream, device)))
+    return (out, lse) if return_lse else out
