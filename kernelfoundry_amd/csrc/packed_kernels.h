@@ -24,12 +24,28 @@ struct PackedParams : AttnParams {  // Q, K, V, O, Mi (LSE), scales, causal, hea
     int n_seqs, tokens_q, tokens_k, ratio;
 };
 
-template <int D, int NW, int RB> struct PackedCfg {
+// A workgroup is NW waves of 32 query rows each; with KS > 1 they form KS
+// groups that take the same rows and a share of the keys each, merged through
+// LDS at the end.
+template <int D, int NW, int KS> struct PackedCfg {
     static constexpr int kThreads = 64 * NW;
-    static constexpr int kRows = 32 * RB * NW;            // query rows per workgroup
-    static constexpr int BC = 32;                         // keys per MFMA tile
-    static constexpr int kStageRows = D >= 256 ? 32 : 64; // keys per LDS stage
-    static constexpr bool kQ1Lds = RB == 2 && D == 128;   // block-1 Q^T read from LDS
+    static constexpr int kRowWaves = NW / KS;             // waves per KV group
+    static constexpr int kRows = 32 * kRowWaves;          // query rows per workgroup
+    static constexpr int BC = 32;                         // keys per MFMA tile and LDS stage
+    // Waves per SIMD that the registers have to allow: three workgroups of 4 waves
+    // a CU at D = 128 (four at D = 64, two at D = 256), two of 8 waves at D = 64.
+    static constexpr int kWavesPerSimd = D == 64 ? 4 : D == 128 && KS == 1 ? 3 : 2;
+    // LDS reads that are issued together, ahead of the MFMAs that need them: K
+    // fragments (16 channels each), and V^T tiles of 32 channels before the
+    // softmax, which does not need them.  As many as the registers leave: with one
+    // or two waves on a SIMD nothing else hides an LDS read's latency (512 queries
+    // against 4096 keys, 32 / 8 heads, D = 128: KS = 1 105.7 -> 96.6 us, KS = 2
+    // 74.3 -> 65.3; full grids lose 1 %).
+    static constexpr int kBatch = D == 256 ? 4 : KS == 1 ? 2 : D / 16;
+    static constexpr int kAhead = D == 256 ? 0 : KS == 1 ? 1 : D / 32;
+    static constexpr bool kOrder = D < 256;               // kept apart from the scheduler
+    // The per-lane LDS offsets of a tile derived from one, for want of registers.
+    static constexpr bool kXorOff = D >= 128;
 };
 
 // One sequence's tokens and keys.
@@ -129,24 +145,72 @@ __device__ __forceinline__ void packed_exp(const f32x16& s, float scale_log2, fl
     p[1] = round8<kBF>(e1);
 }
 
-template <bool kBF, int D, int NW, int RB>
-__global__ __launch_bounds__((PackedCfg<D, NW, RB>::kThreads), 2)
+// Store a wave's 32-row block of O, scaled by inv, as kOut, through kBytes of
+// LDS of the wave's own.  From the accumulators a lane would write 8 or 16 bytes
+// of its row, 32 rows to an instruction; as it lies in LDS the wave writes whole
+// rows, 16 bytes a lane (32 prompts of 128 tokens, 32 / 8 heads, D = 128: 31.6 us -> 22.5).
+// Row r's 16-byte chunk c is at chunk c ^ (r & 15 or fewer), against bank
+// conflicts; as many 32-channel tiles at a time as fit.  `at`: lane r's row in O.
+template <int kOut, int D, int kBytes>
+__device__ __forceinline__ void packed_store(const AttnParams& p, const f32x16 (&o)[D / 32], float inv, char* lds, int at,
+                                             int nrows, int lane) {
+    constexpr int kSize = kOut == kOutF32 ? 4 : 2;
+    constexpr int kTiles = kBytes / (32 * 32 * kSize) < D / 32 ? kBytes / (32 * 32 * kSize) : D / 32;
+    constexpr int kChunks = kTiles * 32 * kSize / 16;     // of a row, at a time
+    constexpr int kMask = (kChunks < 16 ? kChunks : 16) - 1;
+    static_assert(kTiles >= 1 && (D / 32) % kTiles == 0 && (kChunks & kMask) == 0, "whole passes");
+    const int row = lane & 31, g = lane >> 5;
+    char* const mine = lds + row * kChunks * 16;
+#pragma unroll
+    for (int t0 = 0; t0 < D / 32; t0 += kTiles) {
+#pragma unroll
+        for (int td = 0; td < kTiles; ++td)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = 32 * td + 8 * i + 4 * g;    // of the pass
+                const f32x4 v = f32x4{o[t0 + td][4 * i], o[t0 + td][4 * i + 1], o[t0 + td][4 * i + 2],
+                                      o[t0 + td][4 * i + 3]} * inv;
+                if constexpr (kOut == kOutF32) {
+                    *reinterpret_cast<f32x4*>(mine + ((d / 4) ^ (row & kMask)) * 16) = v;
+                } else {
+                    char* const dst = mine + ((d / 8) ^ (row & kMask)) * 16 + g * 8;
+                    if constexpr (kOut == kOutF16)
+                        *reinterpret_cast<f16x4*>(dst) = __builtin_convertvector(v, f16x4);
+                    else
+                        *reinterpret_cast<bf16x4*>(dst) = __builtin_convertvector(v, bf16x4);
+                }
+            }
+        wave_lds_sync();
+        char* const out = reinterpret_cast<char*>(p.O) + t0 * 32 * kSize;
+#pragma unroll 4
+        for (int k = 0; k < kChunks / 2; ++k) {           // 32 kChunks chunks, 64 at a time
+            const int r = (k * 64 + lane) / kChunks, c = (k * 64 + lane) % kChunks;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(lds + (r * kChunks + (c ^ (r & kMask))) * 16);
+            const int to = __shfl(at, r);
+            if (r < nrows) *reinterpret_cast<u32x4*>(out + (size_t)to * (D * kSize) + c * 16) = v;
+        }
+        wave_lds_sync();
+    }
+}
+
+template <bool kBF, int D, int NW, int KS>
+__global__ __launch_bounds__((PackedCfg<D, NW, KS>::kThreads), (PackedCfg<D, NW, KS>::kWavesPerSimd))
 void kf_attn_packed_kernel(PackedParams p) {
-    using Cfg = PackedCfg<D, NW, RB>;
+    using Cfg = PackedCfg<D, NW, KS>;
     using E = Elem<kBF>;
     using X8 = typename E::x8;
     using SW = SwizzleRow<D>;
-    constexpr int BC = Cfg::BC, SR = Cfg::kStageRows, kRows = Cfg::kRows;
+    constexpr int BC = Cfg::BC, kRows = Cfg::kRows;
     constexpr int kRowBytes = D * 2, kChunks = D / 8, kRowsPerInstr = 1024 / kRowBytes;
-    constexpr int kInstr = SR * kRowBytes / 1024;         // LDS-DMA instructions per tensor and stage
-    constexpr int kTensorBytes = SR * kRowBytes;
-    constexpr int kPerWave = 2 * kInstr / NW;
-    static_assert(2 * kInstr % NW == 0 && kInstr % kPerWave == 0, "a wave copies K or V");
+    constexpr int kInstr = BC * kRowBytes / 1024;         // LDS-DMA instructions per tensor and stage
+    constexpr int kTensorBytes = BC * kRowBytes;
+    constexpr int kRowWaves = Cfg::kRowWaves;
+    constexpr int kPerWave = 2 * kInstr / kRowWaves;
+    static_assert(2 * kInstr % kRowWaves == 0 && kInstr % kPerWave == 0, "a wave copies K or V");
     constexpr int kNKK = D / 16, kNTD = D / 32;
-    constexpr bool kQ1Lds = Cfg::kQ1Lds;
-    __shared__ __attribute__((aligned(1024))) char buf0[2 * kTensorBytes];
-    __shared__ __attribute__((aligned(1024))) char buf1[2 * kTensorBytes];
-    __shared__ __attribute__((aligned(256))) char q1_lds[kQ1Lds ? NW * 32 * kRowBytes : 16];
+    constexpr int kBuf = KS * 2 * kTensorBytes;           // a stage of every group
+    __shared__ __attribute__((aligned(1024))) char buf0[kBuf];
+    __shared__ __attribute__((aligned(1024))) char buf1[kBuf];
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -165,56 +229,83 @@ void kf_attn_packed_kernel(PackedParams p) {
     const int ratio = p.ratio, R = sq.qn * ratio, klen = sq.kn;
     const float c = p.scale_log2;
     // Causal: waves w and w + 4 share a SIMD; blocks w and 7 - w.
-    const int wave = (NW == 8 && p.causal && wave_id >= 4) ? 11 - wave_id : wave_id;
+    const int wave = KS > 1 ? wave_id % kRowWaves : (NW == 8 && p.causal && wave_id >= 4) ? 11 - wave_id : wave_id;
+    const int kgrp = KS > 1 ? wave_id / kRowWaves : 0;
     const auto limit = [&](int row) {  // keys that the row sees
         return p.causal ? min(max(row / ratio + klen - sq.qn + 1, 0), klen) : klen;
     };
-    const int r0 = rt * kRows, w0 = r0 + wave * 32 * RB;
+    const int r0 = rt * kRows, w0 = r0 + wave * 32;
     const int blk_lim = limit(min(R, r0 + kRows) - 1);
-    const int wave_min = w0 < R ? limit(w0) : blk_lim;
-    const int wave_max = w0 < R ? limit(min(R, w0 + 32 * RB) - 1) : 0;
-    const int ntiles = (blk_lim + BC - 1) / BC;
-    const int nstages = (blk_lim + SR - 1) / SR;
-    const int nt_w = (wave_max + BC - 1) / BC;            // the wave's tiles; it skips the others
+    // Group kgrp has keys [kv_base, kv_end), as many tiles as every other;
+    // row limits count from kv_base.
+    const int ntiles = ((blk_lim + BC - 1) / BC + KS - 1) / KS;
+    const int kv_base = kgrp * ntiles * BC, kv_end = min(kv_base + ntiles * BC, blk_lim);
+    const auto own = [&](int lim) { return KS > 1 ? min(lim, kv_end) - kv_base : lim; };
+    const int wave_min = own(w0 < R ? limit(w0) : blk_lim);
+    const int wave_max = own(w0 < R ? limit(min(R, w0 + 32) - 1) : 0);
+    const int nt_w = (wave_max + BC - 1) / BC;            // the wave's tiles (none if not positive); it skips the others
 
-    int rows[RB], lim[RB];
-    size_t out_row[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        rows[b] = w0 + 32 * b + (lane & 31);
-        const int rc = min(rows[b], R - 1);               // rows past R compute on it, unstored
-        lim[b] = limit(rc);
-        out_row[b] = ((size_t)(sq.q0 + rc / ratio) * p.heads_kv + hk) * ratio + rc % ratio;
-    }
+    const int lim = own(limit(min(w0 + (lane & 31), R - 1)));
+    const int nrows = R - w0;                             // rows of the wave, if any
+    // The row of O (below tokens_q H_q, an int) of this lane; rows past R
+    // compute on the last one and are not stored.  From an opaque lane, so that
+    // none of it lives across the tiles.
+    auto out_row = [&]() {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const int r = min(w0 + (l & 31), R - 1);
+        return ((sq.q0 + r / ratio) * p.heads_kv + hk) * ratio + r % ratio;
+    };
     if (ntiles == 0) {                                    // no key for any row
+        const int at = out_row();
+        if ((lane & 31) < nrows && kgrp == 0) {
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            if (rows[b] >= R) continue;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) store_out4(p, out_row[b] * D + 8 * i + 4 * g, f32x4{0.f, 0.f, 0.f, 0.f});
-            if (g == 0) store_stats(p, out_row[b], -INFINITY, 0.f);
+            for (int i = 0; i < D / 8; ++i) store_out4(p, (size_t)at * D + 8 * i + 4 * g, f32x4{0.f, 0.f, 0.f, 0.f});
+            if (g == 0) store_stats(p, at, -INFINITY, 0.f);
         }
         return;
     }
 
     const char* Kh = reinterpret_cast<const char*>(p.K + (size_t)sq.k0 * p.k_token + (size_t)hk * p.k_head);
     const char* Vh = reinterpret_cast<const char*>(p.V + (size_t)sq.k0 * p.v_token + (size_t)hk * p.v_head);
-    // LDS-DMA: wave w copies the KiB instructions w kPerWave + i of the
-    // stage, all of K or all of V.  Lane l of one fills row l / kChunks of
+    // LDS-DMA: wave w of a group copies the KiB instructions w kPerWave + i of
+    // its stage, all of K or all of V.  Lane l of one fills row l / kChunks of
     // its rows, physical chunk l % kChunks.
-    const bool is_v = wave_id * kPerWave >= kInstr;
+    const int copier = wave_id % kRowWaves;
+    const bool is_v = copier * kPerWave >= kInstr;
     const char* src = is_v ? Vh : Kh;
-    const size_t row_stride = 2 * (size_t)(is_v ? p.v_token : p.k_token);
-    const int ii0 = wave_id * kPerWave % kInstr;
+    const uint32_t row_stride = 2 * (uint32_t)(is_v ? p.v_token : p.k_token);  // at most 2^25 (the host sees to it)
+    const int ii0 = copier * kPerWave % kInstr;
     const int lr = lane / kChunks;
+    // The swizzle depends on row & 15: the lane offsets of an instruction
+    // within its rows repeat.
+    constexpr int kPeriod = kRowsPerInstr >= 16 ? 1 : 16 / kRowsPerInstr < kPerWave ? 16 / kRowsPerInstr : kPerWave;
+    uint32_t chunk_off[kPeriod];
+#pragma unroll
+    for (int i = 0; i < kPeriod; ++i)
+        chunk_off[i] = (((lane % kChunks) ^ SW::h((ii0 + i) * kRowsPerInstr + lr)) % kChunks) * 16;
     auto issue_stage = [&](char* dst, int kv0) {
         char* d = dst + (is_v ? kTensorBytes : 0) + ii0 * 1024;
+        const int kv = kv_base + kv0 + ii0 * kRowsPerInstr;
+        if (kv_base + kv0 + BC <= klen) {
+            // Whole stage: wave-uniform row base and a 32-bit lane offset,
+            // opaque so that the address stays their sum.
 #pragma unroll
-        for (int i = 0; i < kPerWave; ++i) {
-            const int r = (ii0 + i) * kRowsPerInstr + lr;
-            const int kv = min(kv0 + r, klen - 1);        // rows past the keys re-read the last
-            const char* a = src + (size_t)kv * row_stride + (((lane % kChunks) ^ SW::h(r)) % kChunks) * 16;
-            __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
+            for (int i = 0; i < kPerWave; ++i) {
+                uint32_t off = lr * row_stride + chunk_off[i % kPeriod];
+                asm volatile("" : "+v"(off));
+                const char* a = src + (size_t)(kv + i * kRowsPerInstr) * row_stride + off;
+                __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
+            }
+        } else {
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < kPerWave; ++i) {
+                // Rows past the keys re-read the last one (finite data whose scores are masked).
+                const int row = min(kv + i * kRowsPerInstr + lr, klen - 1);
+                const char* a = src + (size_t)row * row_stride + chunk_off[i % kPeriod];
+                __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
+            }
         }
     };
 
@@ -222,7 +313,8 @@ void kf_attn_packed_kernel(PackedParams p) {
     // (With D >= 128's swizzle the offset of k-step kk is that of the first ^ 32 kk,
     // of V^T tile td ^ 64 td, of its second 8 rows ^ 128 and 8 rows on: derived
     // at each tile where registers for them are short.)
-    constexpr bool kXorOff = D >= 256;
+    constexpr bool kXorOff = Cfg::kXorOff;
+    static_assert(!kXorOff || D >= 128, "XOR offsets use the D >= 128 swizzle");
     int koff[kNKK];
 #pragma unroll
     for (int kk = 0; kk < kNKK; ++kk) {
@@ -242,107 +334,108 @@ void kf_attn_packed_kernel(PackedParams p) {
             }
     }
 
-    issue_stage(buf0, 0);
-    X8 q[RB == 2 && !kQ1Lds ? 2 : 1][kNKK];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        const int rc = min(rows[b], R - 1);
+    char* const b0 = buf0 + kgrp * 2 * kTensorBytes;      // this group's stages
+    char* const b1 = buf1 + kgrp * 2 * kTensorBytes;
+    issue_stage(b0, 0);
+    X8 q[kNKK];
+    {
+        const int rc = min(w0 + (lane & 31), R - 1);
         const uint16_t* Qr = p.Q + (size_t)(sq.q0 + rc / ratio) * p.q_token + (size_t)(hk * ratio + rc % ratio) * p.q_head;
 #pragma unroll
-        for (int kk = 0; kk < kNKK; ++kk) {
-            const X8 v = *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8);
-            if (kQ1Lds && b == 1)
-                *reinterpret_cast<X8*>(q1_lds + wave * 32 * kRowBytes + koff[kk]) = v;
-            else
-                q[b][kk] = v;
-        }
+        for (int kk = 0; kk < kNKK; ++kk) q[kk] = *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8);
     }
-    const char* q1w = q1_lds + wave * 32 * kRowBytes;
 
-    RowState st[RB];
-    f32x16 o[RB][kNTD];
+    RowState st{-INFINITY, -INFINITY, 0.f, -INFINITY};
+    f32x16 o[kNTD];
     const float inv_c = 1.0f / c;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        st[b] = RowState{-INFINITY, -INFINITY, 0.f, -INFINITY};
-#pragma unroll
-        for (int td = 0; td < kNTD; ++td) o[b][td] = f32x16{};
-    }
+    for (int td = 0; td < kNTD; ++td) o[td] = f32x16{};
+    // V^T of 32 channels and 16 keys, V rows at stage + kTensorBytes.
+    auto v_frag = [&](const char* stage, int vb, int td, int jj) {
+        const int vo0 = kXorOff ? vb ^ (64 * td) : voff[td][0];
+        const int vo1 = kXorOff ? (vb ^ (64 * td) ^ 128) + 8 * kRowBytes : voff[td][1];
+        const f16x4 lo = lds_read_tr16(stage + vo0 + jj * 16 * kRowBytes);
+        const f16x4 hi = lds_read_tr16(stage + vo1 + jj * 16 * kRowBytes);
+        return __builtin_bit_cast(X8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
     auto tile = [&](const char* stage, int t) {
         if (t >= nt_w) return;
-        f32x16 s[RB][1];
-#pragma unroll
-        for (int b = 0; b < RB; ++b) s[b][0] = f32x16{};
+        constexpr int kBatch = Cfg::kBatch, kAhead = Cfg::kAhead;
+        static_assert(kNKK % kBatch == 0 && kAhead <= kNTD, "whole batches");
         int kb = koff[0], vb = voff[0][0];
         if constexpr (kXorOff) asm volatile("" : "+v"(kb), "+v"(vb));  // derived per tile
+        f32x16 s[1] = {f32x16{}};
 #pragma unroll
-        for (int kk = 0; kk < kNKK; ++kk) {
-            const X8 kf = *reinterpret_cast<const X8*>(stage + (kXorOff ? kb ^ (32 * kk) : koff[kk]));
+        for (int k0 = 0; k0 < kNKK; k0 += kBatch) {
+            X8 kf[kBatch];
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                if (kQ1Lds && b == 1)
-                    s[b][0] = E::mfma32(kf, *reinterpret_cast<const X8*>(q1w + koff[kk]), s[b][0]);
-                else
-                    s[b][0] = E::mfma32(kf, q[b][kk], s[b][0]);
-            }
+            for (int i = 0; i < kBatch; ++i)
+                kf[i] = *reinterpret_cast<const X8*>(stage + (kXorOff ? kb ^ (32 * (k0 + i)) : koff[k0 + i]));
+            if constexpr (Cfg::kOrder) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) s[0] = E::mfma32(kf[i], q[k0 + i], s[0]);
         }
-        if ((t + 1) * BC > wave_min) {
+        X8 vf[kAhead > 0 ? kAhead : 1][2];
+#pragma unroll
+        for (int td = 0; td < kAhead; ++td)
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) vf[td][jj] = v_frag(stage, vb, td, jj);
+        if constexpr (Cfg::kOrder) __builtin_amdgcn_sched_barrier(0);
+        if ((t + 1) * BC > wave_min) {      // keys that a row does not see -> -inf
             asm volatile("" ::: "memory");  // a branch, not selects in every tile
+            const int lg = lim - t * BC - 4 * g;
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                const int lg = lim[b] - t * BC - 4 * g;
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (8 * (r >> 2) + (r & 3) >= lg) s[b][0][r] = -INFINITY;
-            }
+            for (int r = 0; r < 16; ++r)
+                if (8 * (r >> 2) + (r & 3) >= lg) s[0][r] = -INFINITY;
         }
-        X8 pp[RB][2];
+        X8 pp[2];
+        block_update_max<kNTD>(st, block_rowmax<1>(s), c, inv_c, o);
+        // A row that has seen no key yet keeps m = -inf and must get P = 0, not NaN.
+        packed_exp<kBF>(s[0], c, st.m == -INFINITY ? 0.f : -st.m, pp, st.l);
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            block_update_max<kNTD>(st[b], block_rowmax<1>(s[b]), c, inv_c, o[b]);
-            packed_exp<kBF>(s[b][0], c, st[b].m == -INFINITY ? 0.f : -st[b].m, pp[b], st[b].l);
-        }
+        for (int td = 0; td < kNTD; ++td)
 #pragma unroll
-        for (int td = 0; td < kNTD; ++td) {
-            const int vo0 = kXorOff ? vb ^ (64 * td) : voff[td][0];
-            const int vo1 = kXorOff ? (vb ^ (64 * td) ^ 128) + 8 * kRowBytes : voff[td][1];
-#pragma unroll
-            for (int jj = 0; jj < 2; ++jj) {
-                const f16x4 lo = lds_read_tr16(stage + vo0 + jj * 16 * kRowBytes);
-                const f16x4 hi = lds_read_tr16(stage + vo1 + jj * 16 * kRowBytes);
-                const X8 a = __builtin_bit_cast(X8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int b = 0; b < RB; ++b) o[b][td] = E::mfma32(a, pp[b][jj], o[b][td]);
-            }
-        }
+            for (int jj = 0; jj < 2; ++jj)
+                o[td] = E::mfma32(td < kAhead ? vf[td < kAhead ? td : 0][jj] : v_frag(stage, vb, td, jj), pp[jj], o[td]);
     };
-    constexpr int kSub = SR / BC;
-    for (int js = 0; js < nstages; js += 2) {
+    for (int t0 = 0; t0 < ntiles; t0 += 2) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int j = js + u;
-            if (j >= nstages) break;
-            char* cur = u == 0 ? buf0 : buf1;
-            char* nxt = u == 0 ? buf1 : buf0;
-            // Stage j has landed for every wave; every wave is done with
-            // stage j - 1 (in nxt).
+            const int t = t0 + u;
+            if (t >= ntiles) break;
+            char* cur = u == 0 ? b0 : b1;
+            char* nxt = u == 0 ? b1 : b0;
+            // Stage t has landed for every wave; every wave is done with
+            // stage t - 1 (in nxt).
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (j + 1 < nstages) issue_stage(nxt, (j + 1) * SR);
-            tile(cur, kSub * j);
-            if (kSub == 2 && 2 * j + 1 < ntiles) tile(cur + BC * kRowBytes, 2 * j + 1);
+            if (t + 1 < ntiles) issue_stage(nxt, (t + 1) * BC);
+            tile(cur, t);
         }
     }
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        const float l = sum_xor32(st[b].l);
-        if (rows[b] >= R) continue;
-        const bool empty = !(l > 0.f);                    // causal: no visible key
-        store_o_row_any<D>(p, out_row[b], o[b], empty ? 0.f : 1.0f / l, g);
-        if (g == 0)
-            store_stats(p, out_row[b], st[b].rmax * p.scale,
-                        empty ? 0.f : l * rebase_factor(st[b].m, st[b].rmax, c));
+    if constexpr (KS > 1) {
+        // Merge slot k: 1 KiB of the then free stage buffers.
+        static_assert(kRowWaves * kNTD * 4 * (KS - 1) * 1024 <= 2 * kBuf, "merge slots");
+        __shared__ float merge_ml[2 * NW * 64];
+        const auto slot_base = [&](int k) { return k < kBuf / 1024 ? buf0 + k * 1024 : buf1 + (k * 1024 - kBuf); };
+        merge_kv_groups<D, KS, kRowWaves>(p, st, o, slot_base, merge_ml, wave, kgrp, lane, g, out_row(), 0,
+                                          (lane & 31) < nrows);
+        return;
     }
+    __syncthreads();  // every wave is done with the stages
+    char* const mine = (wave_id < NW / 2 ? buf0 : buf1) + wave_id % (NW / 2) * (2 * kBuf / NW);
+    const float l = sum_xor32(st.l);
+    const bool empty = !(l > 0.f);                        // causal: no visible key
+    const float inv = empty ? 0.f : 1.0f / l;
+    const int at = out_row();
+    if (p.out_dtype == kOutF16)
+        packed_store<kOutF16, D, 2 * kBuf / NW>(p, o, inv, mine, at, nrows, lane);
+    else if (p.out_dtype == kOutBF16)
+        packed_store<kOutBF16, D, 2 * kBuf / NW>(p, o, inv, mine, at, nrows, lane);
+    else
+        packed_store<kOutF32, D, 2 * kBuf / NW>(p, o, inv, mine, at, nrows, lane);
+    if (g == 0 && (lane & 31) < nrows)
+        store_stats(p, at, st.rmax * p.scale, empty ? 0.f : l * rebase_factor(st.m, st.rmax, c));
 }
 
 }  // namespace kf

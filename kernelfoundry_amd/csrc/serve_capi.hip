@@ -66,25 +66,82 @@ int check_attn_flags(int flags) {
 
 // ---- Packed attention. ----
 
-template <bool kBF, int D, int NW, int RB>
+template <bool kBF, int D, int NW, int KS>
 int launch_packed(const kf::PackedParams& prm, long long rows, hipStream_t stream) {
-    using Cfg = kf::PackedCfg<D, NW, RB>;
+    using Cfg = kf::PackedCfg<D, NW, KS>;
     // Tiles of all sequences: a partial one for each at most.
     const long long tiles = rows / Cfg::kRows + std::min<long long>(prm.n_seqs, prm.tokens_q);
     if (tiles * prm.heads_kv > INT_MAX) return KF_ERR_SIZE;
     (void)hipGetLastError();
-    kf::kf_attn_packed_kernel<kBF, D, NW, RB>
+    kf::kf_attn_packed_kernel<kBF, D, NW, KS>
         <<<dim3((unsigned)(tiles * prm.heads_kv)), dim3(Cfg::kThreads), 0, stream>>>(prm);
     return launched();
+}
+
+// The layouts of the packed kernel: 128 rows on 4 waves, of which the CU holds
+// several workgroups, is the cheapest for work enough; KV groups cut the
+// longest chain of key tiles, which bounds a grid that leaves CUs idle.
+// Cost in us of a call of equal sequences, by the averages that the host knows:
+// the longest chain, start + chain per 32-key tile of a KV group, and the grid's
+// work, each workgroup + tile over the device's CUs, joined by their 4-norm.
+// Fitted to 158 shapes a head dimension (1 to 64 sequences of 32 to 8192
+// queries against as many keys or eight times as many; rms 6 to 11 %, and the
+// layout it picks is 1.1 % slower than the best of these at the geometric mean,
+// 14 % at worst).  Always the first layout would be 16 % slower: 1 x 512 queries
+// against 4096 keys, 32 / 8 heads, D = 128, take 96, 58 and 53 us in the three.
+struct PackedLayout {
+    int rows, kv_groups;
+    double start, chain, workgroup, tile;
+};
+constexpr PackedLayout kPacked64[3] = {{128, 1, 3.63, 0.504, 1.734, 0.321},
+                                       {64, 2, 3.78, 0.570, 1.628, 0.362},
+                                       {64, 4, 4.40, 0.784, 3.032, 0.731}};
+constexpr PackedLayout kPacked128[3] = {{128, 1, 4.57, 0.739, 3.546, 0.535},
+                                        {64, 2, 4.73, 0.803, 3.518, 0.652},
+                                        {64, 4, 5.63, 1.235, 6.639, 1.397}};
+constexpr PackedLayout kPacked256[2] = {{128, 1, 6.42, 1.309, 7.246, 1.011}, {128, 2, 9.87, 1.849, 12.804, 2.290}};
+
+int packed_layout(const kf::PackedParams& prm, int D) {
+    const PackedLayout* layouts = D == 64 ? kPacked64 : D == 128 ? kPacked128 : kPacked256;
+    const double queries = std::max(1.0, (double)prm.tokens_q / prm.n_seqs);
+    const double keys = (double)prm.tokens_k / prm.n_seqs;
+    const double cus = current_device_shape().cus;
+    int best = 0;
+    double least = 0.0;
+    for (int i = 0; i < (D == 256 ? 2 : 3); ++i) {
+        const PackedLayout& l = layouts[i];
+        const double tiles = std::ceil(queries * prm.ratio / l.rows);
+        double seen = keys;  // by a row tile, on average
+        if (prm.causal && tiles > 1.0) seen = std::min(keys, keys - (queries - 1.0) / 2 + l.rows / (2.0 * prm.ratio));
+        const double key_tiles = std::max(seen, 0.0) / 32 + 0.5 + (l.kv_groups > 1 ? 0.5 * l.kv_groups : 0.0);
+        const double chain = l.start + l.chain * std::ceil(std::ceil(keys / 32) / l.kv_groups);
+        const double work = prm.n_seqs * (double)prm.heads_kv * tiles *
+                            (l.workgroup + l.tile * key_tiles / l.kv_groups) / cus;
+        const double cost = std::sqrt(std::sqrt(chain * chain * chain * chain + work * work * work * work));
+        if (i == 0 || cost < least) {
+            best = i;
+            least = cost;
+        }
+    }
+    return best;
 }
 
 template <bool kBF>
 int launch_packed_dim(const kf::PackedParams& prm, int D, hipStream_t stream) {
     const long long rows = (long long)prm.tokens_q * prm.ratio;
+    const int layout = packed_layout(prm, D);
     switch (D) {
-        case 64: return launch_packed<kBF, 64, 8, 1>(prm, rows, stream);
-        case 128: return launch_packed<kBF, 128, 8, 1>(prm, rows, stream);
-        default: return launch_packed<kBF, 256, 8, 1>(prm, rows, stream);
+        case 64:
+            return layout == 0   ? launch_packed<kBF, 64, 4, 1>(prm, rows, stream)
+                   : layout == 1 ? launch_packed<kBF, 64, 4, 2>(prm, rows, stream)
+                                 : launch_packed<kBF, 64, 8, 4>(prm, rows, stream);
+        case 128:
+            return layout == 0   ? launch_packed<kBF, 128, 4, 1>(prm, rows, stream)
+                   : layout == 1 ? launch_packed<kBF, 128, 4, 2>(prm, rows, stream)
+                                 : launch_packed<kBF, 128, 8, 4>(prm, rows, stream);
+        default:
+            return layout == 0 ? launch_packed<kBF, 256, 4, 1>(prm, rows, stream)
+                               : launch_packed<kBF, 256, 8, 2>(prm, rows, stream);
     }
 }
 
@@ -229,6 +286,7 @@ int kf_attn_packed(const void* Q, const void* K, const void* V, void* O, float* 
     prm.out_dtype = out_dtype(flags);
     prm.causal = (flags & KF_ATTN_CAUSAL) ? 1 : 0;
     prm.heads_kv = H_kv;
+    prm.n_splits = 1;
     set_scales(prm, D);
     prm.q_token = strides[0];
     prm.q_head = strides[1];
