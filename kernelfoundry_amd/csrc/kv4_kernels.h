@@ -33,6 +33,7 @@ struct Kv4Params {
     int n_seqs, tokens, heads;
     int max_pages, page_shift, num_pages;
     size_t page_bytes;          // of one head
+    int tile;                   // tokens of a workgroup, at most kKv4MaxTile
 };
 
 // Where token t's row lies: its page's bytes and the row in it, or a page of
@@ -42,67 +43,123 @@ struct Kv4Row {
     int page, row;
 };
 __device__ __forceinline__ Kv4Row kv4_row(const Kv4Params& p, int t) {
-    Kv4Row r{-1, 0};
+    Kv4Row r{-1, 0};            // (row 0: readers without a page read the pool's first row)
     if (t < p.starts[0] || t >= p.starts[p.n_seqs]) return r;
     const int b = sequence_of(p.starts, p.n_seqs, t);
     const long long at = (long long)p.kv_lens[b] - p.starts[b + 1] + t;
     if (at < 0 || at >= ((long long)p.max_pages << p.page_shift)) return r;
     const int id = p.block_table[(size_t)b * p.max_pages + (at >> p.page_shift)];
-    if ((unsigned)id < (unsigned)p.num_pages) r.page = id;
+    if ((unsigned)id >= (unsigned)p.num_pages) return r;
+    r.page = id;
     r.row = (int)(at & ((1 << p.page_shift) - 1));
     return r;
 }
 
 constexpr int kKv4Threads = 256;
+constexpr int kKv4MaxTile = 256;   // tokens of a workgroup
 
-// Four neighbouring lanes hold a block, 8 channels (16 bytes in, 4 out) each:
-// loads and stores of a wave are contiguous.  One thread per (token, head,
-// 8 channels); K and V of it by the same thread.
+// Both kernels: a workgroup takes p.tile consecutive tokens.  A thread per token
+// finds its place (a binary search and four dependent loads, once for all heads), then the
+// threads go through the items (token, head, 8 channels of K and of V) side by
+// side, so that a wave's loads and stores are contiguous, kKv4Ahead items
+// of a thread requested together.  Bound by memory: 30000 tokens of 8 heads, D =
+// 128 (156 MB) 38 us written (4.1 TB/s; a copy 4.8), 26 read back (5.9 TB/s);
+// with a thread per item that found its own place 40 and 48.
+constexpr int kKv4Ahead = 2;
+
+// The items of a thread: every 256th of the tile's.
+struct Kv4Item {
+    int t, rest;               // token of the tile; head and chunk in it
+};
+struct Kv4Walk {
+    int per, dt, drest;        // items of a token; a step of 256 items
+    __device__ __forceinline__ explicit Kv4Walk(int per_token)
+        : per(per_token), dt(kKv4Threads / per_token), drest(kKv4Threads % per_token) {}
+    __device__ __forceinline__ Kv4Item first(int tid) const { return Kv4Item{tid / per, tid % per}; }
+    __device__ __forceinline__ void next(Kv4Item& i) const {
+        i.t += dt;
+        i.rest += drest;
+        if (i.rest >= per) {
+            i.rest -= per;
+            ++i.t;
+        }
+    }
+};
+
+// Four neighbouring lanes hold a block, 8 channels (16 bytes in, 4 out) each.
 template <bool kBF, int D>
 __global__ __launch_bounds__(kKv4Threads)
 void kf_kv4_append_kernel(Kv4Params p) {
     using E = Elem<kBF>;
     constexpr int kChunks = D / 8;
-    const int per_token = p.heads * kChunks;
-    const long long item = (long long)blockIdx.x * kKv4Threads + threadIdx.x;
-    const int t = (int)(item / per_token);
-    if (t >= p.tokens) return;
-    const int rest = (int)(item - (long long)t * per_token);
-    const int h = rest / kChunks, c = rest % kChunks;
-    u32x4 raw[2];
+    __shared__ Kv4Row places[kKv4MaxTile];
+    const int tid = threadIdx.x, t0 = blockIdx.x * p.tile, n = min(p.tile, p.tokens - t0);
+    const Kv4Walk walk(p.heads * kChunks);
+    Kv4Item it = walk.first(tid);
+    bool placed = false;
+    // The same trips for all threads, which meet at the barrier in the first.
+    for (int left = (n * walk.per + kKv4Threads - 1) / kKv4Threads; left > 0; left -= kKv4Ahead) {
+        Kv4Item its[kKv4Ahead];
+        u32x4 raw[kKv4Ahead][2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-        raw[s] = *reinterpret_cast<const u32x4*>(p.x[s] + (size_t)t * p.token[s] + (size_t)h * p.head[s] + 8 * c);
-    const Kv4Row at = kv4_row(p, t);
-    if (at.page < 0) return;    // the same for the lanes of a block
+        for (int u = 0; u < kKv4Ahead; ++u) {
+            its[u] = it;
+            const int t = t0 + min(it.t, n - 1), h = it.rest / kChunks, c = it.rest % kChunks;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        // The largest magnitude by the bits: for one sign they order as the
-        // values do, infinity and NaN above all.
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max(raw[s][e] & 0x7fffu, (raw[s][e] >> 16) & 0x7fffu));
-        top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xF, 0xF, false));  // lanes 1 0 3 2
-        top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xF, 0xF, false));  // lanes 2 3 0 1
-        uint32_t exp;
-        if constexpr (kBF) {
-            exp = top >> 7;
-        } else {
-            exp = __float_as_uint((float)__builtin_bit_cast(f16, (uint16_t)top)) >> 23;
+            for (int s = 0; s < 2; ++s)
+                raw[u][s] = *reinterpret_cast<const u32x4*>(p.x[s] + (size_t)t * p.token[s] + (size_t)h * p.head[s] + 8 * c);
+            walk.next(it);
         }
-        const bool bad = top >= E::kExpBits;
-        exp = exp < 3 ? 1 : exp - 2;
-        const float scale = __uint_as_float(exp << 23);
-        const auto v = __builtin_bit_cast(typename E::x8, raw[s]);
-        uint32_t code = 0;
-        code = E::template to_fp4<0>(code, __builtin_shufflevector(v, v, 0, 1), scale);
-        code = E::template to_fp4<1>(code, __builtin_shufflevector(v, v, 2, 3), scale);
-        code = E::template to_fp4<2>(code, __builtin_shufflevector(v, v, 4, 5), scale);
-        code = E::template to_fp4<3>(code, __builtin_shufflevector(v, v, 6, 7), scale);
-        uint8_t* page = p.pages[s] + ((size_t)at.page * p.heads + h) * p.page_bytes;
-        *reinterpret_cast<uint32_t*>(page + (size_t)at.row * (D / 2) + 4 * c) = bad ? 0u : code;
-        if (c % 4 == 0)
-            page[((size_t)(D / 2) << p.page_shift) + (size_t)at.row * (D / 32) + c / 4] = bad ? 255 : exp;
+        if (!placed) {
+            if (tid < n) places[tid] = kv4_row(p, t0 + tid);
+            __syncthreads();
+            placed = true;
+        }
+#pragma unroll
+        for (int u = 0; u < kKv4Ahead; ++u) {
+            const Kv4Row at = places[min(its[u].t, n - 1)];
+            if (its[u].t >= n || at.page < 0) continue;    // the same for the lanes of a block
+            const int h = its[u].rest / kChunks, c = its[u].rest % kChunks;
+            const size_t base = ((size_t)at.page * p.heads + h) * p.page_bytes;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                // The largest magnitude by the bits: for one sign they order as the
+                // values do, infinity and NaN above all.
+                const u32x4 x = raw[u][s];
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+                top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xF, 0xF, false));  // lanes 1 0 3 2
+                top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xF, 0xF, false));  // lanes 2 3 0 1
+                uint32_t exp;
+                if constexpr (kBF) {
+                    exp = top >> 7;
+                } else {
+                    exp = __float_as_uint((float)__builtin_bit_cast(f16, (uint16_t)top)) >> 23;
+                }
+                const bool bad = top >= E::kExpBits;
+                exp = exp < 3 ? 1 : exp - 2;
+                const float scale = __uint_as_float(exp << 23);
+                const auto v = __builtin_bit_cast(typename E::x8, x);
+                uint32_t code = 0;
+                code = E::template to_fp4<0>(code, __builtin_shufflevector(v, v, 0, 1), scale);
+                code = E::template to_fp4<1>(code, __builtin_shufflevector(v, v, 2, 3), scale);
+                code = E::template to_fp4<2>(code, __builtin_shufflevector(v, v, 4, 5), scale);
+                code = E::template to_fp4<3>(code, __builtin_shufflevector(v, v, 6, 7), scale);
+                uint8_t* page = p.pages[s] + base;
+                *reinterpret_cast<uint32_t*>(page + (size_t)at.row * (D / 2) + 4 * c) = bad ? 0u : code;
+                // The scales of up to four blocks (16 lanes) by one lane.
+                uint32_t bytes = bad ? 255 : exp;
+                bytes |= (uint32_t)__builtin_amdgcn_mov_dpp((int)bytes, 0x104, 0xF, 0xF, true) << 8;  // of lane + 4
+                uint8_t* const scales = page + ((size_t)(D / 2) << p.page_shift) + (size_t)at.row * (D / 32) + c / 4;
+                if constexpr (D == 64) {
+                    if (c == 0) *reinterpret_cast<uint16_t*>(scales) = (uint16_t)bytes;
+                } else {
+                    bytes |= (uint32_t)__builtin_amdgcn_mov_dpp((int)bytes, 0x108, 0xF, 0xF, true) << 16;  // of lane + 8
+                    if (c % 16 == 0) *reinterpret_cast<uint32_t*>(scales) = bytes;
+                }
+            }
+        }
     }
 }
 
@@ -114,29 +171,47 @@ __global__ __launch_bounds__(kKv4Threads)
 void kf_kv4_read_kernel(Kv4Params p) {
     using X8 = typename Elem<kBF>::x8;
     constexpr int kChunks = D / 8;
-    const int per_token = p.heads * kChunks;
-    const long long item = (long long)blockIdx.x * kKv4Threads + threadIdx.x;
-    const int t = (int)(item / per_token);
-    if (t >= p.tokens || t < p.starts[0] || t >= p.starts[p.n_seqs]) return;
-    const int rest = (int)(item - (long long)t * per_token);
-    const int h = rest / kChunks, c = rest % kChunks;
-    const Kv4Row at = kv4_row(p, t);
+    __shared__ Kv4Row places[kKv4MaxTile];
+    const int tid = threadIdx.x, t0 = blockIdx.x * p.tile, n = min(p.tile, p.tokens - t0);
+    const int begin = p.starts[0], end = p.starts[p.n_seqs];
+    if (tid < n) places[tid] = kv4_row(p, t0 + tid);
+    const Kv4Walk walk(p.heads * kChunks);
+    Kv4Item it = walk.first(tid);
+    __syncthreads();
+    while (it.t < n) {
+        Kv4Item its[kKv4Ahead];
+        uint32_t code[kKv4Ahead][2], exp[kKv4Ahead][2];
+        bool ok[kKv4Ahead];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        X8 v = {};
-        if (at.page >= 0) {
-            const uint8_t* page = p.pages[s] + ((size_t)at.page * p.heads + h) * p.page_bytes;
-            const uint32_t code = *reinterpret_cast<const uint32_t*>(page + (size_t)at.row * (D / 2) + 4 * c);
-            const uint32_t exp = page[((size_t)(D / 2) << p.page_shift) + (size_t)at.row * (D / 32) + c / 4];
-            const float scale = exp == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(exp << 23);
-            v = from_fp4x8<kBF>(code, scale);
-            if (exp == 255) {
-                // NaN by its bits, whatever the conversion makes of the scale.
+        for (int u = 0; u < kKv4Ahead; ++u) {
+            its[u] = it;
+            const Kv4Row at = places[min(it.t, n - 1)];
+            const int h = it.rest / kChunks, c = it.rest % kChunks;
+            ok[u] = at.page >= 0;
+            // (A token without a page reads the pool's first row.)
+            const size_t base = ((size_t)max(at.page, 0) * p.heads + h) * p.page_bytes;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint8_t* page = p.pages[s] + base;
+                code[u][s] = *reinterpret_cast<const uint32_t*>(page + (size_t)at.row * (D / 2) + 4 * c);
+                exp[u][s] = page[((size_t)(D / 2) << p.page_shift) + (size_t)at.row * (D / 32) + c / 4];
+            }
+            walk.next(it);
+        }
+#pragma unroll
+        for (int u = 0; u < kKv4Ahead; ++u) {
+            const int t = t0 + its[u].t;
+            if (its[u].t >= n || t < begin || t >= end) continue;
+            const int h = its[u].rest / kChunks, c = its[u].rest % kChunks;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                u32x4 v = __builtin_bit_cast(u32x4, from_fp4x8<kBF>(code[u][s], __uint_as_float(exp[u][s] << 23)));
                 const uint32_t nan = kBF ? 0x7fc07fc0u : 0x7e007e00u;
-                v = __builtin_bit_cast(X8, u32x4{nan, nan, nan, nan});
+                if (exp[u][s] == 255) v = u32x4{nan, nan, nan, nan};
+                if (!ok[u]) v = u32x4{0u, 0u, 0u, 0u};
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p.y[s] + ((size_t)t * p.heads + h) * D + 8 * c));
             }
         }
-        *reinterpret_cast<X8*>(p.y[s] + ((size_t)t * p.heads + h) * D + 8 * c) = v;
     }
 }
 
