@@ -31,61 +31,75 @@ KF_ROPE_INTERLEAVED = 32
 _STRIDES = {n: ctypes.c_int64 * n for n in (4, 6, 8)}
 
 
-def _check(torch, named):
-    """The tensors' device after checking that all are on one GPU."""
-    first = named[0][1]
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError(f"{named[0][0]} must be a GPU tensor")
-    grad = torch.is_grad_enabled()
-    for name, t in named:
-        if t.device != device:
-            raise ValueError(f"{name} must be on {device}")
-        if grad and t.requires_grad:
+# The checks below run on every call, and a small call's time is the host's:
+# they compare by device index and identity, and look for words only when
+# something is wrong.
+def _gpu(torch, names, *tensors):
+    """The device of tensors that are all on one GPU and record no gradient."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0 or t.requires_grad:
+            break
+    else:
+        return tensors[0].device
+    for name, t in zip(names, tensors):
+        if t.get_device() != index or index < 0:
+            where = tensors[0].device if index >= 0 else "a GPU"
+            raise ValueError(f"{name} must be a GPU tensor, on {where}")
+        if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad, but there is no backward pass: call under torch.no_grad()")
-    return device
+    return tensors[0].device
 
 
-def _half_flag(torch, named):
+def _half(torch, names, *tensors):
     """KF_BF16 or 0 by the one 16-bit type of the tensors."""
-    dtype = named[0][1].dtype
-    if dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"{named[0][0]} must be float16 or bfloat16")
-    for name, t in named:
-        if t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype}, as {named[0][0]} is")
-    return KF_BF16 if dtype == torch.bfloat16 else 0
+    dtype = tensors[0].dtype
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise TypeError(f"{names[0]} must be float16 or bfloat16")
+    for t in tensors:
+        if t.dtype is not dtype:
+            raise TypeError(f"{' and '.join(names)} must be of one type")
+    return KF_BF16 if dtype is torch.bfloat16 else 0
 
 
-def _heads3(name, t):
-    """A [tokens, heads, D] tensor's token and head strides: D contiguous."""
+def _heads(name, t):
+    """A [tokens, heads, D] tensor's token and head strides (0 where there is one
+    token or head, whose stride may be anything): D contiguous."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, D]")
-    s = t.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8:
-        raise ValueError(f"{name}: the channels must be contiguous, and token and head strides multiples of 8")
-    return s[0], s[1]
+    token, head, channel = t.stride()
+    if channel != 1 or token % 8 or head % 8:
+        tokens, heads, D = t.shape
+        token, head = token if tokens > 1 else 0, head if heads > 1 else 0
+        if (channel != 1 and D > 1) or token % 8 or head % 8:
+            raise ValueError(f"{name}: the channels must be contiguous, token and head strides multiples of 8")
+    return token, head
 
 
 def _ints(torch, name, t, device, shape):
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}")
+    if t.dtype is not torch.int32 or t.get_device() != device.index or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}")
     return t.data_ptr()
 
 
 def _starts(torch, name, t, device):
     if t.dim() != 1 or t.shape[0] < 2:
         raise ValueError(f"{name} must be [sequences + 1]")
-    return _ints(torch, name, t, device, (t.shape[0],))
+    return _ints(torch, name, t, device, t.shape)
 
 
-def _launch(torch, device, call):
-    """call() with `device` current: its streams are the current device's."""
+def _like(torch, t, shape, dtype, stream):
+    """_new on t's device (new_empty takes less time than empty)."""
+    return t.new_empty(shape, dtype=dtype) if stream is None else _new(torch, shape, dtype, t.device, stream)
+
+
+def _launch(torch, device, stream, entry, *args):
+    """entry(*args, stream) with `device` current: its streams are the current device's."""
     if device.index == torch.cuda.current_device():
-        st = call()
+        st = entry(*args, _raw_stream(torch, stream, device))
     else:
         with torch.cuda.device(device):
-            st = call()
+            st = entry(*args, _raw_stream(torch, stream, device))
     if st != KF_OK:
         msg = status_string(st)
         if st == KF_ERR_HIP:
@@ -109,28 +123,26 @@ def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, 
     """
     import torch
 
-    named = (("Q", Q), ("K", K), ("V", V))
-    device = _check(torch, named)
-    flags = _out_flags(torch, out_dtype, return_lse) | _half_flag(torch, named)
-    strides = [s for name, t in named for s in _heads3(name, t)]
+    device = _gpu(torch, "QKV", Q, K, V)
+    flags = _out_flags(torch, out_dtype, return_lse) | _half(torch, "QKV", Q, K, V)
+    strides = _STRIDES[6](*_heads("Q", Q), *_heads("K", K), *_heads("V", V))
     T, H_q, D = Q.shape
     T_kv, H_kv, Dk = K.shape
     if V.shape != K.shape or Dk != D:
         raise ValueError("K and V must be [T_kv, H_kv, D], with Q's D")
-    if kv_starts is None:
-        kv_starts = seq_starts
-    starts = _starts(torch, "seq_starts", seq_starts, device)
-    if kv_starts.shape != seq_starts.shape:
-        raise ValueError("kv_starts and seq_starts must have one length")
-    kstarts = _ints(torch, "kv_starts", kv_starts, device, tuple(kv_starts.shape))
-    out = _output(torch, out, (T, H_q, D), out_dtype, device, stream)
-    lse = _new(torch, (T, H_q), torch.float32, device, stream) if return_lse else None
+    starts = kstarts = _starts(torch, "seq_starts", seq_starts, device)
+    if kv_starts is not None:
+        kstarts = _ints(torch, "kv_starts", kv_starts, device, seq_starts.shape)
+    if out is None:
+        out = _like(torch, Q, (T, H_q, D), out_dtype or torch.float32, stream)
+    else:
+        out = _output(torch, out, (T, H_q, D), out_dtype, device, stream)
+    lse = _like(torch, Q, (T, H_q), torch.float32, stream) if return_lse else None
     if causal:
         flags |= KF_ATTN_CAUSAL
-    _launch(torch, device, lambda: load_library().kf_attn_packed(
-        Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, None,
-        _STRIDES[6](*strides), starts, kstarts, seq_starts.shape[0] - 1, T, T_kv, H_q, H_kv, D, flags,
-        _raw_stream(torch, stream, device)))
+    _launch(torch, device, stream, load_library().kf_attn_packed,
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, None,
+            strides, starts, kstarts, seq_starts.shape[0] - 1, T, T_kv, H_q, H_kv, D, flags)
     return (out, lse) if return_lse else out
 
 
@@ -193,45 +205,51 @@ def qk_norm_rope(Q, K, positions, freqs, out=None, *, q_weight=None, k_weight=No
     """
     import torch
 
-    named = [("Q", Q), ("K", K)]
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            if w.dim() != 1 or w.shape[0] != Q.shape[-1] or not w.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous tensor of D elements")
-            named.append((name, w))
-    device = _check(torch, named)
-    flags = _half_flag(torch, named) | (KF_ROPE_INTERLEAVED if interleaved else 0)
-    strides = [*_heads3("Q", Q), *_heads3("K", K)]
+    device = _gpu(torch, "QK", Q, K)
+    flags = _half(torch, "QK", Q, K) | (KF_ROPE_INTERLEAVED if interleaved else 0)
+    strides = (*_heads("Q", Q), *_heads("K", K))
     T, H_q, D = Q.shape
-    if K.shape[0] != T or K.shape[2] != D:
+    T_k, H_kv, Dk = K.shape
+    if T_k != T or Dk != D:
         raise ValueError("K must be [T, H_kv, D], with Q's T and D")
-    H_kv = K.shape[1]
-    rot = pos = frq = 0
+    wq = wk = pos = frq = None
+    if q_weight is not None:
+        wq = _weight(torch, "q_weight", q_weight, Q, D)
+    if k_weight is not None:
+        wk = _weight(torch, "k_weight", k_weight, Q, D)
+    rot = 0
     if freqs is not None:
-        if freqs.dtype != torch.float64 or freqs.device != device or freqs.dim() != 1 or not freqs.is_contiguous():
+        if freqs.dtype is not torch.float64 or freqs.get_device() != device.index or freqs.dim() != 1 \
+                or not freqs.is_contiguous():
             raise ValueError(f"freqs must be a contiguous float64 [rot / 2] tensor on {device}")
         rot, frq = 2 * freqs.shape[0], freqs.data_ptr()
         if positions is None:
             raise ValueError("freqs without positions")
         pos = _ints(torch, "positions", positions, device, (T,))
     if out is None:
-        out = (_new(torch, (T, H_q, D), Q.dtype, device, stream), _new(torch, (T, H_kv, D), Q.dtype, device, stream))
+        out = (_like(torch, Q, (T, H_q, D), Q.dtype, stream), _like(torch, Q, (T, H_kv, D), Q.dtype, stream))
         strides += (H_q * D, D, H_kv * D, D)
     else:
         for name, y, x in (("out[0]", out[0], Q), ("out[1]", out[1], K)):
             if y.shape != x.shape or y.dtype != x.dtype or y.device != device:
                 raise ValueError(f"{name} must have the shape, type and device of its input")
-            s = _heads3(name, y)
             in_place = y.data_ptr() == x.data_ptr() and y.stride() == x.stride()
             if not (in_place or y.is_contiguous()):
                 raise ValueError(f"{name} must be contiguous, or its input itself")
-            strides += s
-    _launch(torch, device, lambda: load_library().kf_qk_norm_rope(
-        Q.data_ptr(), K.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), _STRIDES[8](*strides),
-        q_weight.data_ptr() if q_weight is not None else None,
-        k_weight.data_ptr() if k_weight is not None else None, pos or None, frq or None, T, H_q, H_kv, D, rot, eps,
-        scale, flags, _raw_stream(torch, stream, device)))
+            strides += _heads(name, y)
+    _launch(torch, device, stream, load_library().kf_qk_norm_rope,
+            Q.data_ptr(), K.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), _STRIDES[8](*strides), wq, wk, pos, frq,
+            T, H_q, H_kv, D, rot, eps, scale, flags)
     return out
+
+
+def _weight(torch, name, w, Q, D):
+    if w.dtype is not Q.dtype or w.requires_grad or w.get_device() != Q.get_device():
+        _gpu(torch, ("Q", name), Q, w)
+        _half(torch, ("Q", name), Q, w)
+    if w.shape != (D,) or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of D elements")
+    return w.data_ptr()
 
 
 def kv4_page_bytes(page_size, D) -> int:
@@ -247,9 +265,9 @@ def _pages(torch, K_pages, V_pages, D):
     """num_pages, H_kv and page_size of a pair of pools."""
     if K_pages.dim() != 3 or K_pages.shape != V_pages.shape:
         raise ValueError("K_pages and V_pages must be [num_pages, H_kv, kv4_page_bytes(page_size, D)]")
-    for t in (K_pages, V_pages):
-        if t.dtype != torch.uint8 or not t.is_contiguous():
-            raise ValueError("K_pages and V_pages must be contiguous uint8 tensors")
+    if K_pages.dtype is not torch.uint8 or V_pages.dtype is not torch.uint8 or not K_pages.is_contiguous() \
+            or not V_pages.is_contiguous():
+        raise ValueError("K_pages and V_pages must be contiguous uint8 tensors")
     n, H_kv, nbytes = K_pages.shape
     page_size, rest = divmod(nbytes * 32, 17 * D) if D > 0 else (0, 1)
     if rest:
@@ -260,7 +278,7 @@ def _pages(torch, K_pages, V_pages, D):
 def _table(torch, block_table, kv_lens, device, n_seqs):
     if block_table.dim() != 2 or block_table.shape[0] != n_seqs:
         raise ValueError("block_table must be [sequences, max_pages_per_seq]")
-    return (_ints(torch, "block_table", block_table, device, tuple(block_table.shape)),
+    return (_ints(torch, "block_table", block_table, device, block_table.shape),
             _ints(torch, "kv_lens", kv_lens, device, (n_seqs,)))
 
 
@@ -275,19 +293,18 @@ def kv4_append(K, V, K_pages, V_pages, block_table, seq_starts, kv_lens, *, stre
     """
     import torch
 
-    named = (("K", K), ("V", V))
-    device = _check(torch, (*named, ("K_pages", K_pages), ("V_pages", V_pages)))
-    flags = _half_flag(torch, named)
-    strides = [s for name, t in named for s in _heads3(name, t)]
+    device = _gpu(torch, ("K", "V", "K_pages", "V_pages"), K, V, K_pages, V_pages)
+    flags = _half(torch, "KV", K, V)
+    strides = _STRIDES[4](*_heads("K", K), *_heads("V", V))
     T, H_kv, D = K.shape
     num_pages, heads, page_size = _pages(torch, K_pages, V_pages, D)
     if V.shape != K.shape or heads != H_kv:
         raise ValueError("K and V must be [T, H_kv, D], with the pools' H_kv")
     starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
     table, lens = _table(torch, block_table, kv_lens, device, n)
-    _launch(torch, device, lambda: load_library().kf_kv4_append(
-        K.data_ptr(), V.data_ptr(), _STRIDES[4](*strides), K_pages.data_ptr(), V_pages.data_ptr(), table, starts,
-        lens, n, T, H_kv, D, page_size, block_table.shape[1], num_pages, flags, _raw_stream(torch, stream, device)))
+    _launch(torch, device, stream, load_library().kf_kv4_append,
+            K.data_ptr(), V.data_ptr(), strides, K_pages.data_ptr(), V_pages.data_ptr(), table, starts, lens, n, T,
+            H_kv, D, page_size, block_table.shape[1], num_pages, flags)
 
 
 def kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, total, D, out=None, *, out_dtype=None,
@@ -305,16 +322,18 @@ def kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, total, D, out=N
     dtype = torch.float16 if out_dtype is None else out_dtype
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("out_dtype must be float16 or bfloat16")
-    device = _check(torch, (("K_pages", K_pages), ("V_pages", V_pages)))
+    device = _gpu(torch, ("K_pages", "V_pages"), K_pages, V_pages)
     num_pages, H_kv, page_size = _pages(torch, K_pages, V_pages, D)
     starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
     table, lens = _table(torch, block_table, kv_lens, device, n)
     shape = (total, H_kv, D)
-    K, V = (_output(torch, x, shape, dtype, device, stream) for x in (out or (None, None)))
-    _launch(torch, device, lambda: load_library().kf_kv4_read(
-        K_pages.data_ptr(), V_pages.data_ptr(), table, starts, lens, K.data_ptr(), V.data_ptr(), n, total, H_kv, D,
-        page_size, block_table.shape[1], num_pages, KF_BF16 if dtype == torch.bfloat16 else 0,
-        _raw_stream(torch, stream, device)))
+    if out is None:
+        K, V = _like(torch, K_pages, shape, dtype, stream), _like(torch, K_pages, shape, dtype, stream)
+    else:
+        K, V = (_output(torch, x, shape, dtype, device, stream) for x in out)
+    _launch(torch, device, stream, load_library().kf_kv4_read,
+            K_pages.data_ptr(), V_pages.data_ptr(), table, starts, lens, K.data_ptr(), V.data_ptr(), n, total, H_kv, D,
+            page_size, block_table.shape[1], num_pages, KF_BF16 if dtype is torch.bfloat16 else 0)
     return K, V
 
 
@@ -336,23 +355,28 @@ def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, caus
     """
     import torch
 
-    named = (("Q", Q),)
-    device = _check(torch, (*named, ("K_pages", K_pages), ("V_pages", V_pages)))
-    flags = _out_flags(torch, out_dtype, return_lse) | _half_flag(torch, named)
+    device = _gpu(torch, ("Q", "K_pages", "V_pages"), Q, K_pages, V_pages)
+    flags = _out_flags(torch, out_dtype, return_lse) | _half(torch, "Q", Q)
     if Q.dim() != 4 or not Q.is_contiguous():
         raise ValueError("Q must be a contiguous [B, H_q, q_len, D] tensor")
     B, H_q, q_len, D = Q.shape
     num_pages, H_kv, page_size = _pages(torch, K_pages, V_pages, D)
     table, lens = _table(torch, block_table, kv_lens, device, B)
     max_pages = block_table.shape[1]
-    out = _output(torch, out, (B, H_q, q_len, D), out_dtype, device, stream)
-    lse = _new(torch, (B, H_q, q_len), torch.float32, device, stream) if return_lse else None
+    if out is None:
+        out = _like(torch, Q, Q.shape, out_dtype or torch.float32, stream)
+    else:
+        out = _output(torch, out, (B, H_q, q_len, D), out_dtype, device, stream)
+    lse = _like(torch, Q, (B, H_q, q_len), torch.float32, stream) if return_lse else None
     need = kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size, max_pages)
-    workspace, ws_bytes = _workspace(torch, workspace, need, lambda: need, device, stream)
+    if workspace is None and need:
+        workspace = _like(torch, Q, need, torch.uint8, stream)
+    else:
+        workspace, need = _workspace(torch, workspace, need, lambda: need, device, stream)
     if causal:
         flags |= KF_ATTN_CAUSAL
-    _launch(torch, device, lambda: load_library().kf_attn_decode_kv4(
-        Q.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), table, lens, out.data_ptr(),
-        lse.data_ptr() if return_lse else None, None, B, q_len, H_q, H_kv, D, page_size, max_pages, num_pages, flags,
-        workspace.data_ptr() if workspace is not None else None, ws_bytes, _raw_stream(torch, stream, device)))
+    _launch(torch, device, stream, load_library().kf_attn_decode_kv4,
+            Q.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), table, lens, out.data_ptr(),
+            lse.data_ptr() if return_lse else None, None, B, q_len, H_q, H_kv, D, page_size, max_pages, num_pages,
+            flags, workspace.data_ptr() if workspace is not None else None, need)
     return (out, lse) if return_lse else out
