@@ -270,8 +270,9 @@ int kf_attn_decode_paged(const void* Q, const void* K_pages, const void* V_pages
  *
  * Q [tokens_q, H_q, D], K and V [tokens_kv, H_kv, D], fp16 (bf16 with
  *   KF_BF16), D = 64, 128 or 256.  `strides`: NULL (contiguous), or six host
- *   values, token and head strides of Q, K and V in elements, multiples of 8;
- *   the D channels of a head are contiguous.
+ *   values, token and head strides of Q, K and V in elements, multiples of 8,
+ *   K's and V's token strides at most 2^28; the D channels of a head are
+ *   contiguous.
  * q_starts, kv_starts: device int [n_seqs + 1], not decreasing: sequence b has
  *   the queries q_starts[b] .. q_starts[b + 1] - 1 and the keys kv_starts[b] ..
  *   kv_starts[b + 1] - 1; either may be empty.  The same array for prompts;
@@ -283,7 +284,10 @@ int kf_attn_decode_paged(const void* Q, const void* K_pages, const void* V_pages
  * O [tokens_q, H_q, D] contiguous, fp32 or by KF_ATTN_OUT_F16 / _BF16; row_max,
  *   row_sumexp [tokens_q, H_q], optional, as in kf_attn_fwd_ex (KF_ATTN_LSE).
  *   Rows of tokens outside the sequences are left as they were.
- * No workspace. */
+ * What tokens outside the sequences and other sequences hold does not matter; a
+ * NaN or an infinity among a sequence's own keys or values may reach any row of
+ * that sequence, also one that does not see it.
+ * tokens_q, tokens_kv and n_seqs are positive.  No workspace. */
 int kf_attn_packed(const void* Q, const void* K, const void* V, void* O,
                    float* row_max, float* row_sumexp, const int64_t* strides,
                    const int* q_starts, const int* kv_starts,

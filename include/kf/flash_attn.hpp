@@ -19,6 +19,10 @@
 //       the same over kf_attn_fwd_ex / kf_attn_decode_paged (causal masking,
 //       per-sequence key counts, paged K/V, fp16 / bf16 O, LSE), which have
 //       no counterpart in the reference.
+//
+//   kf::attn_packed(...), kf::qk_norm_rope(...), kf::kv4_append(...),
+//   kf::kv4_read(...), kf::attn_decode_kv4(...)
+//       the same over the serving entry points of kf/attn.h.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -266,6 +270,63 @@ inline hipError_t attn_decode_paged(const uint16_t* Q, const uint16_t* K_pages,
         return kf_attn_decode_paged(Q, K_pages, V_pages, block_table, kv_lens, O, Mi, Li, B, q_len,
                                     H_q, H_kv, D, page_size, max_pages_per_seq, num_pages, flags,
                                     ws, ws_bytes, static_cast<void*>(stream));
+    });
+}
+
+// kf_attn_packed: packed sequences of different lengths (no workspace).
+inline hipError_t attn_packed(const uint16_t* Q, const uint16_t* K, const uint16_t* V, void* O,
+                              const int64_t* strides, const int* q_starts, const int* kv_starts,
+                              int n_seqs, int tokens_q, int tokens_kv, int H_q, int H_kv, int D,
+                              int flags, hipStream_t stream, float* Mi = nullptr,
+                              float* Li = nullptr) {
+    return status_to_hip(kf_attn_packed(Q, K, V, O, Mi, Li, strides, q_starts, kv_starts, n_seqs,
+                                        tokens_q, tokens_kv, H_q, H_kv, D, flags,
+                                        static_cast<void*>(stream)));
+}
+
+// kf_qk_norm_rope: head norms and rotary positions.
+inline hipError_t qk_norm_rope(const uint16_t* Q, const uint16_t* K, uint16_t* Q_out,
+                               uint16_t* K_out, const int64_t* strides, const uint16_t* q_weight,
+                               const uint16_t* k_weight, const int* positions, const double* freqs,
+                               int tokens, int H_q, int H_kv, int D, int rot, float eps,
+                               float scale, int flags, hipStream_t stream) {
+    return status_to_hip(kf_qk_norm_rope(Q, K, Q_out, K_out, strides, q_weight, k_weight, positions,
+                                         freqs, tokens, H_q, H_kv, D, rot, eps, scale, flags,
+                                         static_cast<void*>(stream)));
+}
+
+// kf_kv4_append and kf_kv4_read: the paged 4-bit cache.
+inline hipError_t kv4_append(const uint16_t* K, const uint16_t* V, const int64_t* strides,
+                             uint8_t* K_pages, uint8_t* V_pages, const int* block_table,
+                             const int* seq_starts, const int* kv_lens, int n_seqs, int tokens,
+                             int H_kv, int D, int page_size, int max_pages_per_seq, int num_pages,
+                             int flags, hipStream_t stream) {
+    return status_to_hip(kf_kv4_append(K, V, strides, K_pages, V_pages, block_table, seq_starts,
+                                       kv_lens, n_seqs, tokens, H_kv, D, page_size,
+                                       max_pages_per_seq, num_pages, flags,
+                                       static_cast<void*>(stream)));
+}
+inline hipError_t kv4_read(const uint8_t* K_pages, const uint8_t* V_pages, const int* block_table,
+                           const int* seq_starts, const int* kv_lens, uint16_t* K, uint16_t* V,
+                           int n_seqs, int tokens, int H_kv, int D, int page_size,
+                           int max_pages_per_seq, int num_pages, int flags, hipStream_t stream) {
+    return status_to_hip(kf_kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, K, V,
+                                     n_seqs, tokens, H_kv, D, page_size, max_pages_per_seq,
+                                     num_pages, flags, static_cast<void*>(stream)));
+}
+
+// kf_attn_decode_kv4 with the per-thread cached workspace, which it cannot do without.
+inline hipError_t attn_decode_kv4(const uint16_t* Q, const uint8_t* K_pages, const uint8_t* V_pages,
+                                  const int* block_table, const int* kv_lens, void* O, int B,
+                                  int q_len, int H_q, int H_kv, int D, int page_size,
+                                  int max_pages_per_seq, int num_pages, int flags,
+                                  hipStream_t stream, float* Mi = nullptr, float* Li = nullptr) {
+    const size_t need = kf_attn_decode_kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size,
+                                                           max_pages_per_seq);
+    return with_workspace(stream, need, [&] { return need; }, [&](void* ws, size_t ws_bytes) {
+        return kf_attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, O, Mi, Li, B, q_len,
+                                  H_q, H_kv, D, page_size, max_pages_per_seq, num_pages, flags, ws,
+                                  ws_bytes, static_cast<void*>(stream));
     });
 }
 

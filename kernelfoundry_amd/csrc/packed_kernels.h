@@ -274,7 +274,7 @@ void kf_attn_packed_kernel(PackedParams p) {
     const int copier = wave_id % kRowWaves;
     const bool is_v = copier * kPerWave >= kInstr;
     const char* src = is_v ? Vh : Kh;
-    const uint32_t row_stride = 2 * (uint32_t)(is_v ? p.v_token : p.k_token);  // at most 2^25 (the host sees to it)
+    const uint32_t row_stride = 2 * (uint32_t)(is_v ? p.v_token : p.k_token);  // at most 2^29 (the host sees to it)
     const int ii0 = copier * kPerWave % kInstr;
     const int lr = lane / kChunks;
     // The swizzle depends on row & 15: the lane offsets of an instruction

@@ -20,6 +20,8 @@ using namespace kf_capi;
 
 bool aligned4(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 3u) == 0; }
 
+constexpr int64_t kMaxKvTokenStride = 1 << 28;
+
 // Strides of 16-byte chunks, not negative; n of them.
 int check_strides(const int64_t* s, int n) {
     for (int i = 0; i < n; ++i) {
@@ -280,6 +282,8 @@ int kf_attn_packed(const void* Q, const void* K, const void* V, void* O, float* 
     const int64_t packed[6] = {(int64_t)H_q * D, D, (int64_t)H_kv * D, D, (int64_t)H_kv * D, D};
     if (!strides) strides = packed;
     if (const int st = check_strides(strides, 6); st != KF_OK) return st;
+    // (A lane's offset within an LDS-DMA instruction, up to 7 rows, has 32 bits.)
+    if (strides[2] > kMaxKvTokenStride || strides[4] > kMaxKvTokenStride) return KF_ERR_SIZE;
     kf::PackedParams prm{};
     prm.Q = static_cast<const uint16_t*>(Q);
     prm.K = static_cast<const uint16_t*>(K);

@@ -126,6 +126,26 @@ def test_what_lies_outside_the_sequences_is_neither_read_nor_written(heads):
     assert (O[60:171] == 0).all() and torch.isinf(LSE[60:171]).all()
 
 
+def test_one_token_may_have_any_stride():
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    buf = torch.randn(4096, generator=gen, device="cuda", dtype=torch.float16)
+    Q, K = buf.as_strided((1, 4, 128), (3, 128, 1)), buf.as_strided((1, 2, 128), (5, 128, 1), 1024)
+    run([1], (4, 2, 128), tensors=(Q, K, K))
+    Q1, K1 = kf.qk_norm_rope(Q, K, ints([7]), kf.rope_freqs(128, device="cuda")[0])
+    Q2, K2 = kf.qk_norm_rope(Q.contiguous(), K.contiguous(), ints([7]), kf.rope_freqs(128, device="cuda")[0])
+    assert torch.equal(Q1, Q2) and torch.equal(K1, K2)
+
+
+def test_a_key_of_another_sequence_does_not_reach_its_neighbours():
+    """NaN and infinities in the keys and values of one sequence: the others' bits."""
+    Q, K, V = make([100, 40, 77], (8, 2, 128), torch.float16)
+    s = ints([0, 100, 140, 217])
+    want = kf.attn_packed(Q, K, V, s, causal=True)
+    K[100:140], V[100:140] = math.nan, math.inf
+    got = kf.attn_packed(Q, K, V, s, causal=True)
+    assert torch.equal(got[:100], want[:100]) and torch.equal(got[140:], want[140:])
+
+
 def test_starts_outside_the_tensors_are_clamped():
     Q, K, V = make([100], (4, 2, 64), torch.float16)
     a = kf.attn_packed(Q, K, V, ints([-5, 40, 1 << 30]), causal=True)

@@ -132,6 +132,14 @@ def test_strides(lib):
             assert call(lib, strides=s) == kf.KF_ERR_SIZE
 
 
+def test_packed_key_strides(lib):
+    top = 1 << 28
+    for i in range(6):
+        s = [1024] * 6
+        s[i] = top + 8
+        assert (packed(lib, strides=s) == kf.KF_ERR_SIZE) == (i in (2, 4)), i
+
+
 def test_decode_workspace(lib):
     need = kf.kv4_workspace_bytes(2, 1, 8, 2, 128, 16, 4)
     assert need > 0 and need % 256 == 0
