@@ -301,7 +301,8 @@ int kf_attn_packed(const void* Q, const void* K, const void* V, void* O,
  *   KF_BF16), D = 16, 64, 128 or 256; `strides`: NULL (contiguous), or eight
  *   host values, token and head strides of Q, K, Q_out and K_out in elements,
  *   multiples of 8.  Q_out may be Q and K_out may be K, with the same strides;
- *   outputs that overlap anything else give undefined rows.
+ *   outputs that overlap anything else give undefined rows, and an output whose
+ *   own rows overlap (a broadcast view in place) is KF_ERR_SIZE.
  * q_weight, k_weight: [D] of the same type, or NULL: Q or K is not normed.
  *   With one, x -> x / sqrt(mean(x^2) + eps) * weight over the D channels.
  * The first `rot` channels (a multiple of 16, 0 to D) of a head are turned by

@@ -31,6 +31,16 @@ int check_strides(const int64_t* s, int n) {
     return KF_OK;
 }
 
+// Whether no two rows of D elements overlap, of which `tokens` lie `token` apart
+// and in each `heads` lie `head` apart.
+bool distinct_rows(int tokens, int64_t token, int heads, int64_t head, int D) {
+    if (tokens == 1) return heads == 1 || head >= D;
+    if (heads == 1) return token >= D;
+    const int64_t inner = std::min(token, head), outer = std::max(token, head);
+    const int n = token < head ? tokens : heads;  // rows `inner` apart
+    return inner >= D && outer / inner >= n - 1 && outer - inner * (n - 1) >= D;
+}
+
 int check_heads(int H_q, int H_kv) {
     if (H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0) return KF_ERR_GQA;
     return KF_OK;
@@ -69,11 +79,17 @@ int check_attn_flags(int flags) {
 // ---- Packed attention. ----
 
 template <bool kBF, int D, int NW, int KS>
-int launch_packed(const kf::PackedParams& prm, long long rows, hipStream_t stream) {
+int launch_packed(kf::PackedParams& prm, long long rows, hipStream_t stream) {
     using Cfg = kf::PackedCfg<D, NW, KS>;
     // Tiles of all sequences: a partial one for each at most.
     const long long tiles = rows / Cfg::kRows + std::min<long long>(prm.n_seqs, prm.tokens_q);
     if (tiles * prm.heads_kv > INT_MAX) return KF_ERR_SIZE;
+    // Strictly by length, the tiles that share keys run far apart, and their keys come
+    // from beyond the L2 each time.  Many workgroups a CU even out by themselves, so
+    // that coarser levels do: 64 x 256 queries, 32 / 8 heads, D = 128 (16 a CU), 97 us
+    // in levels of one tile, 89 of two; 64 of 16 to 4096 (46 a CU) 747 and, of four to
+    // eight, 735 to 729; 8 x 1024, 16 / 16 heads, D = 64 (4 a CU), 28.3 and, of four, 32.0.
+    prm.level_tiles = (int)std::clamp<long long>(tiles * prm.heads_kv / (8LL * current_device_shape().cus), 1, 8);
     (void)hipGetLastError();
     kf::kf_attn_packed_kernel<kBF, D, NW, KS>
         <<<dim3((unsigned)(tiles * prm.heads_kv)), dim3(Cfg::kThreads), 0, stream>>>(prm);
@@ -129,7 +145,7 @@ int packed_layout(const kf::PackedParams& prm, int D) {
 }
 
 template <bool kBF>
-int launch_packed_dim(const kf::PackedParams& prm, int D, hipStream_t stream) {
+int launch_packed_dim(kf::PackedParams& prm, int D, hipStream_t stream) {
     const long long rows = (long long)prm.tokens_q * prm.ratio;
     const int layout = packed_layout(prm, D);
     switch (D) {
@@ -244,8 +260,10 @@ template <bool kBF, int D>
 int launch_rope(const kf::RopeParams& prm, hipStream_t stream) {
     (void)hipGetLastError();
     const dim3 block(64 * kf::kRopeWaves);
-    // A wave per token while that gives every SIMD four; else a workgroup.
-    if (prm.tokens >= 16 * current_device_shape().cus)
+    // A wave per token while that gives every CU ten, else a workgroup: 512 tokens of 32 + 8 heads,
+    // D = 128, 6.3 us by workgroups and 9.5 by waves, 2048 12.9 and 13.8, 3000
+    // 16.7 and 16.1, 6000 30.9 and 27.0; of 32 + 1 heads of 64, 2048 8.9 and 8.9, 8192 24.6 and 19.0.
+    if (prm.tokens >= 10 * current_device_shape().cus)
         kf::kf_qk_norm_rope_kernel<kBF, D, 4><<<dim3((prm.tokens + 3) / 4), block, 0, stream>>>(prm);
     else
         kf::kf_qk_norm_rope_kernel<kBF, D, 1><<<dim3(prm.tokens), block, 0, stream>>>(prm);
@@ -327,6 +345,8 @@ int kf_qk_norm_rope(const void* Q, const void* K, void* Q_out, void* K_out, cons
     const int64_t packed[8] = {(int64_t)H_q * D, D, (int64_t)H_kv * D, D, (int64_t)H_q * D, D, (int64_t)H_kv * D, D};
     if (!strides) strides = packed;
     if (const int st = check_strides(strides, 8); st != KF_OK) return st;
+    if (!distinct_rows(tokens, strides[4], H_q, strides[5], D) || !distinct_rows(tokens, strides[6], H_kv, strides[7], D))
+        return KF_ERR_SIZE;
     kf::RopeParams prm{};
     prm.x[0] = static_cast<const uint16_t*>(Q);
     prm.x[1] = static_cast<const uint16_t*>(K);

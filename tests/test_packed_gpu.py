@@ -86,6 +86,14 @@ def test_long_prompts(S, heads, dtype):
     run([S, 5, S // 3], heads, dtype, fused=True)
 
 
+@pytest.mark.parametrize("n,longest,heads,causal", [(64, 600, (64, 64, 64), True), (40, 900, (32, 32, 64), True),
+                                                    (64, 600, (32, 32, 128), False), (64, 500, (32, 32, 256), True)])
+def test_grids_of_many_rounds(n, longest, heads, causal):
+    """Workgroups enough that several tiles of a sequence are numbered together."""
+    lens = [(i * 7919 + 13) % longest for i in range(n)]
+    run(lens, heads, kv_lens=[(k * 3) // 2 if i % 3 else k // 2 for i, k in enumerate(lens)], causal=causal)
+
+
 def test_views_of_a_fused_projection_equal_their_copies():
     Q, K, V = make([300, 20], (8, 2, 128), torch.float16, fused=True)
     s = ints([0, 300, 320])

@@ -47,7 +47,7 @@ def test_layouts_parts_and_types(D, rot, interleaved, dtype, norm):
     check(Ko, K, kw, 1e-5, pos, freqs, interleaved, 1.25)
 
 
-@pytest.mark.parametrize("T", [1, 2, 3, 5, 255, 4095, 4096, 4099, 9001])
+@pytest.mark.parametrize("T", [1, 2, 3, 5, 255, 2559, 2560, 4095, 4099, 9001])
 @pytest.mark.parametrize("heads", [(32, 8, 128), (1, 1, 64), (3, 1, 256), (40, 1, 16)])
 def test_token_and_head_counts(T, heads):
     if T > 5000 and heads[0] > 4:

@@ -140,6 +140,22 @@ def test_packed_key_strides(lib):
         assert (packed(lib, strides=s) == kf.KF_ERR_SIZE) == (i in (2, 4)), i
 
 
+@pytest.mark.parametrize("token,head,ok", [(1024, 128, True), (128, 512, True), (2048, 136, True), (0, 128, False),
+                                           (1024, 0, False), (1016, 128, False), (120, 512, False), (128, 504, False),
+                                           (1 << 62, 128, True), (1 << 62, 1 << 62, False)])
+def test_rope_outputs_are_not_broadcast(lib, token, head, ok):
+    """4 tokens of 8 heads of 128: rows that overlap would be written twice."""
+    if torch.cuda.is_available() and ok:
+        pytest.skip("the pointers are fakes")
+    s = [1024, 128, 256, 128, token, head, 256, 128]
+    assert rope(lib, strides=s) == (kf.KF_ERR_HIP if ok else kf.KF_ERR_SIZE)
+    s = [1024, 128, 1024, 128, 1024, 128, token, head]
+    assert rope(lib, strides=s, H_kv=8) == (kf.KF_ERR_HIP if ok else kf.KF_ERR_SIZE)
+    # Strides of a single token or head do not count.
+    if not torch.cuda.is_available():
+        assert rope(lib, strides=[1024, 128, 0, 0, 1024, 128, 0, 0], T=1, H_kv=1) == kf.KF_ERR_HIP
+
+
 def test_decode_workspace(lib):
     need = kf.kv4_workspace_bytes(2, 1, 8, 2, 128, 16, 4)
     assert need > 0 and need % 256 == 0
