@@ -232,11 +232,26 @@ void kf_kv4_read_kernel(Kv4Params p) {
 // lane group q holds keys 4 q .. + 3 of both halves of the stage, and V^T is
 // read in that order of the keys.  K(t + 1) is requested when the score MFMAs
 // have consumed K(t), V(t + 1) when V(t) has gone to LDS.
+//
+// Bound by memory: with the loads alone it takes as long.  32 / 8 heads, D = 128, both
+// launches: 32 x 8192 keys (285 MB) 58 us, 4.9 TB/s, the stages themselves at 6.2;
+// 8 x 50000 to 65536, 4 queries each, bf16 (506 MB) 90 to 93, 5.4 to 5.6; 32 x 512
+// to 8192 (84 MB) 25; 1 x 4096 (4.5 MB) 9.  About 10 us are fixed: the launch
+// 2.3, key counts, page ids and first rows one after the other 1.3 to 3.3, the
+// LDS merge 2, the merge launch 3 to 5.  The scale bytes, a row's 4 to 16, cost 2
+// to 10 % of the stages' time.  Tried: 64 keys a trip (spills with three
+// workgroups a CU; with two, 25 -> 29 us for the 84 MB), two stages in flight
+// with Q in LDS (slower), cached instead of non-temporal loads (slower from 84 MB on).
 // ---------------------------------------------------------------------------
+// NQ: 16-row blocks of queries.  Two for more than 16 rows alone: their registers and
+// LDS leave a third fewer workgroups (16 rows on two blocks 58 -> 72 us, 93 -> 123).
 template <int D, int NQ> struct Kv4Cfg {
     static constexpr int kWaves = 4;                          // workers per workgroup
     static constexpr int kThreads = 64 * kWaves;
-    // Workgroups per CU, by registers and LDS.
+    // Workgroups per CU, as many as registers and LDS hold (16 rows, D = 128: one
+    // fewer, two, 58.0 -> 60.7 us for 32 x 8192 and 93 -> 104 for the 506 MB above; calls
+    // whose share is a few stages a wave run up to 20 % faster or 12 % slower,
+    // by how the shares fall on the heads).
     static constexpr int kPerCU = D == 64 ? (NQ == 1 ? 4 : 3) : D == 128 ? (NQ == 1 ? 3 : 2) : NQ == 1 ? 2 : 1;
     static constexpr int kSlot = NQ * 64 * D;                 // a wave's V rows in 16 bits; its partial
 };

@@ -88,9 +88,16 @@ def _starts(torch, name, t, device):
     return _ints(torch, name, t, device, t.shape)
 
 
-def _like(torch, t, shape, dtype, stream):
+def _new_at(torch, t, shape, dtype, stream):
     """_new on t's device (new_empty takes less time than empty)."""
     return t.new_empty(shape, dtype=dtype) if stream is None else _new(torch, shape, dtype, t.device, stream)
+
+
+def _like(torch, t, dtype, stream):
+    """A new contiguous tensor of t's shape (empty_like takes less time again)."""
+    if stream is None:
+        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+    return _new(torch, t.shape, dtype, t.device, stream)
 
 
 def _launch(torch, device, stream, entry, *args):
@@ -134,10 +141,10 @@ def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, 
     if kv_starts is not None:
         kstarts = _ints(torch, "kv_starts", kv_starts, device, seq_starts.shape)
     if out is None:
-        out = _like(torch, Q, (T, H_q, D), out_dtype or torch.float32, stream)
+        out = _like(torch, Q, out_dtype or torch.float32, stream)
     else:
         out = _output(torch, out, (T, H_q, D), out_dtype, device, stream)
-    lse = _like(torch, Q, (T, H_q), torch.float32, stream) if return_lse else None
+    lse = _new_at(torch, Q, (T, H_q), torch.float32, stream) if return_lse else None
     if causal:
         flags |= KF_ATTN_CAUSAL
     _launch(torch, device, stream, load_library().kf_attn_packed,
@@ -227,7 +234,7 @@ def qk_norm_rope(Q, K, positions, freqs, out=None, *, q_weight=None, k_weight=No
             raise ValueError("freqs without positions")
         pos = _ints(torch, "positions", positions, device, (T,))
     if out is None:
-        out = (_like(torch, Q, (T, H_q, D), Q.dtype, stream), _like(torch, Q, (T, H_kv, D), Q.dtype, stream))
+        out = (_like(torch, Q, Q.dtype, stream), _like(torch, K, Q.dtype, stream))
         strides += (H_q * D, D, H_kv * D, D)
     else:
         for name, y, x in (("out[0]", out[0], Q), ("out[1]", out[1], K)):
@@ -328,7 +335,8 @@ def kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, total, D, out=N
     table, lens = _table(torch, block_table, kv_lens, device, n)
     shape = (total, H_kv, D)
     if out is None:
-        K, V = _like(torch, K_pages, shape, dtype, stream), _like(torch, K_pages, shape, dtype, stream)
+        K = _new_at(torch, K_pages, shape, dtype, stream)
+        V = _like(torch, K, dtype, stream)
     else:
         K, V = (_output(torch, x, shape, dtype, device, stream) for x in out)
     _launch(torch, device, stream, load_library().kf_kv4_read,
@@ -364,13 +372,13 @@ def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, caus
     table, lens = _table(torch, block_table, kv_lens, device, B)
     max_pages = block_table.shape[1]
     if out is None:
-        out = _like(torch, Q, Q.shape, out_dtype or torch.float32, stream)
+        out = _like(torch, Q, out_dtype or torch.float32, stream)
     else:
         out = _output(torch, out, (B, H_q, q_len, D), out_dtype, device, stream)
-    lse = _like(torch, Q, (B, H_q, q_len), torch.float32, stream) if return_lse else None
+    lse = _new_at(torch, Q, (B, H_q, q_len), torch.float32, stream) if return_lse else None
     need = kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size, max_pages)
     if workspace is None and need:
-        workspace = _like(torch, Q, need, torch.uint8, stream)
+        workspace = _new_at(torch, Q, need, torch.uint8, stream)
     else:
         workspace, need = _workspace(torch, workspace, need, lambda: need, device, stream)
     if causal:
