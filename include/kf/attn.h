@@ -368,7 +368,9 @@ int kf_kv4_read(const void* K_pages, const void* V_pages, const int* block_table
  * (H_q / H_kv) * q_len <= 32, else KF_ERR_SIZE; D = 64, 128 or 256.  The
  * workspace (256-byte aligned, no initialisation, not shared by calls that can
  * run concurrently) is required.  With KF_BF16 the softmax weights are rounded
- * to bf16 before they meet V, else to fp16; V itself is exact. */
+ * to bf16 before they meet V, else to fp16; V itself is exact.  A NaN among a
+ * sequence's values may reach any of its rows, as in kf_attn_packed; what pages
+ * hold past a sequence's keys does not matter. */
 size_t kf_attn_decode_kv4_workspace_bytes(int B, int q_len, int H_q, int H_kv, int D,
                                           int page_size, int max_pages_per_seq);
 int kf_attn_decode_kv4(const void* Q, const void* K_pages, const void* V_pages,
