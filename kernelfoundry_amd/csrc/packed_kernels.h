@@ -12,14 +12,15 @@
 // -> LDS by LDS-DMA, P^T straight from the score registers.
 //
 // Bound by the matrix units and the softmax between their products: causal, 32 / 8
-// heads, D = 128, 1 x 8192 bf16 takes 510 to 560 us, 1.0 to 1.08 PFLOP/s (a library
+// heads, D = 128, 1 x 8192 bf16 takes 505 to 545 us, 1.0 to 1.09 PFLOP/s (a library
 // product 1.2), MFMA busy 54 % of the SIMD cycles, LDS 28 %, next to no bank
 // conflicts; 16 sequences of 16 to 4096 117 to 126 us (0.75 PFLOP/s), of which
 // a workgroup's first loads and its store (191 MB in all, 38 us of memory time) hide
 // behind other workgroups' products in part; 4 x 512 queries against 4096
 // keys, 16 / 4 heads, D = 256, 150 (0.86 PFLOP/s).  Tried: 64 rows a wave on 8 waves
 // (4 to 6 % faster at 8192, 5 to 40 % slower at the others), the scores of the next
-// stage beside this one's products (its third buffer costs a workgroup a CU: no gain).
+// stage beside this one's products (its third buffer costs a workgroup a CU: no gain),
+// stages requested two tiles ahead (no change: they have landed by then).
 #pragma once
 
 #include "elem.h"
@@ -55,6 +56,11 @@ template <int D, int NW, int KS> struct PackedCfg {
     static constexpr int kBatch = D == 256 ? 4 : KS == 1 ? 2 : D / 16;
     static constexpr int kAhead = D == 256 ? 0 : KS == 1 ? 1 : D / 32;
     static constexpr bool kOrder = D < 256;               // kept apart from the scheduler
+    // Stages copied in asm, from a scalar row and lane offsets that stay in registers; the
+    // builtin's offsets, computed for every stage, cost 1 to 4 % (1 x 8192, 32 / 8 heads,
+    // D = 128, bf16 518 -> 505 us; 1 x 4096, 32 / 1 heads, D = 64, 92.4 -> 88.2). At
+    // D = 256 there are no registers for them: spills, and no gain without.
+    static constexpr bool kAsmCopy = D < 256;
     // The per-lane LDS offsets of a tile derived from one, for want of registers.
     static constexpr bool kXorOff = D >= 128;
 };
@@ -209,6 +215,23 @@ __device__ __forceinline__ void packed_store(const AttnParams& p, const f32x16 (
     }
 }
 
+__device__ __forceinline__ uint32_t lds_addr(char* p) { return (uint32_t)(uintptr_t)(lds_void*)p; }
+
+// LDS-DMA in asm as lds_copy16_nt's, but kept in the L2: other tiles read the same keys.
+__device__ __forceinline__ void lds_copy16(uint32_t lds, const void* base, uint32_t off) {
+    const uint64_t b = (uint64_t)(uintptr_t)base;
+    base = (const void*)(uintptr_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
+                                    (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
+                 ::"{m0}"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void lds_copy16(uint32_t lds, const void* lane_src) {
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, off"
+                 ::"{m0}"(lds), "v"(lane_src) : "memory");
+}
+
 template <bool kBF, int D, int NW, int KS>
 __global__ __launch_bounds__((PackedCfg<D, NW, KS>::kThreads), (PackedCfg<D, NW, KS>::kWavesPerSimd))
 void kf_attn_packed_kernel(PackedParams p) {
@@ -304,14 +327,17 @@ void kf_attn_packed_kernel(PackedParams p) {
         char* d = dst + (is_v ? kTensorBytes : 0) + ii0 * 1024;
         const int kv = kv_base + kv0 + ii0 * kRowsPerInstr;
         if (kv_base + kv0 + BC <= klen) {
-            // Whole stage: wave-uniform row base and a 32-bit lane offset,
-            // opaque so that the address stays their sum.
+            // Whole stage: wave-uniform row base and a 32-bit lane offset.
 #pragma unroll
             for (int i = 0; i < kPerWave; ++i) {
                 uint32_t off = lr * row_stride + chunk_off[i % kPeriod];
-                asm volatile("" : "+v"(off));
-                const char* a = src + (size_t)(kv + i * kRowsPerInstr) * row_stride + off;
-                __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
+                if constexpr (Cfg::kAsmCopy) {
+                    lds_copy16(lds_addr(d + i * 1024), src + (size_t)(kv + i * kRowsPerInstr) * row_stride, off);
+                } else {
+                    asm volatile("" : "+v"(off));  // computed here, so that the address stays their sum
+                    const char* a = src + (size_t)(kv + i * kRowsPerInstr) * row_stride + off;
+                    __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
+                }
             }
         } else {
             asm volatile("" ::: "memory");
@@ -320,7 +346,10 @@ void kf_attn_packed_kernel(PackedParams p) {
                 // Rows past the keys re-read the last one (finite data whose scores are masked).
                 const int row = min(kv + i * kRowsPerInstr + lr, klen - 1);
                 const char* a = src + (size_t)row * row_stride + chunk_off[i % kPeriod];
-                __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
+                if constexpr (Cfg::kAsmCopy)
+                    lds_copy16(lds_addr(d + i * 1024), a);
+                else
+                    __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
             }
         }
     };
@@ -423,8 +452,17 @@ void kf_attn_packed_kernel(PackedParams p) {
             char* nxt = u == 0 ? b1 : b0;
             // Stage t has landed for every wave; every wave is done with
             // stage t - 1 (in nxt).
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+            if constexpr (Cfg::kAsmCopy) {
+                // (A wait that the compiler sees, so that the first tile's loads
+                // of Q do not make it wait for a stage in every tile.)
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+            }
             if (t + 1 < ntiles) issue_stage(nxt, (t + 1) * BC);
             tile(cur, t);
         }
