@@ -215,8 +215,6 @@ __device__ __forceinline__ void packed_store(const AttnParams& p, const f32x16 (
     }
 }
 
-__device__ __forceinline__ uint32_t lds_addr(char* p) { return (uint32_t)(uintptr_t)(lds_void*)p; }
-
 // LDS-DMA in asm as lds_copy16_nt's, but kept in the L2: other tiles read the same keys.
 __device__ __forceinline__ void lds_copy16(uint32_t lds, const void* base, uint32_t off) {
     const uint64_t b = (uint64_t)(uintptr_t)base;
@@ -325,6 +323,7 @@ void kf_attn_packed_kernel(PackedParams p) {
         chunk_off[i] = (((lane % kChunks) ^ SW::h((ii0 + i) * kRowsPerInstr + lr)) % kChunks) * 16;
     auto issue_stage = [&](char* dst, int kv0) {
         char* d = dst + (is_v ? kTensorBytes : 0) + ii0 * 1024;
+        const uint32_t d_lds = (uint32_t)(uintptr_t)(lds_void*)d;
         const int kv = kv_base + kv0 + ii0 * kRowsPerInstr;
         if (kv_base + kv0 + BC <= klen) {
             // Whole stage: wave-uniform row base and a 32-bit lane offset.
@@ -332,7 +331,7 @@ void kf_attn_packed_kernel(PackedParams p) {
             for (int i = 0; i < kPerWave; ++i) {
                 uint32_t off = lr * row_stride + chunk_off[i % kPeriod];
                 if constexpr (Cfg::kAsmCopy) {
-                    lds_copy16(lds_addr(d + i * 1024), src + (size_t)(kv + i * kRowsPerInstr) * row_stride, off);
+                    lds_copy16(d_lds + i * 1024, src + (size_t)(kv + i * kRowsPerInstr) * row_stride, off);
                 } else {
                     asm volatile("" : "+v"(off));  // computed here, so that the address stays their sum
                     const char* a = src + (size_t)(kv + i * kRowsPerInstr) * row_stride + off;
@@ -347,7 +346,7 @@ void kf_attn_packed_kernel(PackedParams p) {
                 const int row = min(kv + i * kRowsPerInstr + lr, klen - 1);
                 const char* a = src + (size_t)row * row_stride + chunk_off[i % kPeriod];
                 if constexpr (Cfg::kAsmCopy)
-                    lds_copy16(lds_addr(d + i * 1024), a);
+                    lds_copy16(d_lds + i * 1024, a);
                 else
                     __builtin_amdgcn_global_load_lds(a, (lds_void*)(d + i * 1024), 16, 0, 0);
             }
