@@ -287,7 +287,8 @@ int kf_attn_decode_paged(const void* Q, const void* K_pages, const void* V_pages
  * What tokens outside the sequences and other sequences hold does not matter; a
  * NaN or an infinity among a sequence's own keys or values may reach any row of
  * that sequence, also one that does not see it.
- * tokens_q, tokens_kv and n_seqs are positive.  No workspace. */
+ * tokens_q, tokens_kv and n_seqs are positive; tokens_q H_q, tokens_kv H_kv and
+ * tokens_kv H_q / H_kv are at most 2^31 - 1025.  No workspace. */
 int kf_attn_packed(const void* Q, const void* K, const void* V, void* O,
                    float* row_max, float* row_sumexp, const int64_t* strides,
                    const int* q_starts, const int* kv_starts,
@@ -341,8 +342,8 @@ size_t kf_kv4_page_bytes(int page_size, int D);  /* 0 for an invalid size */
  * of K and V.  kv_lens: device int [n_seqs], the keys of each sequence with the
  * new tokens: sequence b's packed tokens become its last ones.  A token whose
  * page id is outside [0, num_pages), or whose place is outside the table, is
- * not written; nor is one outside the sequences.  Two sequences of a call that
- * write the same row of the same page leave an undefined row. */
+ * not written; nor is one outside the sequences.  Two tokens of a call whose
+ * places are the same row of the same page leave an undefined row. */
 int kf_kv4_append(const void* K, const void* V, const int64_t* strides,
                   void* K_pages, void* V_pages, const int* block_table,
                   const int* seq_starts, const int* kv_lens,

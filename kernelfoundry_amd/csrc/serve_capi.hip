@@ -21,6 +21,8 @@ using namespace kf_capi;
 bool aligned4(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 3u) == 0; }
 
 constexpr int64_t kMaxKvTokenStride = 1 << 28;
+// Rows and keys have int indexes, and the kernels round them up to whole tiles.
+constexpr long long kMaxIndex = INT_MAX - 1024;
 
 // Strides of 16-byte chunks, not negative; n of them.
 int check_strides(const int64_t* s, int n) {
@@ -51,9 +53,12 @@ int check_heads(int H_q, int H_kv) {
 int check_packed(long long tokens, int heads, int D) {
     if (D != 64 && D != 128 && D != 256) return KF_ERR_HEAD_DIM;
     if (tokens <= 0 || heads <= 0) return KF_ERR_SIZE;
-    if (tokens * heads > INT_MAX) return KF_ERR_SIZE;
+    if (tokens * heads > kMaxIndex) return KF_ERR_SIZE;
     return KF_OK;
 }
+
+// Whether a grid's threads have 32-bit numbers, as the hardware needs.
+bool fits_grid(long long workgroups, int threads) { return workgroups * threads <= (long long)UINT_MAX; }
 
 int launched() {
     const hipError_t e = hipGetLastError();
@@ -83,7 +88,7 @@ int launch_packed(kf::PackedParams& prm, long long rows, hipStream_t stream) {
     using Cfg = kf::PackedCfg<D, NW, KS>;
     // Tiles of all sequences: a partial one for each at most.
     const long long tiles = rows / Cfg::kRows + std::min<long long>(prm.n_seqs, prm.tokens_q);
-    if (tiles * prm.heads_kv > INT_MAX) return KF_ERR_SIZE;
+    if (!fits_grid(tiles * prm.heads_kv, Cfg::kThreads)) return KF_ERR_SIZE;
     // Strictly by length, the tiles that share keys run far apart, and their keys come
     // from beyond the L2 each time.  Many workgroups a CU even out by themselves, so
     // that coarser levels do: 64 x 256 queries, 32 / 8 heads, D = 128 (16 a CU), 97 us
@@ -176,7 +181,7 @@ int kv4_plan(int B, int q_len, int H_q, int H_kv, int D, int page_size, int max_
     if (B <= 0 || q_len <= 0) return KF_ERR_SIZE;
     if (const int st = paged_geometry(page_size, max_pages, num_pages, &pl->shift, &pl->cap); st != KF_OK) return st;
     const long long R = (long long)(H_q / H_kv) * q_len, groups = (long long)B * H_kv;
-    if (R > 32) return KF_ERR_SIZE;
+    if (R > 32 || pl->cap > kMaxIndex) return KF_ERR_SIZE;
     const long long stages = groups * ((pl->cap + 31LL) / 32);
     if (groups > INT_MAX || stages > (1LL << 30) || groups * R * (D / 4) > INT_MAX) return KF_ERR_SIZE;
     pl->R = (int)R;
@@ -263,10 +268,13 @@ int launch_rope(const kf::RopeParams& prm, hipStream_t stream) {
     // A wave per token while that gives every CU ten, else a workgroup: 512 tokens of 32 + 8 heads,
     // D = 128, 6.3 us by workgroups and 9.5 by waves, 2048 12.9 and 13.8, 3000
     // 16.7 and 16.1, 6000 30.9 and 27.0; of 32 + 1 heads of 64, 2048 8.9 and 8.9, 8192 24.6 and 19.0.
-    if (prm.tokens >= 10 * current_device_shape().cus)
-        kf::kf_qk_norm_rope_kernel<kBF, D, 4><<<dim3((prm.tokens + 3) / 4), block, 0, stream>>>(prm);
-    else
+    if (prm.tokens >= 10 * current_device_shape().cus) {
+        const int grid = (prm.tokens + 3) / 4;
+        if (!fits_grid(grid, 64 * kf::kRopeWaves)) return KF_ERR_SIZE;
+        kf::kf_qk_norm_rope_kernel<kBF, D, 4><<<dim3(grid), block, 0, stream>>>(prm);
+    } else {
         kf::kf_qk_norm_rope_kernel<kBF, D, 1><<<dim3(prm.tokens), block, 0, stream>>>(prm);
+    }
     return launched();
 }
 
@@ -292,7 +300,7 @@ int kf_attn_packed(const void* Q, const void* K, const void* V, void* O, float* 
     if (n_seqs <= 0) return KF_ERR_SIZE;
     if (const int st = check_packed(tokens_q, H_q, D); st != KF_OK) return st;
     if (const int st = check_packed(tokens_kv, H_kv, D); st != KF_OK) return st;
-    if ((long long)tokens_kv * (H_q / H_kv) > INT_MAX) return KF_ERR_SIZE;
+    if ((long long)tokens_kv * (H_q / H_kv) > kMaxIndex) return KF_ERR_SIZE;
     if (const int st = check_attn_flags(flags); st != KF_OK) return st;
     if (!Q || !K || !V || !O || !q_starts || !kv_starts) return KF_ERR_NULL;
     if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(O)) return KF_ERR_ALIGN;
@@ -335,7 +343,7 @@ int kf_qk_norm_rope(const void* Q, const void* K, void* Q_out, void* K_out, cons
                     const void* q_weight, const void* k_weight, const int* positions, const double* freqs, int tokens,
                     int H_q, int H_kv, int D, int rot, float eps, float scale, int flags, void* stream) {
     if (D != 16 && D != 64 && D != 128 && D != 256) return KF_ERR_HEAD_DIM;
-    if (tokens <= 0 || H_q <= 0 || H_kv <= 0 || rot < 0 || rot > D || rot % 16 != 0) return KF_ERR_SIZE;
+    if (tokens <= 0 || tokens > kMaxIndex || H_q <= 0 || H_kv <= 0 || rot < 0 || rot > D || rot % 16 != 0) return KF_ERR_SIZE;
     if ((long long)H_q + H_kv > INT_MAX / 2) return KF_ERR_SIZE;
     if ((flags & ~(KF_BF16 | KF_ROPE_INTERLEAVED)) != 0) return KF_ERR_FLAGS;
     if (!Q || !K || !Q_out || !K_out || (rot > 0 && (!positions || !freqs))) return KF_ERR_NULL;

@@ -296,7 +296,7 @@ def kv4_append(K, V, K_pages, V_pages, block_table, seq_starts, kv_lens, *, stre
     with any token and head strides (multiples of 8).  Sequence b's tokens
     become the last of its ``kv_lens[b]`` keys (int32 [N], counted with them);
     ``block_table`` int32 [N, max_pages].  Tokens of an invalid page are not
-    written; no two sequences may write the same row.
+    written; no two tokens of a call may have the same row.
     """
     import torch
 

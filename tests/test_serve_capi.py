@@ -84,6 +84,17 @@ def test_sizes(lib):
     for kw in (dict(n=0), dict(n=-1), dict(tq=0), dict(tk=0), dict(tq=-5), dict(tq=big), dict(tk=big)):
         assert packed(lib, **kw) == kf.KF_ERR_SIZE, kw
     assert packed(lib, H_q=1 << 20, H_kv=1, tq=1, tk=1 << 12) == kf.KF_ERR_SIZE
+    # Indexes that rounding up to a tile would take past an int.
+    top = 2 ** 31 - 1
+    assert packed(lib, tq=top // 8) == kf.KF_ERR_SIZE
+    assert packed(lib, tk=top // 4) == kf.KF_ERR_SIZE
+    assert rope(lib, T=top) == kf.KF_ERR_SIZE
+    # Grids of more threads than a launch can number.
+    assert rope(lib, T=1 << 27, H_q=1, H_kv=1) == kf.KF_ERR_SIZE
+    assert packed(lib, n=1 << 24, tq=1 << 24, H_q=2, H_kv=2) == kf.KF_ERR_SIZE
+    for call in (append, read):
+        assert call(lib, T=top, H_kv=1) == kf.KF_ERR_SIZE
+    assert decode(lib, B=1, H_q=1, H_kv=1, mp=top // 16) == kf.KF_ERR_SIZE
     for kw in (dict(T=0), dict(T=-1), dict(H_q=0), dict(H_kv=0), dict(rot=-16), dict(rot=8), dict(rot=144),
                dict(rot=24)):
         assert rope(lib, **kw) == kf.KF_ERR_SIZE, kw
