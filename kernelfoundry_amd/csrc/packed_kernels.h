@@ -55,7 +55,8 @@ template <int D, int NW, int KS> struct PackedCfg {
     // 74.3 -> 65.3; full grids lose 1 %).
     static constexpr int kBatch = D == 256 ? 4 : KS == 1 ? 2 : D / 16;
     static constexpr int kAhead = D == 256 ? 0 : KS == 1 ? 1 : D / 32;
-    static constexpr bool kOrder = D < 256;               // kept apart from the scheduler
+    // Kept apart from the scheduler, which without KV groups does up to 1 % better by itself.
+    static constexpr bool kOrder = KS > 1 && D < 256;
     // Stages copied in asm, from a scalar row and lane offsets that stay in registers; the
     // builtin's offsets, computed for every stage, cost 1 to 4 % (1 x 8192, 32 / 8 heads,
     // D = 128, bf16 518 -> 505 us; 1 x 4096, 32 / 1 heads, D = 64, 92.4 -> 88.2). At
