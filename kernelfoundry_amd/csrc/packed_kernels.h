@@ -12,15 +12,16 @@
 // -> LDS by LDS-DMA, P^T straight from the score registers.
 //
 // Bound by the matrix units and the softmax between their products: causal, 32 / 8
-// heads, D = 128, 1 x 8192 bf16 takes 505 to 545 us, 1.0 to 1.09 PFLOP/s (a library
-// product 1.2), MFMA busy 54 % of the SIMD cycles, LDS 28 %, next to no bank
-// conflicts; 16 sequences of 16 to 4096 117 to 126 us (0.75 PFLOP/s), of which
+// heads, D = 128, 1 x 8192 bf16 takes 500 to 545 us, 1.0 to 1.1 PFLOP/s (a library
+// product 1.2), MFMA busy 59 % of the SIMD cycles, LDS 30 %, next to no bank
+// conflicts; 16 sequences of 16 to 4096 117 to 122 us (0.76 PFLOP/s), of which
 // a workgroup's first loads and its store (191 MB in all, 38 us of memory time) hide
 // behind other workgroups' products in part; 4 x 512 queries against 4096
 // keys, 16 / 4 heads, D = 256, 150 (0.86 PFLOP/s).  Tried: 64 rows a wave on 8 waves
 // (4 to 6 % faster at 8192, 5 to 40 % slower at the others), the scores of the next
 // stage beside this one's products (its third buffer costs a workgroup a CU: no gain),
-// stages requested two tiles ahead (no change: they have landed by then).
+// stages requested two tiles ahead (no change), two V tiles before the softmax at
+// D = 128 (spills).
 #pragma once
 
 #include "elem.h"
