@@ -20,6 +20,7 @@ gradients.  None of them has a counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 from . import (KF_ATTN_CAUSAL, KF_ERR_HIP, KF_OK, KfError, _new, _out_flags, _output, _raw_stream,
@@ -351,6 +352,15 @@ def kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size, max_pages_per_seq) ->
                                                                  max_pages_per_seq))
 
 
+@functools.lru_cache(maxsize=1024)
+def _kv4_need(index, *sizes):
+    """kv4_workspace_bytes on device `index`, by the sizes alone (0.6 us a call to ask)."""
+    import torch
+
+    with torch.cuda.device(index):
+        return kv4_workspace_bytes(*sizes)
+
+
 def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, causal=False, workspace=None,
                     stream=None, out_dtype=None, return_lse=False):
     """Decode over the paged 4-bit cache that kv4_append writes.
@@ -376,7 +386,7 @@ def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, caus
     else:
         out = _output(torch, out, (B, H_q, q_len, D), out_dtype, device, stream)
     lse = _new_at(torch, Q, (B, H_q, q_len), torch.float32, stream) if return_lse else None
-    need = kv4_workspace_bytes(B, q_len, H_q, H_kv, D, page_size, max_pages)
+    need = _kv4_need(device.index, B, q_len, H_q, H_kv, D, page_size, max_pages)
     if workspace is None and need:
         workspace = _new_at(torch, Q, need, torch.uint8, stream)
     else:
