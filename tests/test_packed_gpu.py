@@ -200,6 +200,22 @@ def test_offsets_past_32_bits():
     assert torch.equal(kf.attn_packed(*views, s, causal=True), kf.attn_packed(*data, s, causal=True))
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_the_widest_key_stride(D):
+    """A copy's 8, 4 or 2 rows of 512 MiB each: 32-bit offsets with the top bit set."""
+    T, stride = 36, 1 << 28
+    buf = torch.empty((T - 1) * stride + 2 * D, dtype=torch.float16, device="cuda")
+    Q, K, V = make([T], (4, 1, D), torch.float16)
+    views = []
+    for i, x in enumerate((K, V)):
+        v = buf.as_strided(x.shape, (stride, D, 1), i * D)
+        v.copy_(x)
+        views.append(v)
+    s = ints([0, T])
+    got = kf.attn_packed(Q, *views, s, causal=True)
+    assert torch.equal(got, kf.attn_packed(Q, K, V, s, causal=True))
+
+
 def test_other_streams_and_graphs():
     Q, K, V = make([64, 500], (8, 2, 128), torch.float16)
     s = ints([0, 64, 564])
