@@ -265,6 +265,9 @@ int kf_attn_decode_paged(const void* Q, const void* K_pages, const void* V_pages
                          int page_size, int max_pages_per_seq, int num_pages, int flags,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* The entry points from here to kf_attn_decode_kv4: a call of which a launch would
+ * have 2^32 threads or more is KF_ERR_SIZE, before anything is launched. */
+
 /* Attention over packed sequences: the tokens of all sequences one after the
  * other, as the projections write them.  No counterpart in the reference.
  *

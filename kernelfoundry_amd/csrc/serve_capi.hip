@@ -194,6 +194,8 @@ int kv4_plan(int B, int q_len, int H_q, int H_kv, int D, int page_size, int max_
     pl->s_bytes = align_up(pl->parts * sizeof(float), kWsAlign);
     pl->ws_bytes = pl->o_bytes + 2 * pl->s_bytes + align_up((size_t)groups * sizeof(kf::u32x4), kWsAlign);
     pl->merge_waves = ragged_merge_waves(pl->R, pl->groups, D);
+    // (A wave per head at least, in workgroups of kRaggedMergeWaves.)
+    if (!fits_grid(groups * pl->merge_waves + kf::kRaggedMergeWaves - 1, 64)) return KF_ERR_SIZE;
     return KF_OK;
 }
 
@@ -242,6 +244,7 @@ int launch_cache(bool append, kf::Kv4Params& prm, hipStream_t stream) {
     const long long share = prm.tokens / (2LL * current_device_shape().cus);
     prm.tile = (int)std::min<long long>(std::max<long long>(fill, std::min<long long>(share, 4LL * fill)), kf::kKv4MaxTile);
     const dim3 grid((prm.tokens + prm.tile - 1) / prm.tile), block(kf::kKv4Threads);
+    if (!fits_grid(grid.x, kf::kKv4Threads)) return KF_ERR_SIZE;
     (void)hipGetLastError();
     if (append)
         kf::kf_kv4_append_kernel<kBF, D><<<grid, block, 0, stream>>>(prm);

@@ -39,8 +39,8 @@ def test_unmarked_tests_launch_nothing_beside_a_gpu(tmp_path):
     (tmp_path / "says_gpu.py").write_text(PLUGIN)
     files = [os.path.join("tests", f) for f in sorted(os.listdir(os.path.join(REPO, "tests")))
              if f.startswith("test_") and f != os.path.basename(__file__)
-             and "FAKE" in open(os.path.join(REPO, "tests", f)).read()]
-    assert {"tests/test_capi.py", "tests/test_serve_capi.py"} <= set(files)
+             and any(word in open(os.path.join(REPO, "tests", f)).read() for word in ("FAKE", "from tests.test_serve_capi"))]
+    assert {"tests/test_capi.py", "tests/test_serve_capi.py", "tests/test_serve_refusals.py"} <= set(files)
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(tmp_path), REPO]))
     r = subprocess.run([sys.executable, "-m", "pytest", "-p", "says_gpu", "-p", "no:cacheprovider", "-q", "-s",
                         "-m", "not gpu", *files], cwd=REPO, env=env, capture_output=True, text=True)
