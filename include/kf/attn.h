@@ -372,9 +372,10 @@ int kf_kv4_read(const void* K_pages, const void* V_pages, const int* block_table
  * (H_q / H_kv) * q_len <= 32, else KF_ERR_SIZE; D = 64, 128 or 256.  The
  * workspace (256-byte aligned, no initialisation, not shared by calls that can
  * run concurrently) is required.  With KF_BF16 the softmax weights are rounded
- * to bf16 before they meet V, else to fp16; V itself is exact.  A NaN among a
- * sequence's values may reach any of its rows, as in kf_attn_packed; what pages
- * hold past a sequence's keys does not matter. */
+ * to bf16 before they meet V, else to fp16; K and V are exactly what kf_kv4_read
+ * with the same flags gives.  So a block with E = 255 is NaN: it makes the rows that
+ * see its key NaN, or their 32 channels, and may reach any other row of its sequence, as
+ * in kf_attn_packed; what pages hold past a sequence's keys does not matter. */
 size_t kf_attn_decode_kv4_workspace_bytes(int B, int q_len, int H_q, int H_kv, int D,
                                           int page_size, int max_pages_per_seq);
 int kf_attn_decode_kv4(const void* Q, const void* K_pages, const void* V_pages,

@@ -6,12 +6,12 @@
 // 2^(E - 127), E one byte, and each channel is a code of 4 bits (sign, 2
 // exponent bits, 1 mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6).  E is the
 // exponent field of the block's largest magnitude (as fp32) less 2, at least
-// 1; x / 2^(E - 127) is rounded to the nearest code, ties to the even one,
-// and magnitudes from 5 up give 6 (the largest is below 8).  Dividing by a power of
-// two is exact, so a code does not depend on the precision it is computed
-// in, and a code times its scale is exact in fp16 and bf16 (of fp16 inputs,
-// and of bf16 ones).  A block that holds an infinity or a NaN gets E = 255
-// and reads back as NaN.
+// 1; x / 2^(E - 127) is rounded to the nearest code, ties to the even one (5
+// to 4), and magnitudes above 5 give 6 (the largest is below 8).  Dividing by a
+// power of two is exact, so a code does not depend on the precision it is
+// computed in, and a code times its scale is exact in fp16 and bf16 (of fp16
+// inputs, and of bf16 ones).  A block that holds an infinity or a NaN gets E =
+// 255 and reads back as NaN, also where the decode reads it.
 //
 // A pool is [num_pages][H_kv][page_size * 17 D / 32] bytes: per page and KV
 // head the codes of the page's rows, [page_size][D / 2] (channel 2 i in the
@@ -362,6 +362,8 @@ void kf_attn_decode_kv4_kernel(AttnParams p) {
                 r.scale[t] = scales[scale_off];
         }
     };
+    // (Exponent byte 255: the conversion takes the scale for a NaN, whatever the code, so
+    // a block that held no finite values makes its scores, or its channels of O, NaN.)
     auto scale_of = [&](const Rows& r, int t, int j) {
         return __uint_as_float((j < 4 ? r.scale[t] & 0xffu : r.scale[t] >> 8) << 23);
     };
