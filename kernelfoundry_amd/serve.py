@@ -14,8 +14,8 @@ kf_qk_norm_rope, kf_kv4_append, kf_kv4_read, kf_attn_decode_kv4).
 The entries run asynchronously on ``stream`` (default: torch's current one)
 and check their arguments on the host only; what device arrays hold
 (sequence starts, key counts, page ids) is bounded by the kernels.  They have
-no backward pass: an input that requires grad is refused while torch records
-gradients.  None of them has a counterpart in the reference.
+no derivatives: an input that requires grad is refused while torch records
+gradients, and one with a tangent always.  None of them has a counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -36,19 +36,27 @@ _STRIDES = {n: ctypes.c_int64 * n for n in (4, 6, 8)}
 # they compare by device index and identity, and look for words only when
 # something is wrong.
 def _gpu(torch, names, *tensors):
-    """The device of tensors that are all on one GPU and record no gradient."""
+    """The device of tensors (or None, but the first) that are all on one GPU and
+    record no gradient, backward or forward."""
     index = tensors[0].get_device()
     for t in tensors:
-        if t.get_device() != index or index < 0 or t.requires_grad:
+        if t is not None and (t.get_device() != index or index < 0 or t.requires_grad):
             break
     else:
-        return tensors[0].device
+        # Tangents exist only inside a level of forward-mode differentiation, whose
+        # number torch keeps in a variable (a call a tensor where it has none).
+        if getattr(torch.autograd.forward_ad, "_current_level", 0) < 0:
+            return tensors[0].device
     for name, t in zip(names, tensors):
+        if t is None:
+            continue
         if t.get_device() != index or index < 0:
             where = tensors[0].device if index >= 0 else "a GPU"
             raise ValueError(f"{name} must be a GPU tensor, on {where}")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad, but there is no backward pass: call under torch.no_grad()")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has a tangent, but there is no forward-mode derivative")
     return tensors[0].device
 
 
@@ -213,7 +221,7 @@ def qk_norm_rope(Q, K, positions, freqs, out=None, *, q_weight=None, k_weight=No
     """
     import torch
 
-    device = _gpu(torch, "QK", Q, K)
+    device = _gpu(torch, ("Q", "K", "q_weight", "k_weight", "freqs"), Q, K, q_weight, k_weight, freqs)
     flags = _half(torch, "QK", Q, K) | (KF_ROPE_INTERLEAVED if interleaved else 0)
     strides = (*_heads("Q", Q), *_heads("K", K))
     T, H_q, D = Q.shape
@@ -227,8 +235,7 @@ def qk_norm_rope(Q, K, positions, freqs, out=None, *, q_weight=None, k_weight=No
         wk = _weight(torch, "k_weight", k_weight, Q, D)
     rot = 0
     if freqs is not None:
-        if freqs.dtype is not torch.float64 or freqs.get_device() != device.index or freqs.dim() != 1 \
-                or not freqs.is_contiguous():
+        if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
             raise ValueError(f"freqs must be a contiguous float64 [rot / 2] tensor on {device}")
         rot, frq = 2 * freqs.shape[0], freqs.data_ptr()
         if positions is None:
@@ -252,8 +259,7 @@ def qk_norm_rope(Q, K, positions, freqs, out=None, *, q_weight=None, k_weight=No
 
 
 def _weight(torch, name, w, Q, D):
-    if w.dtype is not Q.dtype or w.requires_grad or w.get_device() != Q.get_device():
-        _gpu(torch, ("Q", name), Q, w)
+    if w.dtype is not Q.dtype:
         _half(torch, ("Q", name), Q, w)
     if w.shape != (D,) or not w.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of D elements")
