@@ -30,6 +30,7 @@ KF_BF16 = 16
 KF_ROPE_INTERLEAVED = 32
 
 _STRIDES = {n: ctypes.c_int64 * n for n in (4, 6, 8)}
+_WIDE_STRIDE = 1 << 28   # of tokens: the most that attn_packed takes of K and V
 
 
 # The checks below run on every call, and a small call's time is the host's:
@@ -77,7 +78,7 @@ def _heads(name, t):
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, D]")
     token, head, channel = t.stride()
-    if channel != 1 or token % 8 or head % 8:
+    if channel != 1 or token % 8 or head % 8 or token > _WIDE_STRIDE:
         tokens, heads, D = t.shape
         token, head = token if tokens > 1 else 0, head if heads > 1 else 0
         if (channel != 1 and D > 1) or token % 8 or head % 8:
@@ -128,9 +129,9 @@ def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, 
     """Attention over packed sequences.
 
     Q [T, H_q, D], K and V [T_kv, H_kv, D], float16 or bfloat16, D = 64, 128 or
-    256; views with other token and head strides (multiples of 8), as those of
-    a fused projection, are read in place.  ``seq_starts`` int32 [N + 1]: sequence b
-    has the tokens seq_starts[b] .. seq_starts[b + 1] - 1, none or more;
+    256; views with other token and head strides (multiples of 8, those of K's and V's
+    tokens at most 2^28), as those of a fused projection, are read in place.
+    ``seq_starts`` int32 [N + 1]: sequence b has the tokens seq_starts[b] .. seq_starts[b + 1] - 1, none or more;
     ``kv_starts`` the same for the keys (default: seq_starts).  ``causal`` is
     aligned to the last key: query i of n sees keys j <= i + keys - n.
     Returns O [T, H_q, D] (fp32, or ``out_dtype``), or (O, LSE [T, H_q]) with
