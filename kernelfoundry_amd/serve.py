@@ -11,8 +11,8 @@ kf_qk_norm_rope, kf_kv4_append, kf_kv4_read, kf_attn_decode_kv4).
     K, V = kv4_read(K_pages, V_pages, block_table, kv_starts, kv_lens, total, 128)
     O = attn_packed(Q, K, V, seq_starts, kv_starts=kv_starts, causal=True)     # a later chunk
 
-The entries run asynchronously on ``stream`` (default: torch's current one)
-and check their arguments on the host only; what device arrays hold
+The entries run asynchronously on ``stream``, one of the tensors' device (default:
+torch's current one), and check their arguments on the host only; what device arrays hold
 (sequence starts, key counts, page ids) is bounded by the kernels.  They have
 no derivatives: an input that requires grad is refused while torch records
 gradients, and one with a tangent always.  None of them has a counterpart in the reference.
@@ -112,6 +112,8 @@ def _like(torch, t, dtype, stream):
 
 def _launch(torch, device, stream, entry, *args):
     """entry(*args, stream) with `device` current: its streams are the current device's."""
+    if stream is not None and stream.device != device:
+        raise ValueError(f"stream must be a stream of {device}")
     if device.index == torch.cuda.current_device():
         st = entry(*args, _raw_stream(torch, stream, device))
     else:
@@ -131,9 +133,10 @@ def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, 
     Q [T, H_q, D], K and V [T_kv, H_kv, D], float16 or bfloat16, D = 64, 128 or
     256; views with other token and head strides (multiples of 8, those of K's and V's
     tokens at most 2^28), as those of a fused projection, are read in place.
-    ``seq_starts`` int32 [N + 1]: sequence b has the tokens seq_starts[b] .. seq_starts[b + 1] - 1, none or more;
-    ``kv_starts`` the same for the keys (default: seq_starts).  ``causal`` is
-    aligned to the last key: query i of n sees keys j <= i + keys - n.
+    ``seq_starts`` int32 [N + 1]: sequence b has the tokens seq_starts[b] ..
+    seq_starts[b + 1] - 1, none or more; ``kv_starts`` the same for the keys
+    (default: seq_starts).  ``causal`` is aligned to the last key: query i of n
+    sees keys j <= i + keys - n.
     Returns O [T, H_q, D] (fp32, or ``out_dtype``), or (O, LSE [T, H_q]) with
     ``return_lse``; a row without keys gets O = 0, LSE = -inf.  Rows outside
     the sequences are not written.
