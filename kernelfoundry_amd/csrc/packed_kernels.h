@@ -267,8 +267,7 @@ void kf_attn_packed_kernel(PackedParams p) {
     sq.kn = __builtin_amdgcn_readfirstlane(sq.kn);
     const int ratio = p.ratio, R = sq.qn * ratio, klen = sq.kn;
     const float c = p.scale_log2;
-    // Causal: waves w and w + 4 share a SIMD; blocks w and 7 - w.
-    const int wave = KS > 1 ? wave_id % kRowWaves : (NW == 8 && p.causal && wave_id >= 4) ? 11 - wave_id : wave_id;
+    const int wave = KS > 1 ? wave_id % kRowWaves : wave_id;
     const int kgrp = KS > 1 ? wave_id / kRowWaves : 0;
     const auto limit = [&](int row) {  // keys that the row sees
         return p.causal ? min(max(row / ratio + klen - sq.qn + 1, 0), klen) : klen;
