@@ -269,6 +269,8 @@ void kf_attn_packed_kernel(PackedParams p) {
     const float c = p.scale_log2;
     const int wave = KS > 1 ? wave_id % kRowWaves : wave_id;
     const int kgrp = KS > 1 ? wave_id / kRowWaves : 0;
+    // (Of starts in no order the sums by which the tile was found may wrap.)
+    if ((unsigned)rt * (unsigned)kRows >= (unsigned)R) return;
     const auto limit = [&](int row) {  // keys that the row sees
         return p.causal ? min(max(row / ratio + klen - sq.qn + 1, 0), klen) : klen;
     };
