@@ -15,7 +15,9 @@ The entries run asynchronously on ``stream``, one of the tensors' device (defaul
 torch's current one), and check their arguments on the host only; what device arrays hold
 (sequence starts, key counts, page ids) is bounded by the kernels.  They have
 no derivatives: an input that requires grad is refused while torch records
-gradients, and one with a tangent always.  None of them has a counterpart in the reference.
+gradients, and one with a tangent always.  A call needs at least one token, sequence,
+row of K and V and page (else KfError, KF_ERR_SIZE); a sequence among others may be
+empty.  None of them has a counterpart in the reference.
 """
 from __future__ import annotations
 

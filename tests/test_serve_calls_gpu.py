@@ -54,3 +54,24 @@ def test_an_input_with_a_tangent_is_refused():
         with pytest.raises((ValueError, RuntimeError)):
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
             pytest.fail(name)
+
+
+def test_calls_without_tokens_rows_or_pages_are_refused():
+    Kp, Vp, table, _, _ = fill([20], 2, 128, 16)
+    Q, K, s, n, f = normal(20, 8, 128), normal(20, 2, 128), ints([0, 20]), ints([20]), kf.rope_freqs(128, device="cuda")[0]
+    none = ints([0, 0])
+    for call in (lambda: kf.attn_packed(Q[:0], K, K, none, kv_starts=s), lambda: kf.attn_packed(Q, K[:0], K[:0], s, kv_starts=none),
+                 lambda: kf.qk_norm_rope(Q[:0], K[:0], n[:0], f), lambda: kf.kv4_append(K[:0], K[:0], Kp, Vp, table, none, n),
+                 lambda: kf.kv4_append(K, K, Kp, Vp, table[:, :0].contiguous(), s, n),
+                 lambda: kf.kv4_append(K, K, Kp[:0], Vp[:0], table, s, n),
+                 lambda: kf.kv4_read(Kp, Vp, table, none, n, 0, 128),
+                 lambda: kf.attn_decode_kv4(Q[:0, :, None], Kp, Vp, table[:0], n[:0]),
+                 lambda: kf.attn_decode_kv4(Q[:1, :, None], Kp[:0], Vp[:0], table, n)):
+        with pytest.raises(kf.KfError) as e:
+            call()
+        assert e.value.status == kf.KF_ERR_SIZE
+    with pytest.raises(ValueError):
+        kf.attn_packed(Q, K, K, s[:1])
+    # Sequences without tokens or keys among others.
+    O, LSE = kf.attn_packed(Q, K, K, ints([0, 0, 20, 20]), kv_starts=ints([0, 20, 20, 20]), return_lse=True)
+    assert (O == 0).all() and (LSE == -float("inf")).all()
