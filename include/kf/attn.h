@@ -289,7 +289,16 @@ int kf_attn_decode_paged(const void* Q, const void* K_pages, const void* V_pages
  *   Rows of tokens outside the sequences are left as they were.
  * What tokens outside the sequences and other sequences hold does not matter; a
  * NaN or an infinity among a sequence's own keys or values may reach any row of
- * that sequence, also one that does not see it.
+ * that sequence, also one that does not see it.  The statistics of a row that one
+ * has reached mean nothing: its LSE may be NaN, or -inf as of a row without keys.
+ * The softmax weights are rounded to the inputs' type before they meet V (relative
+ * 2^-11 in fp16, 2^-8 in bf16, whatever O's type), since that product takes 16-bit
+ * operands; Li and the LSE sum them in fp32.
+ * Scores q . k / sqrt(D) may reach 9e7 in magnitude; from there on their fp32 rounding
+ * can pass the range of a 16-bit weight, and rows may be NaN.
+ * The sizes choose one of several layouts, which add up in different orders: a
+ * sequence's last bits may differ between batches of other sizes, but not between
+ * calls of the same sizes.
  * tokens_q, tokens_kv and n_seqs are positive; tokens_q H_q, tokens_kv H_kv and
  * tokens_kv H_q / H_kv are at most 2^31 - 1025.  No workspace. */
 int kf_attn_packed(const void* Q, const void* K, const void* V, void* O,
@@ -315,7 +324,8 @@ int kf_attn_packed(const void* Q, const void* K, const void* V, void* O,
  *   (i, i + rot / 2) or, with KF_ROPE_INTERLEAVED, (2i, 2i + 1), and multiplied
  *   by `scale`; the others keep their normed values.
  * positions: device int [tokens].  positions and freqs may be NULL if rot is 0.
- * Computed in fp32 (the angles in fp64) and rounded once. */
+ * Computed in fp32 (the angles in fp64) and rounded once; the squares of a normed
+ * bf16 row whose root mean square is above 1e18 pass fp32's range. */
 int kf_qk_norm_rope(const void* Q, const void* K, void* Q_out, void* K_out,
                     const int64_t* strides, const void* q_weight, const void* k_weight,
                     const int* positions, const double* freqs,
@@ -375,7 +385,8 @@ int kf_kv4_read(const void* K_pages, const void* V_pages, const int* block_table
  * to bf16 before they meet V, else to fp16; K and V are exactly what kf_kv4_read
  * with the same flags gives.  So a block with E = 255 is NaN: it makes the rows that
  * see its key NaN, or their 32 channels, and may reach any other row of its sequence, as
- * in kf_attn_packed; what pages hold past a sequence's keys does not matter. */
+ * in kf_attn_packed; what pages hold past a sequence's keys does not matter.  Statistics
+ * of such rows, the size of scores and the order of sums: as in kf_attn_packed. */
 size_t kf_attn_decode_kv4_workspace_bytes(int B, int q_len, int H_q, int H_kv, int D,
                                           int page_size, int max_pages_per_seq);
 int kf_attn_decode_kv4(const void* Q, const void* K_pages, const void* V_pages,

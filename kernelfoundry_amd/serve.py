@@ -141,7 +141,8 @@ def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, 
     sees keys j <= i + keys - n.
     Returns O [T, H_q, D] (fp32, or ``out_dtype``), or (O, LSE [T, H_q]) with
     ``return_lse``; a row without keys gets O = 0, LSE = -inf.  Rows outside
-    the sequences are not written.
+    the sequences are not written.  The softmax weights are rounded to the inputs' type
+    before they meet V; scores q . k / sqrt(D) may reach 9e7.
     """
     import torch
 
@@ -180,7 +181,9 @@ def rope_freqs(rot, base=10000.0, *, scaling=None, factor=1.0, original_len=None
               interpolated, the highest kept;
     "yarn"    by the turns f_i makes over ``original_len`` positions: kept from
               beta_fast turns on, interpolated up to beta_slow, in between
-              linearly mixed; the rotated channels times 1 + ln(factor) / 10.
+              linearly mixed; the rotated channels times 1 + ln(factor) / 10.  The
+              mix is linear in the turns; a checkpoint that was tuned with one linear
+              in the channel index brings its own frequencies.
     """
     import torch
 
@@ -380,7 +383,9 @@ def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, caus
     Q [B, H_q, q_len, D] float16 or bfloat16, at most 32 query rows per KV head
     (H_q / H_kv * q_len); the other arguments and the results are those of
     attn_decode_paged: O [B, H_q, q_len, D] fp32 or ``out_dtype``, (O, LSE) with
-    ``return_lse``.  ``workspace``: a buffer of kv4_workspace_bytes to use
+    ``return_lse``.  The softmax weights are rounded to Q's type before they meet V.
+    K and V are what kv4_read with Q's type gives (fp16 cannot hold all of a cache
+    written from bfloat16).  ``workspace``: a buffer of kv4_workspace_bytes to use
     instead of a new one.
     """
     import torch
