@@ -234,9 +234,9 @@ void kf_kv4_read_kernel(Kv4Params p) {
 // have consumed K(t), V(t + 1) when V(t) has gone to LDS.
 //
 // Bound by memory: with the loads alone it takes as long.  32 / 8 heads, D = 128, both
-// launches: 32 x 8192 keys (285 MB) 58 us, 4.9 TB/s, the stages themselves at 6.2;
-// 8 x 50000 to 65536, 4 queries each, bf16 (506 MB) 90 to 93, 5.4 to 5.6; 32 x 512
-// to 8192 (84 MB) 25; 1 x 4096 (4.5 MB) 9.  About 10 us are fixed: the launch
+// launches: 32 x 8192 keys (285 MB) 58 us, 4.9 TB/s, the stages themselves at 6.2
+// (63 with pages of 16 rows); 8 x 50000 to 65536, 4 queries each, bf16 (506 MB) 88 to
+// 93, 5.4 to 5.7; 32 x 512 to 8192 (84 MB) 25; 1 x 4096 (4.5 MB) 9.  About 10 us are fixed: the launch
 // 2.3, key counts, page ids and first rows one after the other 1.3 to 3.3, the
 // LDS merge 2, the merge launch 3 to 5.  The scale bytes, a row's 4 to 16, cost 2
 // to 10 % of the stages' time.  Tried: 64 keys a trip (spills with three
@@ -245,6 +245,9 @@ void kf_kv4_read_kernel(Kv4Params p) {
 // ---------------------------------------------------------------------------
 // NQ: 16-row blocks of queries.  Two for more than 16 rows alone: their registers and
 // LDS leave a third fewer workgroups (16 rows on two blocks 58 -> 72 us, 93 -> 123).
+// With 32 rows, 8 queries a sequence, 32 x 8192 keys take 77 to 79 us and 8 x 57000 (496
+// MB) 123 to 129; with 32 / 1 heads 64 x 8192 (71 MB) 32 and 8 x 16384 (18 MB) 20, of
+// which a wave's share is two stages and the partials half as many bytes as the keys.
 template <int D, int NQ> struct Kv4Cfg {
     static constexpr int kWaves = 4;                          // workers per workgroup
     static constexpr int kThreads = 64 * kWaves;
@@ -454,7 +457,7 @@ void kf_attn_decode_kv4_kernel(AttnParams p) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) e[r] = exp2_hw(fmaf(s[n][r >> 2][r & 3], c, neg_m));
             rs.l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-            pb[n] = round8<kBF>(e);
+            pb[n] = round8<kBF>(e);    // as the product takes it (see packed_exp); summed in fp32
         }
         // V rows to LDS (chunks XOR-swizzled by the row), back as V^T.
 #pragma unroll

@@ -12,12 +12,16 @@
 // -> LDS by LDS-DMA, P^T straight from the score registers.
 //
 // Bound by the matrix units and the softmax between their products: causal, 32 / 8
-// heads, D = 128, 1 x 8192 bf16 takes 500 to 545 us, 1.0 to 1.1 PFLOP/s (a library
-// product 1.2), MFMA busy 59 % of the SIMD cycles, LDS 30 %, next to no bank
-// conflicts; 16 sequences of 16 to 4096 117 to 122 us (0.76 PFLOP/s), of which
-// a workgroup's first loads and its store (191 MB in all, 38 us of memory time) hide
-// behind other workgroups' products in part; 4 x 512 queries against 4096
-// keys, 16 / 4 heads, D = 256, 150 (0.86 PFLOP/s).  Tried: 64 rows a wave on 8 waves
+// heads, D = 128, 1 x 8192 takes 507 to 518 us in bf16 and 545 in fp16, 1.0 to 1.1
+// PFLOP/s (a library product 1.2), MFMA busy 59 % of the SIMD cycles, LDS 30 %, next to
+// no bank conflicts; 16 sequences of 16 to 4096 111 to 119 us (0.77 to 0.82 PFLOP/s), of
+// which a workgroup's first loads and its store (191 MB in all, 38 us of memory time)
+// hide behind other workgroups' products in part; 4 x 512 queries against 4096
+// keys, 16 / 4 heads, D = 256, 146 to 154 (0.84 to 0.88).  1 x 4096 in fp16: 144 us at 32
+// / 8 heads of 128 (0.95; with fp32 output 146), 91 at 32 / 1 of 64 (0.76), 165 to 169
+// at 16 / 4 of 256 (0.81 to 0.83), 276 at 32 / 8 of 256 (0.99); without the mask 283 at 32 / 8 of
+// 128 (0.97), 164 at 32 / 8 of 64 (0.84), 268 at 16 / 4 of 256 (1.03).  What bounds
+// D = 64 is not measured.  Tried: 64 rows a wave on 8 waves
 // (4 to 6 % faster at 8192, 5 to 40 % slower at the others), the scores of the next
 // stage beside this one's products (its third buffer costs a workgroup a CU: no gain),
 // stages requested two tiles ahead (no change), two V tiles before the softmax at
@@ -56,11 +60,12 @@ template <int D, int NW, int KS> struct PackedCfg {
     // 74.3 -> 65.3; full grids lose 1 %).
     static constexpr int kBatch = D == 256 ? 4 : KS == 1 ? 2 : D / 16;
     static constexpr int kAhead = D == 256 ? 0 : KS == 1 ? 1 : D / 32;
-    // Kept apart from the scheduler, which without KV groups does up to 1 % better by itself.
+    // Kept apart from the scheduler; without KV groups it does as well by itself (1 x 8192,
+    // 32 / 8 heads, D = 128: bf16 518 and 514 us, no more than two runs differ by).
     static constexpr bool kOrder = KS > 1 && D < 256;
     // Stages copied in asm, from a scalar row and lane offsets that stay in registers; the
-    // builtin's offsets, computed for every stage, cost 1 to 4 % (1 x 8192, 32 / 8 heads,
-    // D = 128, bf16 518 -> 505 us; 1 x 4096, 32 / 1 heads, D = 64, 92.4 -> 88.2). At
+    // builtin's offsets, computed for every stage, cost 2 to 3 % (1 x 8192, 32 / 8 heads,
+    // D = 128, bf16 524 -> 512 us; 1 x 4096, 32 / 1 heads, D = 64, 93.2 -> 90.2). At
     // D = 256 there are no registers for them: spills, and no gain without.
     static constexpr bool kAsmCopy = D < 256;
     // The per-lane LDS offsets of a tile derived from one, for want of registers.
@@ -147,8 +152,10 @@ __device__ __forceinline__ bool packed_find(const PackedParams& p, int lane, int
     }
 }
 
-// exp2 and 16-bit pack of a 32-row score block; the fp32 values are summed, so
-// that the log-sum-exp has their precision.
+// exp2 and 16-bit pack of a 32-row score block.  The product with V takes 16-bit
+// operands, so the weights are rounded (relative 2^-11 or 2^-8: with O's own
+// rounding 1.2 to 1.4 times the error of weights kept in fp32); the fp32 values are
+// summed, so that the log-sum-exp has their precision.
 template <bool kBF>
 __device__ __forceinline__ void packed_exp(const f32x16& s, float scale_log2, float neg_m,
                                            typename Elem<kBF>::x8 (&p)[2], float& acc) {

@@ -78,8 +78,8 @@ __device__ __forceinline__ float row_sum(float v) {
 // and cosines are the same for all its rows.  Bound by memory: kAhead passes' rows
 // are requested together, the first ones before the angles; the stores, which
 // nothing here reads again, go past the caches.  17918 tokens of 32 + 8 heads, D =
-// 128 (367 MB): 79.5 us, 4.6 TB/s, where a copy reaches 4.8; one pass ahead 94,
-// three 89 (registers), cached stores 84.6.
+// 128 (367 MB): 76.5 us, 4.8 TB/s, as a copy reaches.  Where this form took 79.5,
+// one pass ahead took 94, three 89 (registers), cached stores 84.6.
 template <bool kBF, int D, int kTokens>
 __global__ __launch_bounds__(64 * kRopeWaves)
 void kf_qk_norm_rope_kernel(RopeParams p) {

@@ -112,6 +112,9 @@ int launch_packed(kf::PackedParams& prm, long long rows, hipStream_t stream) {
 // layout it picks is 1.1 % slower than the best of these at the geometric mean,
 // 14 % at worst).  Always the first layout would be 16 % slower: 1 x 512 queries
 // against 4096 keys, 32 / 8 heads, D = 128, take 96, 58 and 53 us in the three.
+// The averages say little of a batch of very unequal lengths, whose longest chain is
+// then underrated: 1 x 2048 queries beside 31 x 1, 8 / 8 heads, D = 128, take 50 us in
+// the first layout, where the 2048 alone get KV groups and take 28.
 struct PackedLayout {
     int rows, kv_groups;
     double start, chain, workgroup, tile;
