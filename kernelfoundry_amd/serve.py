@@ -25,7 +25,7 @@ import ctypes
 import functools
 import math
 
-from . import (KF_ATTN_CAUSAL, KF_ERR_HIP, KF_OK, KfError, _new, _out_flags, _output, _raw_stream,
+from . import (KF_ATTN_CAUSAL, KF_ERR_HIP, KF_ERR_SIZE, KF_OK, KfError, _new, _out_flags, _output, _raw_stream,
                _workspace, load_library, status_string)
 
 KF_BF16 = 16
@@ -33,6 +33,7 @@ KF_ROPE_INTERLEAVED = 32
 
 _STRIDES = {n: ctypes.c_int64 * n for n in (4, 6, 8)}
 _WIDE_STRIDE = 1 << 28   # of tokens: the most that attn_packed takes of K and V
+_MOST = 2 ** 31 - 1      # a size of the C entries: an int, to which ctypes cuts without a word
 
 
 # The checks below run on every call, and a small call's time is the host's:
@@ -112,6 +113,10 @@ def _like(torch, t, dtype, stream):
     return _new(torch, t.shape, dtype, t.device, stream)
 
 
+def _too_many():
+    return KfError(KF_ERR_SIZE, status_string(KF_ERR_SIZE))
+
+
 def _launch(torch, device, stream, entry, *args):
     """entry(*args, stream) with `device` current: its streams are the current device's."""
     if stream is not None and stream.device != device:
@@ -154,6 +159,9 @@ def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, 
     if V.shape != K.shape or Dk != D:
         raise ValueError("K and V must be [T_kv, H_kv, D], with Q's D")
     starts = kstarts = _starts(torch, "seq_starts", seq_starts, device)
+    n = seq_starts.shape[0] - 1
+    if T > _MOST or T_kv > _MOST or H_q > _MOST or H_kv > _MOST or n > _MOST:
+        raise _too_many()
     if kv_starts is not None:
         kstarts = _ints(torch, "kv_starts", kv_starts, device, seq_starts.shape)
     if out is None:
@@ -165,7 +173,7 @@ def attn_packed(Q, K, V, seq_starts, out=None, *, kv_starts=None, causal=False, 
         flags |= KF_ATTN_CAUSAL
     _launch(torch, device, stream, load_library().kf_attn_packed,
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, None,
-            strides, starts, kstarts, seq_starts.shape[0] - 1, T, T_kv, H_q, H_kv, D, flags)
+            strides, starts, kstarts, n, T, T_kv, H_q, H_kv, D, flags)
     return (out, lse) if return_lse else out
 
 
@@ -237,6 +245,8 @@ def qk_norm_rope(Q, K, positions, freqs, out=None, *, q_weight=None, k_weight=No
     T_k, H_kv, Dk = K.shape
     if T_k != T or Dk != D:
         raise ValueError("K must be [T, H_kv, D], with Q's T and D")
+    if T > _MOST or H_q > _MOST or H_kv > _MOST:
+        raise _too_many()
     wq = wk = pos = frq = None
     if q_weight is not None:
         wq = _weight(torch, "q_weight", q_weight, Q, D)
@@ -325,9 +335,12 @@ def kv4_append(K, V, K_pages, V_pages, block_table, seq_starts, kv_lens, *, stre
         raise ValueError("K and V must be [T, H_kv, D], with the pools' H_kv")
     starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
     table, lens = _table(torch, block_table, kv_lens, device, n)
+    max_pages = block_table.shape[1]
+    if T > _MOST or H_kv > _MOST or n > _MOST or max_pages > _MOST:
+        raise _too_many()
     _launch(torch, device, stream, load_library().kf_kv4_append,
             K.data_ptr(), V.data_ptr(), strides, K_pages.data_ptr(), V_pages.data_ptr(), table, starts, lens, n, T,
-            H_kv, D, page_size, block_table.shape[1], num_pages, flags)
+            H_kv, D, page_size, max_pages, num_pages, flags)
 
 
 def kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, total, D, out=None, *, out_dtype=None,
@@ -349,6 +362,9 @@ def kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, total, D, out=N
     num_pages, H_kv, page_size = _pages(torch, K_pages, V_pages, D)
     starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
     table, lens = _table(torch, block_table, kv_lens, device, n)
+    max_pages = block_table.shape[1]
+    if total > _MOST or n > _MOST or max_pages > _MOST:
+        raise _too_many()
     shape = (total, H_kv, D)
     if out is None:
         K = _new_at(torch, K_pages, shape, dtype, stream)
@@ -357,7 +373,7 @@ def kv4_read(K_pages, V_pages, block_table, seq_starts, kv_lens, total, D, out=N
         K, V = (_output(torch, x, shape, dtype, device, stream) for x in out)
     _launch(torch, device, stream, load_library().kf_kv4_read,
             K_pages.data_ptr(), V_pages.data_ptr(), table, starts, lens, K.data_ptr(), V.data_ptr(), n, total, H_kv, D,
-            page_size, block_table.shape[1], num_pages, KF_BF16 if dtype is torch.bfloat16 else 0)
+            page_size, max_pages, num_pages, KF_BF16 if dtype is torch.bfloat16 else 0)
     return K, V
 
 
@@ -398,6 +414,8 @@ def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, caus
     num_pages, H_kv, page_size = _pages(torch, K_pages, V_pages, D)
     table, lens = _table(torch, block_table, kv_lens, device, B)
     max_pages = block_table.shape[1]
+    if max_pages > _MOST:
+        raise _too_many()
     if out is None:
         out = _like(torch, Q, out_dtype or torch.float32, stream)
     else:
