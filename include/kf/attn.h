@@ -62,7 +62,7 @@ enum kf_status {
 #define KF_ATTN_OUT_BF16 4 /* O is written as bf16 (RNE of the fp32 result)     */
 #define KF_ATTN_LSE 8      /* row_max receives LSE = Mi + ln(Li) (natural log;
                               -inf for a row without keys); row_sumexp unused */
-/* kf_attn_packed, kf_qk_norm_rope, kf_kv4_* and kf_attn_decode_kv4 flags. */
+/* Flags of kf_attn_packed and the entry points after it. */
 #define KF_BF16 16         /* 16-bit inputs (and the cache's 16-bit side) are bf16,
                               not fp16                                          */
 #define KF_ROPE_INTERLEAVED 32 /* kf_qk_norm_rope: pairs (2i, 2i + 1), not
@@ -265,7 +265,7 @@ int kf_attn_decode_paged(const void* Q, const void* K_pages, const void* V_pages
                          int page_size, int max_pages_per_seq, int num_pages, int flags,
                          void* workspace, size_t workspace_bytes, void* stream);
 
-/* The entry points from here to kf_attn_decode_kv4: a call of which a launch would
+/* The entry points from here to kf_kv_evict: a call of which a launch would
  * have 2^32 threads or more is KF_ERR_SIZE, before anything is launched. */
 
 /* Attention over packed sequences: the tokens of all sequences one after the
@@ -395,6 +395,94 @@ int kf_attn_decode_kv4(const void* Q, const void* K_pages, const void* V_pages,
                        int B, int q_len, int H_q, int H_kv, int D,
                        int page_size, int max_pages_per_seq, int num_pages, int flags,
                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* A paged K/V cache in 16 bits that is filled, attended to and kept small.  No
+ * counterpart in the reference.
+ *
+ * K_pages, V_pages: [num_pages, H_kv, page_size, D] fp16 or bf16 page pools, as in
+ *   kf_attn_decode_paged, which reads an fp16 one too.  D = 64, 128 or 256;
+ *   page_size a power of two in [16, 2^20].
+ * weights: [num_pages, H_kv, page_size] fp32, what every key has gathered
+ *   (kf_kv_weigh), by the same block table.
+ * block_table: device int [n_seqs, max_pages_per_seq], as in kf_attn_decode_paged;
+ *   kv_lens: device int [n_seqs], the keys of each sequence, clamped to the
+ *   table's places; seq_starts: device int [n_seqs + 1], as in kf_attn_packed:
+ *   sequence b's packed tokens are the last of its kv_lens[b] keys.
+ * Sequences may share pages that are only read. */
+
+/* Write the new tokens' K and V into the cache: kf_kv4_append's call for 16-bit
+ * pages, copied bit for bit, so that fp16 and bf16 are alike (`flags`: 0 or KF_BF16).
+ * weights: NULL, or the pool in which the new tokens' weights become 0. */
+int kf_kv_append(const void* K, const void* V, const int64_t* strides,
+                 void* K_pages, void* V_pages, float* weights, const int* block_table,
+                 const int* seq_starts, const int* kv_lens,
+                 int n_seqs, int tokens, int H_kv, int D,
+                 int page_size, int max_pages_per_seq, int num_pages,
+                 int flags, void* stream);
+
+/* Attention of packed new tokens over the pages, their own keys among them (append
+ * first): a step of one token, a chunk of a prompt over its context, or any mix.
+ *
+ * Q [tokens, H_q, D] fp16 (bf16 with KF_BF16, as the pools); `strides`: NULL
+ *   (contiguous), or two host values, Q's token and head strides in elements,
+ *   multiples of 8.  O [tokens, H_q, D], row_max, row_sumexp, flags (KF_ATTN_CAUSAL,
+ *   _OUT_F16, _OUT_BF16, _LSE, KF_BF16) and what they give as in kf_attn_packed,
+ *   the keys of sequence b being kv_lens[b]: query i of n sees keys j <= i +
+ *   kv_lens[b] - n with KF_ATTN_CAUSAL.  A key whose page id is outside [0,
+ *   num_pages) counts as none, and is never read; what pages hold past a
+ *   sequence's keys does not matter.  NaN and infinities among a sequence's own
+ *   keys, the size of scores, the rounding of the weights and the order of sums: as in
+ *   kf_attn_packed; a sequence's keys are cut where the work of the whole call is
+ *   shared out, so that its last bits depend on the other sequences' lengths.
+ * Workspace: kf_attn_paged_workspace_bytes() bytes (may be 0, then NULL will do),
+ *   256-byte aligned, no initialisation, not shared by calls that can run
+ *   concurrently; KF_ERR_WORKSPACE without.
+ * n_seqs, tokens and tokens H_q as in kf_attn_packed. */
+size_t kf_attn_paged_workspace_bytes(int n_seqs, int tokens, int H_q, int H_kv, int D,
+                                     int page_size, int max_pages_per_seq);
+int kf_attn_paged(const void* Q, const int64_t* strides, const void* K_pages, const void* V_pages,
+                  const int* block_table, const int* seq_starts, const int* kv_lens,
+                  void* O, float* row_max, float* row_sumexp,
+                  int n_seqs, int tokens, int H_q, int H_kv, int D,
+                  int page_size, int max_pages_per_seq, int num_pages, int flags,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* The attention weight that the keys gather:
+ *   weights[key j] += sum over the new tokens i that see j and the query heads of the
+ *   KV head's group of exp(q_i . k_j / sqrt(D) - lse_i),
+ * in fp32 (the products' sums too), in an order that the sizes and lengths fix.
+ * Q, strides, K_pages, tables and counts as in kf_attn_paged, of which lse
+ * [tokens, H_q] is the row_max with KF_ATTN_LSE (natural logarithm); a row whose lse
+ * is -inf adds nothing.  flags: KF_ATTN_CAUSAL, KF_BF16.  A NaN or an infinity in a
+ * row of Q, in its lse, or in a key reaches the keys that the row sees, or the key's
+ * own weight.  Sequences that share a page race for its weights: they must not. */
+int kf_kv_weigh(const void* Q, const int64_t* strides, const void* K_pages, float* weights,
+                const int* block_table, const int* seq_starts, const int* kv_lens,
+                const float* lse, int n_seqs, int tokens, int H_q, int H_kv, int D,
+                int page_size, int max_pages_per_seq, int num_pages, int flags, void* stream);
+
+/* Cut every sequence from n = kv_lens[b] to m = min(n, budgets[b]) keys (device int
+ * [n_seqs], a negative one counts as 0).  Of every KV head the last r = min(recent, m)
+ * keys stay, and of the n - r before them the k = m - r of largest weight, ties to
+ * the lowest place; a NaN counts as larger than any number, -0 as 0.
+ * Attention does not depend on the order of the keys, and the new order is the one of
+ * fewest moves: kept keys in places below k stay there, those from k on go, in
+ * order, to the freed places below k, in order, and the last r to k .. m - 1.  K, V and
+ * weights move alike; places from m on are left as they were.
+ * kept: device int [n_seqs], receives m, or n where nothing is cut or a page id of the
+ *   n keys is outside [0, num_pages): such a sequence is left as it is.  It may be
+ *   kv_lens or budgets itself.
+ * Sequences that are cut must not share a page with another one of the call, nor
+ *   have one twice: what these pages hold is then undefined.
+ * Workspace: kf_kv_evict_workspace_bytes() bytes, 256-byte aligned, no initialisation,
+ *   not shared by calls that can run concurrently. */
+size_t kf_kv_evict_workspace_bytes(int n_seqs, int H_kv, int D, int page_size,
+                                   int max_pages_per_seq);
+int kf_kv_evict(void* K_pages, void* V_pages, float* weights, const int* block_table,
+                const int* kv_lens, const int* budgets, int* kept,
+                int n_seqs, int H_kv, int D,
+                int page_size, int max_pages_per_seq, int num_pages, int recent,
+                void* workspace, size_t workspace_bytes, void* stream);
 
 /* The reference launcher's contract (tests/test_flash_attn.cu:52-113):
  * q_len = kv_len = S, scratch allocated and freed by the call, stream

@@ -21,7 +21,8 @@
 //       no counterpart in the reference.
 //
 //   kf::attn_packed(...), kf::qk_norm_rope(...), kf::kv4_append(...),
-//   kf::kv4_read(...), kf::attn_decode_kv4(...)
+//   kf::kv4_read(...), kf::attn_decode_kv4(...), kf::kv_append(...),
+//   kf::attn_paged(...), kf::kv_weigh(...), kf::kv_evict(...)
 //       the same over the serving entry points of kf/attn.h.
 #pragma once
 
@@ -327,6 +328,59 @@ inline hipError_t attn_decode_kv4(const uint16_t* Q, const uint8_t* K_pages, con
         return kf_attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, O, Mi, Li, B, q_len,
                                   H_q, H_kv, D, page_size, max_pages_per_seq, num_pages, flags, ws,
                                   ws_bytes, static_cast<void*>(stream));
+    });
+}
+
+// kf_kv_append: new tokens into the paged 16-bit cache.
+inline hipError_t kv_append(const uint16_t* K, const uint16_t* V, const int64_t* strides,
+                            uint16_t* K_pages, uint16_t* V_pages, float* weights,
+                            const int* block_table, const int* seq_starts, const int* kv_lens,
+                            int n_seqs, int tokens, int H_kv, int D, int page_size,
+                            int max_pages_per_seq, int num_pages, int flags, hipStream_t stream) {
+    return status_to_hip(kf_kv_append(K, V, strides, K_pages, V_pages, weights, block_table,
+                                      seq_starts, kv_lens, n_seqs, tokens, H_kv, D, page_size,
+                                      max_pages_per_seq, num_pages, flags,
+                                      static_cast<void*>(stream)));
+}
+
+// kf_attn_paged with the per-thread cached workspace.
+inline hipError_t attn_paged(const uint16_t* Q, const int64_t* strides, const uint16_t* K_pages,
+                             const uint16_t* V_pages, const int* block_table,
+                             const int* seq_starts, const int* kv_lens, void* O, int n_seqs,
+                             int tokens, int H_q, int H_kv, int D, int page_size,
+                             int max_pages_per_seq, int num_pages, int flags, hipStream_t stream,
+                             float* Mi = nullptr, float* Li = nullptr) {
+    const size_t need = kf_attn_paged_workspace_bytes(n_seqs, tokens, H_q, H_kv, D, page_size,
+                                                      max_pages_per_seq);
+    return with_workspace(stream, need, [&] { return need; }, [&](void* ws, size_t ws_bytes) {
+        return kf_attn_paged(Q, strides, K_pages, V_pages, block_table, seq_starts, kv_lens, O, Mi,
+                             Li, n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq,
+                             num_pages, flags, ws, ws_bytes, static_cast<void*>(stream));
+    });
+}
+
+// kf_kv_weigh: the attention weight that keys gather.
+inline hipError_t kv_weigh(const uint16_t* Q, const int64_t* strides, const uint16_t* K_pages,
+                           float* weights, const int* block_table, const int* seq_starts,
+                           const int* kv_lens, const float* lse, int n_seqs, int tokens, int H_q,
+                           int H_kv, int D, int page_size, int max_pages_per_seq, int num_pages,
+                           int flags, hipStream_t stream) {
+    return status_to_hip(kf_kv_weigh(Q, strides, K_pages, weights, block_table, seq_starts,
+                                     kv_lens, lse, n_seqs, tokens, H_q, H_kv, D, page_size,
+                                     max_pages_per_seq, num_pages, flags,
+                                     static_cast<void*>(stream)));
+}
+
+// kf_kv_evict with the per-thread cached workspace, which it cannot do without.
+inline hipError_t kv_evict(uint16_t* K_pages, uint16_t* V_pages, float* weights,
+                           const int* block_table, const int* kv_lens, const int* budgets,
+                           int* kept, int n_seqs, int H_kv, int D, int page_size,
+                           int max_pages_per_seq, int num_pages, int recent, hipStream_t stream) {
+    const size_t need = kf_kv_evict_workspace_bytes(n_seqs, H_kv, D, page_size, max_pages_per_seq);
+    return with_workspace(stream, need, [&] { return need; }, [&](void* ws, size_t ws_bytes) {
+        return kf_kv_evict(K_pages, V_pages, weights, block_table, kv_lens, budgets, kept, n_seqs,
+                           H_kv, D, page_size, max_pages_per_seq, num_pages, recent, ws, ws_bytes,
+                           static_cast<void*>(stream));
     });
 }
 

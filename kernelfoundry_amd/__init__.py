@@ -27,6 +27,9 @@ Interface, mirroring the reference harness (sviraaj/kernelfoundry):
   ``kv4_read``, ``attn_decode_kv4`` -- what a server runs beside these: packed
   prompts, head norms with rotary positions, a paged cache in 4 bits and the
   decode over it (serve.py; no reference counterpart).
+* ``kv_append``, ``attn_paged``, ``kv_weigh``, ``kv_evict`` -- a paged 16-bit cache
+  that is filled, attended to by chunks and steps, and cut to the keys that
+  gathered the most attention (serve.py; no reference counterpart).
 """
 from __future__ import annotations
 
@@ -47,6 +50,7 @@ __all__ = [
     "workspace_bytes_least", "kernel_names",
     "KF_BF16", "KF_ROPE_INTERLEAVED", "attn_packed", "rope_freqs", "qk_norm_rope", "kv4_page_bytes",
     "kv4_append", "kv4_read", "kv4_workspace_bytes", "attn_decode_kv4",
+    "kv_append", "attn_paged", "paged_attn_workspace_bytes", "kv_weigh", "kv_evict", "evict_workspace_bytes",
 ]
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -176,6 +180,18 @@ def load_library(path: str = LIB_PATH):
     lib.kf_attn_decode_kv4_workspace_bytes.restype = sz
     lib.kf_attn_decode_kv4.argtypes = [p] * 8 + [i] * 9 + [p, sz, p]
     lib.kf_attn_decode_kv4.restype = i
+    lib.kf_kv_append.argtypes = [p, p, i64s] + [p] * 6 + [i] * 8 + [p]
+    lib.kf_kv_append.restype = i
+    lib.kf_attn_paged_workspace_bytes.argtypes = [i] * 7
+    lib.kf_attn_paged_workspace_bytes.restype = sz
+    lib.kf_attn_paged.argtypes = [p, i64s] + [p] * 8 + [i] * 9 + [p, sz, p]
+    lib.kf_attn_paged.restype = i
+    lib.kf_kv_weigh.argtypes = [p, i64s] + [p] * 6 + [i] * 9 + [p]
+    lib.kf_kv_weigh.restype = i
+    lib.kf_kv_evict_workspace_bytes.argtypes = [i] * 5
+    lib.kf_kv_evict_workspace_bytes.restype = sz
+    lib.kf_kv_evict.argtypes = [p] * 7 + [i] * 7 + [p, sz, p]
+    lib.kf_kv_evict.restype = i
     lib.kf_launch_flash_attn.argtypes = [p, p, p, p] + [i] * 5 + [p]
     lib.kf_launch_flash_attn.restype = i
     lib.kf_status_string.argtypes = [i]
@@ -470,5 +486,6 @@ def attn_decode_paged(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, re
     return (out, Mi, Li) if return_stats else out
 
 
-from .serve import (KF_BF16, KF_ROPE_INTERLEAVED, attn_decode_kv4, attn_packed,  # noqa: E402
-                    kv4_append, kv4_page_bytes, kv4_read, kv4_workspace_bytes, qk_norm_rope, rope_freqs)
+from .serve import (KF_BF16, KF_ROPE_INTERLEAVED, attn_decode_kv4, attn_packed, attn_paged,  # noqa: E402
+                    evict_workspace_bytes, kv4_append, kv4_page_bytes, kv4_read, kv4_workspace_bytes, kv_append,
+                    kv_evict, kv_weigh, paged_attn_workspace_bytes, qk_norm_rope, rope_freqs)

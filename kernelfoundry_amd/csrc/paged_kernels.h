@@ -1,0 +1,542 @@
+// paged_kernels.h -- attention of packed new tokens over a paged 16-bit K/V cache,
+// and the attention weight that each of its keys gathers.
+//
+// Pools are [num_pages][H_kv][page_size][D] (attn_decode_paged's); sequence b's new
+// tokens are the packed ones q_starts[b] .. q_starts[b + 1] - 1 and the last of its
+// kv_lens[b] keys.  The query rows that read a KV head are (token, head of its group),
+// token major: row r of a sequence is query r / ratio of group head r % ratio.
+#pragma once
+
+#include "elem.h"
+#include "packed_kernels.h"
+
+namespace kf {
+
+struct PagedParams : AttnParams {  // Q, K, V, O, Mi (LSE), scales, causal, heads_kv, out_dtype, pages, kv_lens
+    long long q_token, q_head;     // strides in elements
+    const int* q_starts;           // [n_seqs + 1]
+    int n_seqs, tokens_q, ratio;
+    // Row tiles are cut into parts along the keys where there are too few of them for
+    // the device: `target` parts of a KV head are aimed at (0: no cuts), none smaller
+    // than min_share units of 32 << unit_shift keys.
+    int target, min_share, unit_shift;
+    const float* row_lse;          // kf_kv_weigh: [tokens_q][H_q]
+    float* weights;                // kf_kv_weigh: [num_pages][H_kv][page_size]
+};
+
+// One sequence's new tokens and keys.
+struct PagedSeq {
+    int q0, qn, kn;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int i) {
+    PagedSeq s;
+    s.q0 = min(max(p.q_starts[i], 0), p.tokens_q);
+    s.qn = min(max(p.q_starts[i + 1], s.q0), p.tokens_q) - s.q0;
+    s.kn = min(max(p.kv_lens[i], 0), p.kv_len);
+    return s;
+}
+
+// A part of a row tile: its sequence, tile and part in it, of how many, and, where there
+// are several, the partial that it writes.
+struct PagedItem {
+    int seq, tile, part, parts, slot;
+};
+
+// Item j of a KV head, by the lanes of a wave; false past the last.  Every tile of a
+// sequence has the same number of parts, so many that one has at most `share` units of
+// keys; `share` is the work of all tiles over p.target.  So no more than target + tiles
+// parts come out, and 2 target of tiles that are cut: more than one part means more
+// than `share` units, and fewer than twice as many parts as shares.  Up to 64 sequences have a
+// lane each, of more a lane has a run of consecutive ones.  kCut: j counts the tiles
+// that are cut, not the parts.
+template <int kRows, bool kCut>
+__device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j, PagedItem& it) {
+    struct Count {
+        int tiles, units;
+    };
+    const auto count = [&](int i) {
+        const PagedSeq s = paged_seq(p, i);
+        return Count{(int)(((long long)s.qn * p.ratio + kRows - 1) / kRows),
+                     (key_stages(s.kn) + (1 << p.unit_shift) - 1) >> p.unit_shift};
+    };
+    const int per = (p.n_seqs + 63) / 64, first = min(lane * per, p.n_seqs), last = min(first + per, p.n_seqs);
+    Count mine{0, 0};
+    if (per == 1 && first < last) mine = count(first);
+    int share = 0;
+    if (p.target > 0) {
+        int sum = mine.tiles * mine.units;
+        if (per > 1)
+            for (int i = first; i < last; ++i) {
+                const Count c = count(i);
+                sum += c.tiles * c.units;
+            }
+        const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+        share = max((int)((unsigned)total + (unsigned)p.target - 1u) / p.target, p.min_share);
+    }
+    const auto parts_of = [&](const Count& c) { return share > 0 ? max((c.units + share - 1) / share, 1) : 1; };
+    const auto items_of = [&](const Count& c, int parts) { return kCut ? (parts > 1 ? c.tiles : 0) : c.tiles * parts; };
+    const auto slots_of = [&](const Count& c, int parts) { return parts > 1 ? c.tiles * parts : 0; };
+    int parts = parts_of(mine), items = items_of(mine, parts), slots = slots_of(mine, parts);
+    if (per > 1) {
+        items = slots = 0;
+        for (int i = first; i < last; ++i) {
+            const Count c = count(i);
+            parts = parts_of(c);
+            items += items_of(c, parts);
+            slots += slots_of(c, parts);
+        }
+    }
+    const int inc = wave_scan(items), slot_inc = wave_scan(slots);
+    const uint64_t past = __ballot(inc > j);
+    if (past == 0) return false;
+    const int run = __builtin_ctzll(past);
+    int left = j - (__builtin_amdgcn_readlane(inc, run) - __builtin_amdgcn_readlane(items, run));
+    int slot = __builtin_amdgcn_readlane(slot_inc, run) - __builtin_amdgcn_readlane(slots, run);
+    int tiles;
+    if (per == 1) {
+        it.seq = run;
+        it.parts = __builtin_amdgcn_readlane(parts, run);
+        tiles = __builtin_amdgcn_readlane(mine.tiles, run);
+    } else {
+        const int end = min((run + 1) * per, p.n_seqs);
+        for (int i0 = run * per;; i0 += 64) {
+            if (i0 >= end) return false;  // not reached
+            mine = i0 + lane < end ? count(i0 + lane) : Count{0, 0};
+            parts = parts_of(mine);
+            items = items_of(mine, parts);
+            slots = slots_of(mine, parts);
+            const int in = wave_scan(items), sl = wave_scan(slots);
+            const uint64_t over = __ballot(in > left);
+            if (over != 0) {
+                const int at = __builtin_ctzll(over);
+                it.seq = i0 + at;
+                it.parts = __builtin_amdgcn_readlane(parts, at);
+                tiles = __builtin_amdgcn_readlane(mine.tiles, at);
+                left -= __builtin_amdgcn_readlane(in, at) - __builtin_amdgcn_readlane(items, at);
+                slot += __builtin_amdgcn_readlane(sl, at) - __builtin_amdgcn_readlane(slots, at);
+                break;
+            }
+            left -= __builtin_amdgcn_readlane(in, 63);
+            slot += __builtin_amdgcn_readlane(sl, 63);
+        }
+    }
+    if (kCut) {
+        it.part = 0;
+        it.tile = left;
+    } else {
+        it.part = left % it.parts;
+        // Causal tiles see the more keys the later they are: the last ones first.
+        it.tile = tiles - 1 - left / it.parts;
+    }
+    it.slot = slot + it.tile * it.parts + it.part;
+    // (Of starts in no order the sums may wrap: no partial outside the workspace.)
+    return it.parts == 1 || (unsigned)it.slot + (kCut ? it.parts : 1u) <= 2u * (unsigned)p.target;
+}
+
+// A workgroup is NW waves of 32 query rows each; with KS > 1 they form KS groups that
+// take the same rows and a share of the keys each, merged through LDS at the end.
+template <int D, int NW, int KS> struct PagedCfg {
+    static constexpr int kThreads = 64 * NW;
+    static constexpr int kRowWaves = NW / KS;             // waves per KV group
+    static constexpr int kRows = 32 * kRowWaves;          // query rows per workgroup
+    static constexpr int BC = 32;                         // keys per MFMA tile and LDS stage
+    // Waves per SIMD that the registers have to allow.
+    static constexpr int kWavesPerSimd =
+        D == 64 ? (KS == 4 ? 2 : 4) : D == 128 ? (KS == 1 ? 3 : KS == 2 ? 2 : 1) : KS == 1 ? 2 : 1;
+};
+
+// What a masked key's V row is read from, so that its weight 0 meets finite values: 16
+// rows of zeros.
+static __device__ const u32x4 paged_zeros[16 * 256 * 2 / 16] = {};
+
+template <bool kBF, int D, int NW, int KS>
+__global__ __launch_bounds__((PagedCfg<D, NW, KS>::kThreads), (PagedCfg<D, NW, KS>::kWavesPerSimd))
+void kf_attn_paged_kernel(PagedParams p) {
+    using Cfg = PagedCfg<D, NW, KS>;
+    using E = Elem<kBF>;
+    using X8 = typename E::x8;
+    using SW = SwizzleRow<D>;
+    constexpr int BC = Cfg::BC, kRows = Cfg::kRows, kRowWaves = Cfg::kRowWaves;
+    constexpr int kRowBytes = D * 2, kChunks = D / 8, kRowsPerInstr = 1024 / kRowBytes;
+    constexpr int kTensorBytes = BC * kRowBytes;
+    // A unit of copying: 16 rows of K or V, which lie in one page.
+    constexpr int kUnitInstr = 16 / kRowsPerInstr, kUnitsPerWave = 4 / kRowWaves;
+    static_assert(kRowWaves == 1 || kRowWaves == 2 || kRowWaves == 4, "whole units");
+    constexpr int kNKK = D / 16, kNTD = D / 32;
+    constexpr int kBuf = KS * 2 * kTensorBytes;           // a stage of every group
+    __shared__ __attribute__((aligned(1024))) char buf0[kBuf];
+    __shared__ __attribute__((aligned(1024))) char buf1[kBuf];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave_id = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 5;
+    // KV heads next to each other: with ids dealt round-robin over the XCDs, 8
+    // heads have an XCD, and its L2, each.
+    const int hk = blockIdx.x % p.heads_kv;
+    PagedItem it;
+    if (!paged_find<kRows, false>(p, lane, blockIdx.x / p.heads_kv, it)) return;
+    PagedSeq sq = paged_seq(p, it.seq);
+    sq.q0 = __builtin_amdgcn_readfirstlane(sq.q0);
+    sq.qn = __builtin_amdgcn_readfirstlane(sq.qn);
+    sq.kn = __builtin_amdgcn_readfirstlane(sq.kn);
+    const int ratio = p.ratio, R = sq.qn * ratio, klen = sq.kn, sh = p.page_shift;
+    const float c = p.scale_log2;
+    const int wave = KS > 1 ? wave_id % kRowWaves : wave_id;
+    const int kgrp = KS > 1 ? wave_id / kRowWaves : 0;
+    // (Of starts in no order the sums by which the item was found may wrap.)
+    if ((unsigned)it.tile * (unsigned)kRows >= (unsigned)R) return;
+    const auto limit = [&](int row) {  // keys that the row sees
+        return p.causal ? min(max(klen - sq.qn + row / ratio + 1, 0), klen) : klen;
+    };
+    const int r0 = it.tile * kRows, w0 = r0 + wave * 32;
+    const int blk_lim = limit(min(R, r0 + kRows) - 1);
+    // This part's stages of those that the tile sees, and the groups' of these, as many
+    // as any other's; row limits count from kv_base.
+    const int seen = key_stages(blk_lim), per_part = (seen + it.parts - 1) / it.parts;
+    const int s0 = min(it.part * per_part, seen), s1 = min(s0 + per_part, seen);
+    const int ntiles = (s1 - s0 + KS - 1) / KS;
+    const int kv_base = (s0 + kgrp * ntiles) * BC, kv_end = min(min(kv_base + ntiles * BC, s1 * BC), blk_lim);
+    const auto own = [&](int lim) { return min(lim, kv_end) - kv_base; };
+    const int wave_min = own(w0 < R ? limit(w0) : blk_lim);
+    const int wave_max = own(w0 < R ? limit(min(R, w0 + 32) - 1) : 0);
+    const int nt_w = (wave_max + BC - 1) / BC;            // the wave's tiles (none if not positive); it skips the others
+
+    const int lim = own(limit(min(w0 + (lane & 31), R - 1)));
+    const int nrows = R - w0;                             // rows of the wave, if any
+    // The row of O (below tokens_q H_q, an int) of this lane; rows past R
+    // compute on the last one and are not stored.  From an opaque lane, so that
+    // none of it lives across the tiles.
+    auto out_row = [&]() {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const int r = min(w0 + (l & 31), R - 1);
+        return ((sq.q0 + r / ratio) * p.heads_kv + hk) * ratio + r % ratio;
+    };
+    // The partial of this lane's row.
+    const auto part_row = [&]() {
+        return ((size_t)it.slot * p.heads_kv + hk) * kRows + wave * 32 + (lane & 31);
+    };
+    if (ntiles == 0) {                                    // no key for any row
+        if ((lane & 31) < nrows && kgrp == 0) {
+            if (it.parts > 1) {
+                if (g == 0) {
+                    p.Mpart[part_row()] = -INFINITY;
+                    p.Lpart[part_row()] = 0.f;
+                }
+            } else {
+                const int at = out_row();
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) store_out4(p, (size_t)at * D + 8 * i + 4 * g, f32x4{0.f, 0.f, 0.f, 0.f});
+                if (g == 0) store_stats(p, at, -INFINITY, 0.f);
+            }
+        }
+        return;
+    }
+
+    // The ids of 64 pages from page0 on, one to a lane; stages come in order.
+    const int* const table = p.block_table + (size_t)it.seq * p.max_pages;
+    int page0 = kv_base >> sh;
+    int ids = table[min(page0 + lane, p.max_pages - 1)];
+    auto page_of = [&](int key) {                         // of a key below klen
+        if ((key >> sh) - page0 >= 64) {
+            page0 = key >> sh;
+            ids = table[min(page0 + lane, p.max_pages - 1)];
+        }
+        return __builtin_amdgcn_readlane(ids, (key >> sh) - page0);
+    };
+    const char* const Kp = reinterpret_cast<const char*>(p.K);
+    const char* const Vp = reinterpret_cast<const char*>(p.V);
+    // LDS-DMA: lane l of an instruction fills row l / kChunks of its rows, physical chunk
+    // l % kChunks.  The swizzle depends on row & 15: the units' lane offsets are alike.
+    const int copier = wave_id % kRowWaves;
+    const int lr = lane / kChunks;
+    uint32_t chunk_off[kUnitInstr];
+#pragma unroll
+    for (int i = 0; i < kUnitInstr; ++i)
+        chunk_off[i] = (((lane % kChunks) ^ SW::h(i * kRowsPerInstr + lr)) % kChunks) * 16;
+    // Requests the stage that begins at key kv_base + kv0; returns which of its halves lie on
+    // no valid page, bit 0 keys 0 .. 15, bit 1 the others.
+    auto issue_stage = [&](char* dst, int kv0) {
+        const int kv = kv_base + kv0;
+        int id[2], bad = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            id[h] = kv + 16 * h < klen ? page_of(kv + 16 * h) : -1;
+            bad |= (unsigned)id[h] < (unsigned)p.num_pages ? 0 : 1 << h;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnitsPerWave; ++u) {
+            const int unit = copier * kUnitsPerWave + u, h = unit & 1;
+            const bool is_v = unit >= 2;
+            const uint32_t d_lds = (uint32_t)(uintptr_t)(lds_void*)(dst + unit * (kTensorBytes / 2));
+            const int key = kv + 16 * h;
+            const int page = h ? id[1] : id[0];
+            const bool ok = (bad >> h & 1) == 0;
+            const size_t row = (((size_t)(ok ? page : 0) * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1));
+            const char* src = (is_v ? Vp : Kp) + row * kRowBytes;
+            if (!ok) src = reinterpret_cast<const char*>(paged_zeros);
+            if (!ok || key + 16 <= klen) {
+#pragma unroll
+                for (int i = 0; i < kUnitInstr; ++i)
+                    lds_copy16(d_lds + i * 1024, src + i * 1024, lr * kRowBytes + chunk_off[i]);
+            } else {
+                // Rows past the keys re-read the last one (finite data whose scores are masked).
+#pragma unroll
+                for (int i = 0; i < kUnitInstr; ++i)
+                    lds_copy16(d_lds + i * 1024, src, min(i * kRowsPerInstr + lr, klen - 1 - key) * kRowBytes + chunk_off[i]);
+            }
+        }
+        return bad;
+    };
+
+    // LDS reads, as in the packed kernel.
+    constexpr bool kXorOff = D >= 128;
+    int koff[kNKK];
+#pragma unroll
+    for (int kk = 0; kk < kNKK; ++kk) {
+        const int r = lane & 31;
+        koff[kk] = r * kRowBytes + (((2 * kk + g) ^ SW::h(r)) % kChunks) * 16;
+    }
+    int voff[kNTD][2];
+    {
+        const int G = lane >> 4, w = lane & 15;
+#pragma unroll
+        for (int td = 0; td < kNTD; ++td)
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+                const int r = 4 * (G >> 1) + (w >> 2) + 8 * h2;
+                const int d = 32 * td + 16 * (G & 1) + 4 * (w & 3);
+                voff[td][h2] = kTensorBytes + r * kRowBytes + (((d >> 3) ^ SW::h(r)) % kChunks) * 16 + ((d >> 2) & 1) * 8;
+            }
+    }
+
+    char* const b0 = buf0 + kgrp * 2 * kTensorBytes;      // this group's stages
+    char* const b1 = buf1 + kgrp * 2 * kTensorBytes;
+    int bad_next = issue_stage(b0, 0);
+    X8 q[kNKK];
+    {
+        const int rc = min(w0 + (lane & 31), R - 1);
+        const uint16_t* Qr = p.Q + (size_t)(sq.q0 + rc / ratio) * p.q_token + (size_t)(hk * ratio + rc % ratio) * p.q_head;
+#pragma unroll
+        for (int kk = 0; kk < kNKK; ++kk) q[kk] = *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8);
+    }
+
+    RowState st{-INFINITY, -INFINITY, 0.f, -INFINITY};
+    f32x16 o[kNTD];
+    const float inv_c = 1.0f / c;
+#pragma unroll
+    for (int td = 0; td < kNTD; ++td) o[td] = f32x16{};
+    // V^T of 32 channels and 16 keys, V rows at stage + kTensorBytes.
+    auto v_frag = [&](const char* stage, int vb, int td, int jj) {
+        const int vo0 = kXorOff ? vb ^ (64 * td) : voff[td][0];
+        const int vo1 = kXorOff ? (vb ^ (64 * td) ^ 128) + 8 * kRowBytes : voff[td][1];
+        const f16x4 lo = lds_read_tr16(stage + vo0 + jj * 16 * kRowBytes);
+        const f16x4 hi = lds_read_tr16(stage + vo1 + jj * 16 * kRowBytes);
+        return __builtin_bit_cast(X8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto tile = [&](const char* stage, int t, int bad) {
+        if (t >= nt_w) return;
+        int kb = koff[0], vb = voff[0][0];
+        if constexpr (kXorOff) asm volatile("" : "+v"(kb), "+v"(vb));  // derived per tile
+        f32x16 s[1] = {f32x16{}};
+#pragma unroll
+        for (int kk = 0; kk < kNKK; ++kk) {
+            const X8 kf = *reinterpret_cast<const X8*>(stage + (kXorOff ? kb ^ (32 * kk) : koff[kk]));
+            s[0] = E::mfma32(kf, q[kk], s[0]);
+        }
+        if ((t + 1) * BC > wave_min || bad != 0) {      // keys that a row does not see -> -inf
+            asm volatile("" ::: "memory");              // a branch, not selects in every tile
+            const int lg = lim - t * BC - 4 * g;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (8 * (r >> 2) + (r & 3) >= lg || (bad >> (r >> 3) & 1)) s[0][r] = -INFINITY;
+        }
+        X8 pp[2];
+        block_update_max<kNTD>(st, block_rowmax<1>(s), c, inv_c, o);
+        // A row that has seen no key yet keeps m = -inf and must get P = 0, not NaN.
+        packed_exp<kBF>(s[0], c, st.m == -INFINITY ? 0.f : -st.m, pp, st.l);
+#pragma unroll
+        for (int td = 0; td < kNTD; ++td)
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) o[td] = E::mfma32(v_frag(stage, vb, td, jj), pp[jj], o[td]);
+    };
+    for (int t0 = 0; t0 < ntiles; t0 += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int t = t0 + u;
+            if (t >= ntiles) break;
+            char* cur = u == 0 ? b0 : b1;
+            char* nxt = u == 0 ? b1 : b0;
+            // Stage t has landed for every wave; every wave is done with stage t - 1 (in
+            // nxt).  A wave that copies its stages itself waits for itself alone.
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+            if constexpr (kRowWaves > 1) __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const int bad = bad_next;
+            if (t + 1 < ntiles) bad_next = issue_stage(nxt, (t + 1) * BC);
+            tile(cur, t, bad);
+        }
+    }
+    if constexpr (KS > 1) {
+        // Merge slot k: 1 KiB of the then free stage buffers.
+        static_assert(kRowWaves * kNTD * 4 * (KS - 1) * 1024 <= 2 * kBuf, "merge slots");
+        __shared__ float merge_ml[2 * NW * 64];
+        const auto slot_base = [&](int k) { return k < kBuf / 1024 ? buf0 + k * 1024 : buf1 + (k * 1024 - kBuf); };
+        p.n_splits = it.parts;
+        merge_kv_groups<D, KS, kRowWaves>(p, st, o, slot_base, merge_ml, wave, kgrp, lane, g, out_row(), part_row(),
+                                          (lane & 31) < nrows);
+        return;
+    }
+    __syncthreads();  // every wave is done with the stages
+    char* const mine = (wave_id < NW / 2 ? buf0 : buf1) + wave_id % (NW / 2) * (2 * kBuf / NW);
+    const float l = sum_xor32(st.l);
+    if (it.parts > 1) {
+        // Rebased to the rows' true maxima, for the merge.
+        const bool none = st.rmax == -INFINITY;
+        const float beta = none ? 0.f : rebase_factor(st.m, st.rmax, c);
+        const size_t at = part_row();
+        p.O = p.Opart + (at - (lane & 31)) * D;
+        packed_store<kOutF32, D, 2 * kBuf / NW>(p, o, beta, mine, lane & 31, nrows, lane);
+        if (g == 0 && (lane & 31) < nrows) {
+            p.Mpart[at] = none ? -INFINITY : st.rmax * p.scale;
+            p.Lpart[at] = l * beta;
+        }
+        return;
+    }
+    const bool empty = !(l > 0.f);                        // no visible key
+    const float inv = empty ? 0.f : 1.0f / l;
+    const int at = out_row();
+    if (p.out_dtype == kOutF16)
+        packed_store<kOutF16, D, 2 * kBuf / NW>(p, o, inv, mine, at, nrows, lane);
+    else if (p.out_dtype == kOutBF16)
+        packed_store<kOutBF16, D, 2 * kBuf / NW>(p, o, inv, mine, at, nrows, lane);
+    else
+        packed_store<kOutF32, D, 2 * kBuf / NW>(p, o, inv, mine, at, nrows, lane);
+    if (g == 0 && (lane & 31) < nrows)
+        store_stats(p, at, st.rmax * p.scale, empty ? 0.f : l * rebase_factor(st.m, st.rmax, c));
+}
+
+// The parts of the tiles that were cut, joined: a workgroup per tile and KV head, a
+// lane per 4 channels of a row.  O = sum_i w_i O_i / L, L = sum_i w_i l_i, w_i = exp(m_i - max m), in
+// the order of the keys; a part in which a row saw no key (m_i = -inf) wrote no O.
+constexpr int kPagedMergeThreads = 256;
+template <int D, int kRows>
+__global__ __launch_bounds__(kPagedMergeThreads)
+void kf_attn_paged_merge_kernel(PagedParams p) {
+    const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv;
+    PagedItem it;
+    if (!paged_find<kRows, true>(p, lane, blockIdx.x / p.heads_kv, it)) return;
+    const PagedSeq sq = paged_seq(p, it.seq);
+    const int R = sq.qn * p.ratio, r0 = it.tile * kRows;
+    if ((unsigned)it.tile * (unsigned)kRows >= (unsigned)R) return;
+    const int n = min(kRows, R - r0) * (D / 4);
+    constexpr int kUnroll = 4;
+    for (int i = threadIdx.x; i < n; i += kPagedMergeThreads) {
+        const int r = i / (D / 4), c4 = i % (D / 4) * 4;
+        const auto at = [&](int k) { return ((size_t)(it.slot + k) * p.heads_kv + hk) * kRows + r; };
+        float m = -INFINITY, l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < it.parts; k0 += kUnroll) {
+            float mv[kUnroll], lv[kUnroll];
+            f32x4 ov[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const size_t pi = at(min(k0 + u, it.parts - 1));
+                mv[u] = p.Mpart[pi];
+                lv[u] = p.Lpart[pi];
+                ov[u] = *reinterpret_cast<const f32x4*>(p.Opart + pi * D + c4);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (k0 + u >= it.parts || mv[u] == -INFINITY) continue;
+                const float top = fmaxf(m, mv[u]);
+                const float keep = m == -INFINITY ? 0.f : exp2_hw((m - top) * kLog2e);
+                const float w = exp2_hw((mv[u] - top) * kLog2e);
+                l = l * keep + w * lv[u];
+                acc = acc * keep + ov[u] * w;
+                m = top;
+            }
+        }
+        const int row = r0 + r, to = ((sq.q0 + row / p.ratio) * p.heads_kv + hk) * p.ratio + row % p.ratio;
+        store_out4(p, (size_t)to * D + c4, acc * (l > 0.f ? 1.0f / l : 0.f));
+        if (c4 == 0) store_stats(p, to, m, l);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The attention weight that keys gather: weights[j] += sum over the query rows of
+// exp(s_rj - lse_r), r over the new tokens that see key j and the heads of its group.
+//
+// S^T = K Q^T by the 32x32x16 MFMA: a wave holds 32 keys as the A operand and goes
+// through the query rows, 32 at a time, as the B operand; lane l has row l % 32 of 16
+// keys, and adds their weights up in registers.  At the end the lanes' sums of a key are
+// added, and the one wave that has the key adds them to its weight: no atomics,
+// always the same order.
+// ---------------------------------------------------------------------------
+constexpr int kWeighThreads = 256;
+constexpr int kWeighKeys = 32 * kWeighThreads / 64;   // keys of a workgroup
+
+template <bool kBF, int D>
+__global__ __launch_bounds__(kWeighThreads)
+void kf_kv_weigh_kernel(PagedParams p) {
+    using E = Elem<kBF>;
+    using X8 = typename E::x8;
+    constexpr int kNKK = D / 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const int hk = blockIdx.x % p.heads_kv, sh = p.page_shift;
+    const int blocks = (p.kv_len + kWeighKeys - 1) / kWeighKeys;
+    const int seq = blockIdx.x / p.heads_kv / blocks, block = blockIdx.x / p.heads_kv % blocks;
+    const PagedSeq sq = paged_seq(p, seq);
+    const int R = sq.qn * p.ratio, k0 = block * kWeighKeys + wave * 32;
+    if (k0 >= sq.kn || R == 0) return;
+    const int* const table = p.block_table + (size_t)seq * p.max_pages;
+    // This lane's key of the A operand.  Past the keys, or on no valid page, any row will do:
+    // it reaches no other key's sum, and its own is dropped.
+    const auto page_of = [&](int key) { return key < sq.kn ? table[key >> sh] : -1; };
+    const auto valid = [&](int id) { return (unsigned)id < (unsigned)p.num_pages; };
+    const int key = k0 + (lane & 31), id = page_of(key);
+    const uint16_t* Kr = p.K + ((((size_t)(valid(id) ? id : 0) * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))) * D;
+    X8 kf[kNKK];
+#pragma unroll
+    for (int kk = 0; kk < kNKK; ++kk) kf[kk] = *reinterpret_cast<const X8*>(Kr + (2 * kk + g) * 8);
+    f32x16 sum = {};
+    // Causal: query i sees keys j <= i + before; the first that sees any of these.
+    const int before = sq.kn - sq.qn;
+    const int first = p.causal ? max(k0 - before, 0) : 0;
+    for (int r0 = first * p.ratio / 32 * 32; r0 < R; r0 += 32) {
+        const int row = min(r0 + (lane & 31), R - 1), q = row / p.ratio;
+        const uint16_t* Qr = p.Q + (size_t)(sq.q0 + q) * p.q_token + (size_t)(hk * p.ratio + row % p.ratio) * p.q_head;
+        const float e = p.row_lse[((size_t)(sq.q0 + q) * p.heads_kv + hk) * p.ratio + row % p.ratio];
+        f32x16 s = {};
+#pragma unroll
+        for (int kk = 0; kk < kNKK; ++kk) s = E::mfma32(kf[kk], *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8), s);
+        // Rows past the last, and those without a key, add nothing.
+        const float off = r0 + (lane & 31) < R && e > -INFINITY ? -e * kLog2e : -INFINITY;
+        const int lim = (p.causal ? q + before + 1 : sq.kn) - k0 - 4 * g;   // keys of this lane that the row sees
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float w = exp2_hw(fmaf(s[r], p.scale_log2, off));
+            sum[r] += 8 * (r >> 2) + (r & 3) < lim ? w : 0.f;
+        }
+    }
+    // Over the 32 rows: with every exchange a lane keeps half of its keys, in the end
+    // lane l (and l ^ 16) the one of register l % 16.
+#pragma unroll
+    for (int b = 3; b >= 0; --b)
+#pragma unroll
+        for (int r = 0; r < 1 << b; ++r) {
+            const bool up = (lane >> b & 1) != 0;
+            const float give = up ? sum[r] : sum[r + (1 << b)];
+            sum[r] = (up ? sum[r + (1 << b)] : sum[r]) + __shfl_xor(give, 1 << b);
+        }
+    const float total = sum[0] + __shfl_xor(sum[0], 16);
+    const int to = k0 + acc_row(lane & 15, lane), to_id = page_of(to);
+    if ((lane & 16) == 0 && valid(to_id)) {
+        float* const w = p.weights + (((size_t)to_id * p.heads_kv + hk) << sh) + (to & ((1 << sh) - 1));
+        *w += total;
+    }
+}
+
+}  // namespace kf

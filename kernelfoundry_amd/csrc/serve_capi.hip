@@ -1,6 +1,7 @@
 // serve_capi.hip -- C ABI of what stands beside the attention forward in a
 // server: packed prompts, head norms with rotary positions, the 4-bit cache
-// and decode over it.  Entry points are declared in include/kf/attn.h; as in
+// and decode over it, the 16-bit cache with attention of new tokens over it, the
+// weights that its keys gather and eviction by them.  Entry points are declared in include/kf/attn.h; as in
 // attn_capi.hip, every argument check runs before the first HIP call.
 #include <hip/hip_runtime.h>
 
@@ -9,9 +10,11 @@
 #include <cmath>
 #include <cstdint>
 
+#include "cache_kernels.h"
 #include "capi_internal.h"
 #include "kv4_kernels.h"
 #include "packed_kernels.h"
+#include "paged_kernels.h"
 #include "rope_kernels.h"
 
 namespace {
@@ -238,14 +241,18 @@ int check_kv4(int tokens, int n_seqs, int H_kv, int D, int page_size, int max_pa
     return KF_OK;
 }
 
-template <bool kBF, int D>
-int launch_cache(bool append, kf::Kv4Params& prm, hipStream_t stream) {
-    // Tokens of a workgroup: enough to give its threads an item each, and up to four
-    // while that leaves two workgroups a CU (16 x 1000 tokens, 8 heads, D = 128, 19.3 us
-    // written; eight items and four workgroups 21.6).
+// Tokens of a workgroup: enough to give its threads an item each, and up to four
+// while that leaves two workgroups a CU (16 x 1000 tokens, 8 heads, D = 128, 19.3 us
+// written in 4 bits; eight items and four workgroups 21.6).
+int cache_tile(const kf::Kv4Params& prm, int D) {
     const int per_token = prm.heads * (D / 8), fill = (kf::kKv4Threads + per_token - 1) / per_token;
     const long long share = prm.tokens / (2LL * current_device_shape().cus);
-    prm.tile = (int)std::min<long long>(std::max<long long>(fill, std::min<long long>(share, 4LL * fill)), kf::kKv4MaxTile);
+    return (int)std::min<long long>(std::max<long long>(fill, std::min<long long>(share, 4LL * fill)), kf::kKv4MaxTile);
+}
+
+template <bool kBF, int D>
+int launch_cache(bool append, kf::Kv4Params& prm, hipStream_t stream) {
+    prm.tile = cache_tile(prm, D);
     const dim3 grid((prm.tokens + prm.tile - 1) / prm.tile), block(kf::kKv4Threads);
     if (!fits_grid(grid.x, kf::kKv4Threads)) return KF_ERR_SIZE;
     (void)hipGetLastError();
@@ -292,6 +299,155 @@ int launch_rope_dim(const kf::RopeParams& prm, int D, hipStream_t stream) {
         case 128: return launch_rope<kBF, 128>(prm, stream);
         default: return launch_rope<kBF, 256>(prm, stream);
     }
+}
+
+// ---- Attention over the paged 16-bit cache. ----
+
+// Rows of a tile and KV groups of the layouts of the paged kernel (PagedCfg).
+struct PagedPlan {
+    int rows, slots;
+    long long items, cut_tiles;           // at most, of a KV head
+    size_t o_bytes, s_bytes, ws_bytes;
+    kf::PagedParams prm;
+};
+
+int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, int max_pages, int num_pages,
+               PagedPlan* pl) {
+    if (D != 64 && D != 128 && D != 256) return KF_ERR_HEAD_DIM;
+    if (const int st = check_heads(H_q, H_kv); st != KF_OK) return st;
+    if (n_seqs <= 0) return KF_ERR_SIZE;
+    if (const int st = check_packed(tokens, H_q, D); st != KF_OK) return st;
+    kf::PagedParams& prm = pl->prm;
+    if (const int st = paged_geometry(page_size, max_pages, num_pages, &prm.page_shift, &prm.kv_len); st != KF_OK)
+        return st;
+    if (prm.kv_len > kMaxIndex) return KF_ERR_SIZE;
+    const long long rows = (long long)tokens * (H_q / H_kv);
+    const double avg = (double)rows / n_seqs;
+    pl->rows = D == 256 ? (avg > 32 ? 128 : 32) : avg > 64 ? 128 : avg > 32 ? 64 : 32;
+    const long long least = (rows + pl->rows - 1) / pl->rows;
+    const long long tiles = rows / pl->rows + std::min<long long>(n_seqs, tokens);
+    const long long stages = ((long long)prm.kv_len + 31) / 32;
+    const int wanted = std::max(1, 2 * current_device_shape().cus / H_kv);
+    prm.target = least >= 2 * wanted || stages <= 8 ? 0 : wanted;
+    prm.unit_shift = 0;
+    while (tiles * ((stages >> prm.unit_shift) + 1) > INT_MAX) ++prm.unit_shift;
+    prm.min_share = std::max(1, 8 >> prm.unit_shift);
+    pl->items = tiles + prm.target;
+    pl->cut_tiles = std::min<long long>(tiles, prm.target);
+    pl->slots = 2 * prm.target;
+    const size_t parts = (size_t)pl->slots * H_kv * pl->rows;
+    pl->o_bytes = align_up(parts * D * sizeof(float), kWsAlign);
+    pl->s_bytes = align_up(parts * sizeof(float), kWsAlign);
+    pl->ws_bytes = pl->o_bytes + 2 * pl->s_bytes;
+    if (!fits_grid(pl->items * H_kv, 256)) return KF_ERR_SIZE;
+    return KF_OK;
+}
+
+template <bool kBF, int D, int NW, int KS>
+int launch_paged(const PagedPlan& pl, hipStream_t stream) {
+    using Cfg = kf::PagedCfg<D, NW, KS>;
+    const kf::PagedParams& prm = pl.prm;
+    (void)hipGetLastError();
+    kf::kf_attn_paged_kernel<kBF, D, NW, KS>
+        <<<dim3((unsigned)(pl.items * prm.heads_kv)), dim3(Cfg::kThreads), 0, stream>>>(prm);
+    if (const int st = launched(); st != KF_OK || prm.target == 0) return st;
+    kf::kf_attn_paged_merge_kernel<D, Cfg::kRows>
+        <<<dim3((unsigned)(pl.cut_tiles * prm.heads_kv)), dim3(kf::kPagedMergeThreads), 0, stream>>>(prm);
+    return launched();
+}
+
+template <bool kBF>
+int launch_paged_dim(const PagedPlan& pl, int D, hipStream_t stream) {
+    switch (D) {
+        case 64:
+            return pl.rows == 128  ? launch_paged<kBF, 64, 4, 1>(pl, stream)
+                   : pl.rows == 64 ? launch_paged<kBF, 64, 4, 2>(pl, stream)
+                                   : launch_paged<kBF, 64, 4, 4>(pl, stream);
+        case 128:
+            return pl.rows == 128  ? launch_paged<kBF, 128, 4, 1>(pl, stream)
+                   : pl.rows == 64 ? launch_paged<kBF, 128, 4, 2>(pl, stream)
+                                   : launch_paged<kBF, 128, 4, 4>(pl, stream);
+        default: return pl.rows == 128 ? launch_paged<kBF, 256, 4, 1>(pl, stream) : launch_paged<kBF, 256, 2, 2>(pl, stream);
+    }
+}
+
+// What the paged attention and the gathered weights have in common, the sizes apart.
+void set_paged(kf::PagedParams& prm, const void* Q, const int64_t* strides, const void* K_pages, const int* block_table,
+               const int* seq_starts, const int* kv_lens, int n_seqs, int tokens, int H_q, int H_kv, int D,
+               int max_pages, int num_pages, int flags) {
+    prm.Q = static_cast<const uint16_t*>(Q);
+    prm.K = static_cast<const uint16_t*>(K_pages);
+    prm.q_token = strides ? strides[0] : (int64_t)H_q * D;
+    prm.q_head = strides ? strides[1] : D;
+    prm.q_starts = seq_starts;
+    prm.kv_lens = kv_lens;
+    prm.block_table = block_table;
+    prm.max_pages = max_pages;
+    prm.num_pages = num_pages;
+    prm.n_seqs = n_seqs;
+    prm.tokens_q = tokens;
+    prm.heads_kv = H_kv;
+    prm.ratio = H_q / H_kv;
+    prm.causal = (flags & KF_ATTN_CAUSAL) ? 1 : 0;
+    prm.n_splits = 1;
+    set_scales(prm, D);
+}
+
+template <bool kBF>
+int launch_weigh(const kf::PagedParams& prm, int D, hipStream_t stream) {
+    const long long blocks = ((long long)prm.kv_len + kf::kWeighKeys - 1) / kf::kWeighKeys;
+    if (!fits_grid(blocks * prm.n_seqs, kf::kWeighThreads) ||
+        !fits_grid(blocks * prm.n_seqs * prm.heads_kv, kf::kWeighThreads))
+        return KF_ERR_SIZE;
+    const dim3 grid((unsigned)(blocks * prm.n_seqs * prm.heads_kv)), block(kf::kWeighThreads);
+    (void)hipGetLastError();
+    switch (D) {
+        case 64: kf::kf_kv_weigh_kernel<kBF, 64><<<grid, block, 0, stream>>>(prm); break;
+        case 128: kf::kf_kv_weigh_kernel<kBF, 128><<<grid, block, 0, stream>>>(prm); break;
+        default: kf::kf_kv_weigh_kernel<kBF, 256><<<grid, block, 0, stream>>>(prm);
+    }
+    return launched();
+}
+
+// ---- The 16-bit cache: new tokens, eviction. ----
+
+template <int D>
+int launch_append(kf::KvAppendParams& prm, hipStream_t stream) {
+    prm.tile = cache_tile(prm, D);
+    const dim3 grid((prm.tokens + prm.tile - 1) / prm.tile), block(kf::kKv4Threads);
+    if (!fits_grid(grid.x, kf::kKv4Threads)) return KF_ERR_SIZE;
+    (void)hipGetLastError();
+    kf::kf_kv_append_kernel<D><<<grid, block, 0, stream>>>(prm);
+    return launched();
+}
+
+struct EvictPlan {
+    int shift, capacity;
+    size_t counts_bytes, cuts_bytes, ws_bytes;
+};
+
+int evict_plan(int n_seqs, int H_kv, int D, int page_size, int max_pages, int num_pages, EvictPlan* pl) {
+    if (D != 64 && D != 128 && D != 256) return KF_ERR_HEAD_DIM;
+    if (n_seqs <= 0 || H_kv <= 0) return KF_ERR_SIZE;
+    if (const int st = paged_geometry(page_size, max_pages, num_pages, &pl->shift, &pl->capacity); st != KF_OK) return st;
+    const long long groups = (long long)n_seqs * H_kv;
+    if (pl->capacity > kMaxIndex || !fits_grid(groups, kf::kSelectThreads) ||
+        !fits_grid(groups * (D / 32), kf::kMoveThreads))
+        return KF_ERR_SIZE;
+    pl->counts_bytes = align_up((size_t)groups * sizeof(int), kWsAlign);
+    pl->cuts_bytes = align_up((size_t)groups * 2 * sizeof(int), kWsAlign);
+    pl->ws_bytes = pl->counts_bytes + pl->cuts_bytes + align_up((size_t)groups * pl->capacity * sizeof(int), kWsAlign);
+    return KF_OK;
+}
+
+template <int D>
+int launch_evict(const kf::EvictParams& prm, hipStream_t stream) {
+    const int groups = prm.n_seqs * prm.heads;
+    (void)hipGetLastError();
+    kf::kf_kv_evict_select_kernel<<<dim3(groups), dim3(kf::kSelectThreads), 0, stream>>>(prm);
+    if (const int st = launched(); st != KF_OK) return st;
+    kf::kf_kv_evict_move_kernel<D><<<dim3(groups * (D / 32)), dim3(kf::kMoveThreads), 0, stream>>>(prm);
+    return launched();
 }
 
 }  // namespace
@@ -496,6 +652,146 @@ int kf_attn_decode_kv4(const void* Q, const void* K_pages, const void* V_pages, 
         case 64: return launch_kv4<false, 64>(pl, prm, s);
         case 128: return launch_kv4<false, 128>(pl, prm, s);
         default: return launch_kv4<false, 256>(pl, prm, s);
+    }
+}
+
+int kf_kv_append(const void* K, const void* V, const int64_t* strides, void* K_pages, void* V_pages, float* weights,
+                 const int* block_table, const int* seq_starts, const int* kv_lens, int n_seqs, int tokens, int H_kv,
+                 int D, int page_size, int max_pages_per_seq, int num_pages, int flags, void* stream) {
+    kf::KvAppendParams prm{};
+    if (const int st = check_kv4(tokens, n_seqs, H_kv, D, page_size, max_pages_per_seq, num_pages, flags, block_table,
+                                 seq_starts, kv_lens, &prm);
+        st != KF_OK)
+        return st;
+    if (!K || !V || !K_pages || !V_pages) return KF_ERR_NULL;
+    if (!aligned16(K) || !aligned16(V) || !aligned16(K_pages) || !aligned16(V_pages) || !aligned4(weights))
+        return KF_ERR_ALIGN;
+    const int64_t packed[4] = {(int64_t)H_kv * D, D, (int64_t)H_kv * D, D};
+    if (!strides) strides = packed;
+    if (const int st = check_strides(strides, 4); st != KF_OK) return st;
+    prm.x[0] = static_cast<const uint16_t*>(K);
+    prm.x[1] = static_cast<const uint16_t*>(V);
+    prm.pages[0] = static_cast<uint8_t*>(K_pages);
+    prm.pages[1] = static_cast<uint8_t*>(V_pages);
+    for (int i = 0; i < 2; ++i) {
+        prm.token[i] = strides[2 * i];
+        prm.head[i] = strides[2 * i + 1];
+    }
+    prm.page_bytes = (size_t)page_size * D * 2;
+    prm.weights = weights;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (D) {
+        case 64: return launch_append<64>(prm, s);
+        case 128: return launch_append<128>(prm, s);
+        default: return launch_append<256>(prm, s);
+    }
+}
+
+size_t kf_attn_paged_workspace_bytes(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size,
+                                     int max_pages_per_seq) {
+    PagedPlan pl{};
+    return paged_plan(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq, 1, &pl) == KF_OK ? pl.ws_bytes : 0;
+}
+
+int kf_attn_paged(const void* Q, const int64_t* strides, const void* K_pages, const void* V_pages,
+                  const int* block_table, const int* seq_starts, const int* kv_lens, void* O, float* row_max,
+                  float* row_sumexp, int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size,
+                  int max_pages_per_seq, int num_pages, int flags, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+    PagedPlan pl{};
+    if (const int st = paged_plan(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq, num_pages, &pl);
+        st != KF_OK)
+        return st;
+    if (const int st = check_attn_flags(flags); st != KF_OK) return st;
+    if (!Q || !K_pages || !V_pages || !O || !block_table || !seq_starts || !kv_lens) return KF_ERR_NULL;
+    if (!aligned16(Q) || !aligned16(K_pages) || !aligned16(V_pages) || !aligned16(O)) return KF_ERR_ALIGN;
+    if (!aligned4(block_table) || !aligned4(seq_starts) || !aligned4(kv_lens)) return KF_ERR_ALIGN;
+    if (strides)
+        if (const int st = check_strides(strides, 2); st != KF_OK) return st;
+    if (pl.ws_bytes > 0) {
+        if (!workspace || workspace_bytes < pl.ws_bytes) return KF_ERR_WORKSPACE;
+        if ((reinterpret_cast<uintptr_t>(workspace) & (kWsAlign - 1)) != 0) return KF_ERR_ALIGN;
+    }
+    kf::PagedParams& prm = pl.prm;
+    set_paged(prm, Q, strides, K_pages, block_table, seq_starts, kv_lens, n_seqs, tokens, H_q, H_kv, D,
+              max_pages_per_seq, num_pages, flags);
+    prm.V = static_cast<const uint16_t*>(V_pages);
+    prm.O = static_cast<float*>(O);
+    prm.Mi = row_max;
+    prm.Li = row_sumexp;
+    prm.lse = (flags & KF_ATTN_LSE) ? 1 : 0;
+    prm.out_dtype = out_dtype(flags);
+    char* ws = static_cast<char*>(workspace);
+    prm.Opart = reinterpret_cast<float*>(ws);
+    prm.Mpart = reinterpret_cast<float*>(ws + pl.o_bytes);
+    prm.Lpart = reinterpret_cast<float*>(ws + pl.o_bytes + pl.s_bytes);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return (flags & KF_BF16) ? launch_paged_dim<true>(pl, D, s) : launch_paged_dim<false>(pl, D, s);
+}
+
+int kf_kv_weigh(const void* Q, const int64_t* strides, const void* K_pages, float* weights, const int* block_table,
+                const int* seq_starts, const int* kv_lens, const float* lse, int n_seqs, int tokens, int H_q, int H_kv,
+                int D, int page_size, int max_pages_per_seq, int num_pages, int flags, void* stream) {
+    PagedPlan pl{};
+    if (const int st = paged_plan(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq, num_pages, &pl);
+        st != KF_OK)
+        return st;
+    if ((flags & ~(KF_ATTN_CAUSAL | KF_BF16)) != 0) return KF_ERR_FLAGS;
+    if (!Q || !K_pages || !weights || !block_table || !seq_starts || !kv_lens || !lse) return KF_ERR_NULL;
+    if (!aligned16(Q) || !aligned16(K_pages)) return KF_ERR_ALIGN;
+    if (!aligned4(weights) || !aligned4(block_table) || !aligned4(seq_starts) || !aligned4(kv_lens) || !aligned4(lse))
+        return KF_ERR_ALIGN;
+    if (strides)
+        if (const int st = check_strides(strides, 2); st != KF_OK) return st;
+    set_paged(pl.prm, Q, strides, K_pages, block_table, seq_starts, kv_lens, n_seqs, tokens, H_q, H_kv, D,
+              max_pages_per_seq, num_pages, flags);
+    pl.prm.row_lse = lse;
+    pl.prm.weights = weights;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return (flags & KF_BF16) ? launch_weigh<true>(pl.prm, D, s) : launch_weigh<false>(pl.prm, D, s);
+}
+
+size_t kf_kv_evict_workspace_bytes(int n_seqs, int H_kv, int D, int page_size, int max_pages_per_seq) {
+    EvictPlan pl;
+    return evict_plan(n_seqs, H_kv, D, page_size, max_pages_per_seq, 1, &pl) == KF_OK ? pl.ws_bytes : 0;
+}
+
+int kf_kv_evict(void* K_pages, void* V_pages, float* weights, const int* block_table, const int* kv_lens,
+                const int* budgets, int* kept, int n_seqs, int H_kv, int D, int page_size, int max_pages_per_seq,
+                int num_pages, int recent, void* workspace, size_t workspace_bytes, void* stream) {
+    EvictPlan pl;
+    if (const int st = evict_plan(n_seqs, H_kv, D, page_size, max_pages_per_seq, num_pages, &pl); st != KF_OK) return st;
+    if (recent < 0) return KF_ERR_SIZE;
+    if (!K_pages || !V_pages || !weights || !block_table || !kv_lens || !budgets || !kept) return KF_ERR_NULL;
+    if (!aligned16(K_pages) || !aligned16(V_pages)) return KF_ERR_ALIGN;
+    if (!aligned4(weights) || !aligned4(block_table) || !aligned4(kv_lens) || !aligned4(budgets) || !aligned4(kept))
+        return KF_ERR_ALIGN;
+    if (!workspace || workspace_bytes < pl.ws_bytes) return KF_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & (kWsAlign - 1)) != 0) return KF_ERR_ALIGN;
+    kf::EvictParams prm{};
+    prm.pages[0] = static_cast<uint8_t*>(K_pages);
+    prm.pages[1] = static_cast<uint8_t*>(V_pages);
+    prm.weights = reinterpret_cast<uint32_t*>(weights);
+    prm.block_table = block_table;
+    prm.kv_lens = kv_lens;
+    prm.budgets = budgets;
+    prm.kept = kept;
+    prm.n_seqs = n_seqs;
+    prm.heads = H_kv;
+    prm.recent = recent;
+    prm.max_pages = max_pages_per_seq;
+    prm.page_shift = pl.shift;
+    prm.num_pages = num_pages;
+    prm.capacity = pl.capacity;
+    char* ws = static_cast<char*>(workspace);
+    prm.counts = reinterpret_cast<int*>(ws);
+    prm.cuts = reinterpret_cast<int*>(ws + pl.counts_bytes);
+    prm.moves = reinterpret_cast<int*>(ws + pl.counts_bytes + pl.cuts_bytes);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (D) {
+        case 64: return launch_evict<64>(prm, s);
+        case 128: return launch_evict<128>(prm, s);
+        default: return launch_evict<256>(prm, s);
     }
 }
 

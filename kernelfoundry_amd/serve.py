@@ -1,7 +1,8 @@
 """What a server runs beside the attention forward, on torch GPU tensors:
-packed prompts, head norms with rotary positions, and a paged K/V cache in 4
-bits with the decode that reads it (include/kf/attn.h: kf_attn_packed,
-kf_qk_norm_rope, kf_kv4_append, kf_kv4_read, kf_attn_decode_kv4).
+packed prompts, head norms with rotary positions, a paged K/V cache in 4
+bits with the decode that reads it, and one in 16 bits that is filled, attended to and
+kept small (include/kf/attn.h: kf_attn_packed, kf_qk_norm_rope, kf_kv4_append,
+kf_kv4_read, kf_attn_decode_kv4, kf_kv_append, kf_attn_paged, kf_kv_weigh, kf_kv_evict).
 
     freqs, scale = rope_freqs(128, scaling="yarn", factor=4.0, original_len=8192, device="cuda")
     Q, K = qk_norm_rope(Q, K, positions, freqs, q_weight=wq, k_weight=wk, scale=scale)
@@ -10,6 +11,11 @@ kf_qk_norm_rope, kf_kv4_append, kf_kv4_read, kf_attn_decode_kv4).
     O = attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens)             # a step
     K, V = kv4_read(K_pages, V_pages, block_table, kv_starts, kv_lens, total, 128)
     O = attn_packed(Q, K, V, seq_starts, kv_starts=kv_starts, causal=True)     # a later chunk
+
+    kv_append(K, V, K_pages, V_pages, block_table, seq_starts, kv_lens, weights=weights)
+    O, lse = attn_paged(Q, K_pages, V_pages, block_table, seq_starts, kv_lens, causal=True, return_lse=True)
+    kv_weigh(Q, K_pages, weights, block_table, seq_starts, kv_lens, lse, causal=True)
+    kv_lens = kv_evict(K_pages, V_pages, weights, block_table, kv_lens, budgets, recent=128)
 
 The entries run asynchronously on ``stream``, one of the tensors' device (default:
 torch's current one), and check their arguments on the host only; what device arrays hold
@@ -31,7 +37,7 @@ from . import (KF_ATTN_CAUSAL, KF_ERR_HIP, KF_ERR_SIZE, KF_OK, KfError, _new, _o
 KF_BF16 = 16
 KF_ROPE_INTERLEAVED = 32
 
-_STRIDES = {n: ctypes.c_int64 * n for n in (4, 6, 8)}
+_STRIDES = {n: ctypes.c_int64 * n for n in (2, 4, 6, 8)}
 _WIDE_STRIDE = 1 << 28   # of tokens: the most that attn_packed takes of K and V
 _MOST = 2 ** 31 - 1      # a size of the C entries: an int, to which ctypes cuts without a word
 
@@ -433,3 +439,204 @@ def attn_decode_kv4(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, caus
             lse.data_ptr() if return_lse else None, None, B, q_len, H_q, H_kv, D, page_size, max_pages, num_pages,
             flags, workspace.data_ptr() if workspace is not None else None, need)
     return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# The 16-bit cache.
+# ---------------------------------------------------------------------------
+def _pools(torch, names, dtype, *pools):
+    """The shape of page pools [num_pages, H_kv, page_size, D] of one shape and type."""
+    shape = pools[0].shape
+    if len(shape) != 4:
+        raise ValueError(f"{names[0]} must be [num_pages, H_kv, page_size, D]")
+    for name, t in zip(names, pools):
+        if t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{' and '.join(names)} must be contiguous and of one shape")
+        if t.dtype is not dtype:
+            raise TypeError(f"{name} must be {dtype}, as the other 16-bit tensors")
+    if shape[0] > _MOST or shape[1] > _MOST or shape[2] > _MOST:
+        raise _too_many()
+    return shape
+
+
+def _weights(torch, weights, pools):
+    if weights.dtype is not torch.float32 or weights.shape != pools[:3] or not weights.is_contiguous():
+        raise ValueError(f"weights must be a contiguous float32 tensor of shape {tuple(pools[:3])}")
+    return weights.data_ptr()
+
+
+def kv_append(K, V, K_pages, V_pages, block_table, seq_starts, kv_lens, *, weights=None, stream=None):
+    """Write new tokens into a paged 16-bit cache.
+
+    K, V [T, H_kv, D] float16 or bfloat16, packed by ``seq_starts`` (int32 [N + 1]),
+    with any token and head strides (multiples of 8); K_pages, V_pages [num_pages,
+    H_kv, page_size, D] of the same type, D = 64, 128 or 256.  Sequence b's tokens become
+    the last of its ``kv_lens[b]`` keys (int32 [N], counted with them);
+    ``block_table`` int32 [N, max_pages].  ``weights`` (float32 [num_pages, H_kv,
+    page_size]): those of the new tokens become 0.  Tokens of an invalid page are not
+    written; no two tokens of a call may have the same row.
+    """
+    import torch
+
+    device = _gpu(torch, ("K", "V", "K_pages", "V_pages", "weights"), K, V, K_pages, V_pages, weights)
+    flags = _half(torch, "KV", K, V)
+    strides = _STRIDES[4](*_heads("K", K), *_heads("V", V))
+    T, H_kv, D = K.shape
+    pools = num_pages, heads, page_size, Dp = _pools(torch, ("K_pages", "V_pages"), K.dtype, K_pages, V_pages)
+    if V.shape != K.shape or heads != H_kv or Dp != D:
+        raise ValueError("K and V must be [T, H_kv, D], with the pools' H_kv and D")
+    starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
+    table, lens = _table(torch, block_table, kv_lens, device, n)
+    max_pages = block_table.shape[1]
+    if T > _MOST or n > _MOST or max_pages > _MOST:
+        raise _too_many()
+    _launch(torch, device, stream, load_library().kf_kv_append,
+            K.data_ptr(), V.data_ptr(), strides, K_pages.data_ptr(), V_pages.data_ptr(),
+            None if weights is None else _weights(torch, weights, pools), table, starts, lens, n, T, H_kv, D,
+            page_size, max_pages, num_pages, flags)
+
+
+def paged_attn_workspace_bytes(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq) -> int:
+    """Workspace of attn_paged (kf_attn_paged_workspace_bytes)."""
+    return int(load_library().kf_attn_paged_workspace_bytes(n_seqs, tokens, H_q, H_kv, D, page_size,
+                                                            max_pages_per_seq))
+
+
+def evict_workspace_bytes(n_seqs, H_kv, D, page_size, max_pages_per_seq) -> int:
+    """Workspace of kv_evict (kf_kv_evict_workspace_bytes)."""
+    return int(load_library().kf_kv_evict_workspace_bytes(n_seqs, H_kv, D, page_size, max_pages_per_seq))
+
+
+@functools.lru_cache(maxsize=1024)
+def _need(size_of, index, *sizes):
+    """A workspace's bytes on device `index`, by the sizes alone."""
+    import torch
+
+    with torch.cuda.device(index):
+        return size_of(*sizes)
+
+
+def _workspace_at(torch, workspace, need, t, stream):
+    """The caller's workspace if it has `need` bytes, or a new one on t's device."""
+    if not need:
+        return None
+    if workspace is None:
+        return _new_at(torch, t, need, torch.uint8, stream)
+    return _workspace(torch, workspace, need, lambda: need, t.device, stream)[0]
+
+
+def attn_paged(Q, K_pages, V_pages, block_table, seq_starts, kv_lens, out=None, *, causal=False, workspace=None,
+               stream=None, out_dtype=None, return_lse=False):
+    """Attention of packed new tokens over a paged 16-bit cache.
+
+    Q [T, H_q, D], packed by ``seq_starts`` (int32 [N + 1]), with any token and head strides
+    (multiples of 8); K_pages, V_pages [num_pages, H_kv, page_size, D]; all float16
+    or bfloat16, D = 64, 128 or 256.  ``kv_lens`` int32 [N]: the keys of each sequence,
+    of which its tokens are the last (kv_append them first): one for a step, many for a
+    chunk of a prompt over its context, any mix.  ``block_table`` int32 [N,
+    max_pages]; a key on an invalid page counts as none.  ``causal``: query i of n
+    sees keys j <= i + kv_lens[b] - n.
+    Returns O [T, H_q, D] (fp32, or ``out_dtype``), or (O, LSE [T, H_q]) with
+    ``return_lse``; a row without keys gets O = 0, LSE = -inf.  Rows outside
+    the sequences are not written.  The softmax weights are rounded to the inputs' type
+    before they meet V; scores q . k / sqrt(D) may reach 9e7.  ``workspace``: a buffer of
+    paged_attn_workspace_bytes to use instead of a new one.
+    """
+    import torch
+
+    device = _gpu(torch, ("Q", "K_pages", "V_pages"), Q, K_pages, V_pages)
+    flags = _out_flags(torch, out_dtype, return_lse) | _half(torch, "Q", Q)
+    strides = _STRIDES[2](*_heads("Q", Q))
+    T, H_q, D = Q.shape
+    num_pages, H_kv, page_size, Dp = _pools(torch, ("K_pages", "V_pages"), Q.dtype, K_pages, V_pages)
+    if Dp != D:
+        raise ValueError("Q must have the pools' D")
+    starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
+    table, lens = _table(torch, block_table, kv_lens, device, n)
+    max_pages = block_table.shape[1]
+    if T > _MOST or H_q > _MOST or n > _MOST or max_pages > _MOST:
+        raise _too_many()
+    if out is None:
+        out = _like(torch, Q, out_dtype or torch.float32, stream)
+    else:
+        out = _output(torch, out, (T, H_q, D), out_dtype, device, stream)
+    lse = _new_at(torch, Q, (T, H_q), torch.float32, stream) if return_lse else None
+    need = _need(paged_attn_workspace_bytes, device.index, n, T, H_q, H_kv, D, page_size, max_pages)
+    workspace = _workspace_at(torch, workspace, need, Q, stream)
+    if causal:
+        flags |= KF_ATTN_CAUSAL
+    _launch(torch, device, stream, load_library().kf_attn_paged,
+            Q.data_ptr(), strides, K_pages.data_ptr(), V_pages.data_ptr(), table, starts, lens, out.data_ptr(),
+            lse.data_ptr() if return_lse else None, None, n, T, H_q, H_kv, D, page_size, max_pages, num_pages, flags,
+            workspace.data_ptr() if workspace is not None else None, need)
+    return (out, lse) if return_lse else out
+
+
+def kv_weigh(Q, K_pages, weights, block_table, seq_starts, kv_lens, lse, *, causal=False, stream=None):
+    """Add the attention weight that keys of a paged 16-bit cache get from new tokens.
+
+    weights[j] (float32 [num_pages, H_kv, page_size], by the pages of the keys) += the sum of
+    exp(q . k_j / sqrt(D) - lse) over the tokens that see key j and the query heads of
+    its KV head.  ``lse`` float32 [T, H_q] as attn_paged returns it (a row of -inf adds
+    nothing), the other arguments as attn_paged's.  Sequences must not share pages.
+    """
+    import torch
+
+    device = _gpu(torch, ("Q", "K_pages", "weights", "lse"), Q, K_pages, weights, lse)
+    flags = _half(torch, "Q", Q)
+    strides = _STRIDES[2](*_heads("Q", Q))
+    T, H_q, D = Q.shape
+    pools = num_pages, H_kv, page_size, Dp = _pools(torch, ("K_pages",), Q.dtype, K_pages)
+    if Dp != D:
+        raise ValueError("Q must have the pool's D")
+    starts, n = _starts(torch, "seq_starts", seq_starts, device), seq_starts.shape[0] - 1
+    table, lens = _table(torch, block_table, kv_lens, device, n)
+    max_pages = block_table.shape[1]
+    if T > _MOST or H_q > _MOST or n > _MOST or max_pages > _MOST:
+        raise _too_many()
+    if lse.dtype is not torch.float32 or lse.shape != (T, H_q) or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous float32 [T, H_q] tensor")
+    if causal:
+        flags |= KF_ATTN_CAUSAL
+    _launch(torch, device, stream, load_library().kf_kv_weigh,
+            Q.data_ptr(), strides, K_pages.data_ptr(), _weights(torch, weights, pools), table, starts, lens,
+            lse.data_ptr(), n, T, H_q, H_kv, D, page_size, max_pages, num_pages, flags)
+
+
+def kv_evict(K_pages, V_pages, weights, block_table, kv_lens, budgets, out=None, *, recent=0, workspace=None,
+             stream=None):
+    """Cut the sequences of a paged 16-bit cache to ``budgets`` (int32 [N]) keys.
+
+    Of every KV head the last ``recent`` keys stay, and of the others those with the largest
+    ``weights`` (float32 [num_pages, H_kv, page_size]; ties to the lowest place, a NaN
+    above any number).  With n keys cut to m, r = min(recent, m) and k = m - r: kept keys in
+    places below k stay there, the others go in order to the places below k that were
+    freed, and the last r to k .. m - 1.  K, V and weights move; places from m on are
+    left as they were.
+    Returns the new key counts, int32 [N] (``out``, which may be kv_lens): a sequence with an
+    invalid page among its keys is left as it is.  Sequences that are cut must not share
+    pages.  ``workspace``: a buffer of evict_workspace_bytes to use instead of a new one.
+    """
+    import torch
+
+    device = _gpu(torch, ("K_pages", "V_pages", "weights"), K_pages, V_pages, weights)
+    _half(torch, ("K_pages", "V_pages"), K_pages, V_pages)
+    pools = num_pages, H_kv, page_size, D = _pools(torch, ("K_pages", "V_pages"), K_pages.dtype, K_pages, V_pages)
+    n, max_pages = block_table.shape if block_table.dim() == 2 else (-1, 0)
+    table, lens = _table(torch, block_table, kv_lens, device, n)
+    if n > _MOST or max_pages > _MOST or recent > _MOST:
+        raise _too_many()
+    if recent < 0:
+        raise ValueError("recent must not be negative")
+    least = _ints(torch, "budgets", budgets, device, (n,))
+    if out is None:
+        out = _like(torch, kv_lens, torch.int32, stream)
+    else:
+        _ints(torch, "out", out, device, (n,))
+    need = _need(evict_workspace_bytes, device.index, n, H_kv, D, page_size, max_pages)
+    workspace = _workspace_at(torch, workspace, need, K_pages, stream)
+    _launch(torch, device, stream, load_library().kf_kv_evict,
+            K_pages.data_ptr(), V_pages.data_ptr(), _weights(torch, weights, pools), table, lens, least,
+            out.data_ptr(), n, H_kv, D, page_size, max_pages, num_pages, recent,
+            workspace.data_ptr() if workspace is not None else None, need)
+    return out
