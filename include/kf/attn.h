@@ -455,11 +455,16 @@ int kf_attn_paged(const void* Q, const int64_t* strides, const void* K_pages, co
  * [tokens, H_q] is the row_max with KF_ATTN_LSE (natural logarithm); a row whose lse
  * is -inf adds nothing.  flags: KF_ATTN_CAUSAL, KF_BF16.  A NaN or an infinity in a
  * row of Q, in its lse, or in a key reaches the keys that the row sees, or the key's
- * own weight.  Sequences that share a page race for its weights: they must not. */
+ * own weight.  Sequences that share a page race for its weights: they must not.
+ * Workspace: kf_kv_weigh_workspace_bytes() bytes (may be 0, then NULL will do), as
+ * kf_attn_paged's. */
+size_t kf_kv_weigh_workspace_bytes(int n_seqs, int tokens, int H_q, int H_kv, int D,
+                                   int page_size, int max_pages_per_seq);
 int kf_kv_weigh(const void* Q, const int64_t* strides, const void* K_pages, float* weights,
                 const int* block_table, const int* seq_starts, const int* kv_lens,
                 const float* lse, int n_seqs, int tokens, int H_q, int H_kv, int D,
-                int page_size, int max_pages_per_seq, int num_pages, int flags, void* stream);
+                int page_size, int max_pages_per_seq, int num_pages, int flags,
+                void* workspace, size_t workspace_bytes, void* stream);
 
 /* Cut every sequence from n = kv_lens[b] to m = min(n, budgets[b]) keys (device int
  * [n_seqs], a negative one counts as 0).  Of every KV head the last r = min(recent, m)

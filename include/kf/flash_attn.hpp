@@ -359,16 +359,19 @@ inline hipError_t attn_paged(const uint16_t* Q, const int64_t* strides, const ui
     });
 }
 
-// kf_kv_weigh: the attention weight that keys gather.
+// kf_kv_weigh with the per-thread cached workspace: the attention weight that keys gather.
 inline hipError_t kv_weigh(const uint16_t* Q, const int64_t* strides, const uint16_t* K_pages,
                            float* weights, const int* block_table, const int* seq_starts,
                            const int* kv_lens, const float* lse, int n_seqs, int tokens, int H_q,
                            int H_kv, int D, int page_size, int max_pages_per_seq, int num_pages,
                            int flags, hipStream_t stream) {
-    return status_to_hip(kf_kv_weigh(Q, strides, K_pages, weights, block_table, seq_starts,
-                                     kv_lens, lse, n_seqs, tokens, H_q, H_kv, D, page_size,
-                                     max_pages_per_seq, num_pages, flags,
-                                     static_cast<void*>(stream)));
+    const size_t need = kf_kv_weigh_workspace_bytes(n_seqs, tokens, H_q, H_kv, D, page_size,
+                                                    max_pages_per_seq);
+    return with_workspace(stream, need, [&] { return need; }, [&](void* ws, size_t ws_bytes) {
+        return kf_kv_weigh(Q, strides, K_pages, weights, block_table, seq_starts, kv_lens, lse,
+                           n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq, num_pages,
+                           flags, ws, ws_bytes, static_cast<void*>(stream));
+    });
 }
 
 // kf_kv_evict with the per-thread cached workspace, which it cannot do without.

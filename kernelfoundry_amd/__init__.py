@@ -50,7 +50,8 @@ __all__ = [
     "workspace_bytes_least", "kernel_names",
     "KF_BF16", "KF_ROPE_INTERLEAVED", "attn_packed", "rope_freqs", "qk_norm_rope", "kv4_page_bytes",
     "kv4_append", "kv4_read", "kv4_workspace_bytes", "attn_decode_kv4",
-    "kv_append", "attn_paged", "paged_attn_workspace_bytes", "kv_weigh", "kv_evict", "evict_workspace_bytes",
+    "kv_append", "attn_paged", "paged_attn_workspace_bytes", "kv_weigh", "weigh_workspace_bytes", "kv_evict",
+    "evict_workspace_bytes",
 ]
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -186,7 +187,9 @@ def load_library(path: str = LIB_PATH):
     lib.kf_attn_paged_workspace_bytes.restype = sz
     lib.kf_attn_paged.argtypes = [p, i64s] + [p] * 8 + [i] * 9 + [p, sz, p]
     lib.kf_attn_paged.restype = i
-    lib.kf_kv_weigh.argtypes = [p, i64s] + [p] * 6 + [i] * 9 + [p]
+    lib.kf_kv_weigh_workspace_bytes.argtypes = [i] * 7
+    lib.kf_kv_weigh_workspace_bytes.restype = sz
+    lib.kf_kv_weigh.argtypes = [p, i64s] + [p] * 6 + [i] * 9 + [p, sz, p]
     lib.kf_kv_weigh.restype = i
     lib.kf_kv_evict_workspace_bytes.argtypes = [i] * 5
     lib.kf_kv_evict_workspace_bytes.restype = sz
@@ -488,4 +491,4 @@ def attn_decode_paged(Q, K_pages, V_pages, block_table, kv_lens, out=None, *, re
 
 from .serve import (KF_BF16, KF_ROPE_INTERLEAVED, attn_decode_kv4, attn_packed, attn_paged,  # noqa: E402
                     evict_workspace_bytes, kv4_append, kv4_page_bytes, kv4_read, kv4_workspace_bytes, kv_append,
-                    kv_evict, kv_weigh, paged_attn_workspace_bytes, qk_norm_rope, rope_freqs)
+                    kv_evict, kv_weigh, paged_attn_workspace_bytes, qk_norm_rope, rope_freqs, weigh_workspace_bytes)

@@ -16,12 +16,13 @@ struct PagedParams : AttnParams {  // Q, K, V, O, Mi (LSE), scales, causal, head
     long long q_token, q_head;     // strides in elements
     const int* q_starts;           // [n_seqs + 1]
     int n_seqs, tokens_q, ratio;
-    // Row tiles are cut into parts along the keys where there are too few of them for
-    // the device: `target` parts of a KV head are aimed at (0: no cuts), none smaller
-    // than min_share units of 32 << unit_shift keys.
+    // Tiles are cut into parts where there are too few of them for the device (see
+    // paged_find): `target` parts of a KV head are aimed at (0: no cuts), none smaller
+    // than min_share units.
     int target, min_share, unit_shift;
     const float* row_lse;          // kf_kv_weigh: [tokens_q][H_q]
     float* weights;                // kf_kv_weigh: [num_pages][H_kv][page_size]
+    int stride;                    // kf_kv_weigh: workgroups of a KV head
 };
 
 // One sequence's new tokens and keys.
@@ -36,29 +37,34 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int i) {
     return s;
 }
 
-// A part of a row tile: its sequence, tile and part in it, of how many, and, where there
+// The work of a sequence in a KV head: tiles, and how many units each could be cut into.
+struct PagedCount {
+    int tiles, units;
+};
+// Attention: tiles of kRows query rows, units of 32 << unit_shift keys.
+template <int kRows>
+__device__ __forceinline__ PagedCount paged_count(const PagedParams& p, int i) {
+    const PagedSeq s = paged_seq(p, i);
+    return PagedCount{(int)(((long long)s.qn * p.ratio + kRows - 1) / kRows),
+                      (key_stages(s.kn) + (1 << p.unit_shift) - 1) >> p.unit_shift};
+}
+
+// A part of a tile: its sequence, tile and part in it, of how many, and, where there
 // are several, the partial that it writes.
 struct PagedItem {
     int seq, tile, part, parts, slot;
 };
 
 // Item j of a KV head, by the lanes of a wave; false past the last.  Every tile of a
-// sequence has the same number of parts, so many that one has at most `share` units of
-// keys; `share` is the work of all tiles over p.target.  So no more than target + tiles
+// sequence has the same number of parts, so many that one has at most `share`
+// units; `share` is the work of all tiles over p.target.  So no more than target + tiles
 // parts come out, and 2 target of tiles that are cut: more than one part means more
 // than `share` units, and fewer than twice as many parts as shares.  Up to 64 sequences have a
 // lane each, of more a lane has a run of consecutive ones.  kCut: j counts the tiles
-// that are cut, not the parts.
-template <int kRows, bool kCut>
-__device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j, PagedItem& it) {
-    struct Count {
-        int tiles, units;
-    };
-    const auto count = [&](int i) {
-        const PagedSeq s = paged_seq(p, i);
-        return Count{(int)(((long long)s.qn * p.ratio + kRows - 1) / kRows),
-                     (key_stages(s.kn) + (1 << p.unit_shift) - 1) >> p.unit_shift};
-    };
+// that are cut, not the parts.  kLastFirst: a sequence's last tiles come first.
+template <bool kCut, bool kLastFirst, class CountOf>
+__device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j, PagedItem& it, const CountOf& count) {
+    using Count = PagedCount;
     const int per = (p.n_seqs + 63) / 64, first = min(lane * per, p.n_seqs), last = min(first + per, p.n_seqs);
     Count mine{0, 0};
     if (per == 1 && first < last) mine = count(first);
@@ -125,8 +131,7 @@ __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j
         it.tile = left;
     } else {
         it.part = left % it.parts;
-        // Causal tiles see the more keys the later they are: the last ones first.
-        it.tile = tiles - 1 - left / it.parts;
+        it.tile = kLastFirst ? tiles - 1 - left / it.parts : left / it.parts;
     }
     it.slot = slot + it.tile * it.parts + it.part;
     // (Of starts in no order the sums may wrap: no partial outside the workspace.)
@@ -175,7 +180,9 @@ void kf_attn_paged_kernel(PagedParams p) {
     // heads have an XCD, and its L2, each.
     const int hk = blockIdx.x % p.heads_kv;
     PagedItem it;
-    if (!paged_find<kRows, false>(p, lane, blockIdx.x / p.heads_kv, it)) return;
+    // (Causal tiles see the more keys the later they are.)
+    if (!paged_find<false, true>(p, lane, blockIdx.x / p.heads_kv, it, [&](int i) { return paged_count<kRows>(p, i); }))
+        return;
     PagedSeq sq = paged_seq(p, it.seq);
     sq.q0 = __builtin_amdgcn_readfirstlane(sq.q0);
     sq.qn = __builtin_amdgcn_readfirstlane(sq.qn);
@@ -427,7 +434,8 @@ __global__ __launch_bounds__(kPagedMergeThreads)
 void kf_attn_paged_merge_kernel(PagedParams p) {
     const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv;
     PagedItem it;
-    if (!paged_find<kRows, true>(p, lane, blockIdx.x / p.heads_kv, it)) return;
+    if (!paged_find<true, true>(p, lane, blockIdx.x / p.heads_kv, it, [&](int i) { return paged_count<kRows>(p, i); }))
+        return;
     const PagedSeq sq = paged_seq(p, it.seq);
     const int R = sq.qn * p.ratio, r0 = it.tile * kRows;
     if ((unsigned)it.tile * (unsigned)kRows >= (unsigned)R) return;
@@ -469,74 +477,402 @@ void kf_attn_paged_merge_kernel(PagedParams p) {
 // The attention weight that keys gather: weights[j] += sum over the query rows of
 // exp(s_rj - lse_r), r over the new tokens that see key j and the heads of its group.
 //
-// S^T = K Q^T by the 32x32x16 MFMA: a wave holds 32 keys as the A operand and goes
-// through the query rows, 32 at a time, as the B operand; lane l has row l % 32 of 16
-// keys, and adds their weights up in registers.  At the end the lanes' sums of a key are
-// added, and the one wave that has the key adds them to its weight: no atomics,
-// always the same order.
+// S^T = K Q^T by the 32x32x16 MFMA: a wave holds 64 keys as the A operand, straight
+// from the pages, and the query rows go by as the B operand, 32 at a time, in LDS
+// stages of 64 that the workgroup's waves share; lane l has row l % 32 of 16 keys a
+// product, and adds their weights up in registers.  At the end the lanes' sums of a
+// key are added, and the one wave that has the key adds them to its weight: no
+// atomics, always the same order.  Blocks of keys with many rows may be cut along the
+// rows (paged_find); the parts' sums then go through the workspace.
+//
+// A sequence of up to 32 rows, a step's, is read once from the pages: there the wave
+// holds the rows, and its keys go by through LDS stages of its own (weigh_step).
 // ---------------------------------------------------------------------------
 constexpr int kWeighThreads = 256;
-constexpr int kWeighKeys = 32 * kWeighThreads / 64;   // keys of a workgroup
+constexpr int kWeighRows = 64;                                      // query rows of a stage
+template <int D> struct WeighCfg {
+    // 32-key tiles of a wave: two of 256 channels would not fit its registers.
+    static constexpr int kTiles = D == 256 ? 1 : 2;
+    static constexpr int kWaveKeys = 32 * kTiles;
+    static constexpr int kKeys = kWaveKeys * kWeighThreads / 64;    // of a workgroup: a block
+    static constexpr int kWavesPerSimd = 2;
+    // Steps: 32-key tiles of a wave, channels of a stage, and the stages of a ring.
+    static constexpr int kStepTiles = 4, kStepKeys = kStepTiles * 32 * kWeighThreads / 64;
+    static constexpr int kStepWidth = D < 128 ? D : 128, kRing = D == 64 ? 4 : 2;
+    static constexpr int kStepStage = 32 * kStepWidth * 2;
+    static constexpr int kRowsBytes = 2 * kWeighRows * 2 * D, kRingBytes = kWeighThreads / 64 * kRing * kStepStage;
+    static constexpr int kLds = kRowsBytes > kRingBytes ? kRowsBytes : kRingBytes;
+};
+
+// Tiles are blocks of keys, units 64 << unit_shift query rows.
+template <int D>
+__device__ __forceinline__ PagedCount weigh_count(const PagedParams& p, int i) {
+    using Cfg = WeighCfg<D>;
+    const PagedSeq s = paged_seq(p, i);
+    const long long rows = (long long)s.qn * p.ratio;
+    const int stages = (int)((rows + kWeighRows - 1) / kWeighRows), keys = rows <= 32 ? Cfg::kStepKeys : Cfg::kKeys;
+    return PagedCount{stages > 0 ? (s.kn + keys - 1) / keys : 0, (stages + (1 << p.unit_shift) - 1) >> p.unit_shift};
+}
+
+// A block of a sequence of R <= 32 rows.  S = Q K^T: lane l has key l % 32 and 16 of the
+// rows, the sum over which needs one exchange; of fewer rows only those groups of eight
+// that there are have exponentials.  Every wave copies its own stages, 32 keys or half of
+// their 256 channels, and waits for itself alone.
+template <bool kBF, int D>
+__device__ __forceinline__ void weigh_step(const PagedParams& p, const PagedSeq& sq, int seq, int kb, int hk, int wave,
+                                           int lane, char* lds) {
+    using Cfg = WeighCfg<D>;
+    using E = Elem<kBF>;
+    using X8 = typename E::x8;
+    constexpr int W = Cfg::kStepWidth, kChunks = W / 8, kRowBytes = 2 * W, kRowsPerInstr = 1024 / kRowBytes;
+    using SW = SwizzleRow<W>;
+    constexpr int kNKK = D / 16, kStageKK = W / 16, kHalves = D / W, kHalfInstr = 16 / kRowsPerInstr;
+    const int g = lane >> 5, sh = p.page_shift, ratio = p.ratio, R = sq.qn * ratio;
+    const int k0 = kb + wave * (32 * Cfg::kStepTiles), keys = sq.kn - k0;
+    if (keys <= 0) return;
+    const int ntiles = min((keys + 31) / 32, Cfg::kStepTiles), nst = ntiles * kHalves;
+    // The ids of the wave's pages, one to a lane: no more than 9.
+    const int page0 = k0 >> sh;
+    const int ids = p.block_table[(size_t)seq * p.max_pages + min(page0 + lane, (sq.kn - 1) >> sh)];
+    const int lr = lane / kChunks;
+    uint32_t lane_off[kHalfInstr];
+#pragma unroll
+    for (int i = 0; i < kHalfInstr; ++i) {
+        const int r = i * kRowsPerInstr + lr;
+        lane_off[i] = (uint32_t)(r * 2 * D) + (((lane % kChunks) ^ SW::h(r)) % kChunks) * 16;
+    }
+    char* const ring = lds + wave * (Cfg::kRing * Cfg::kStepStage);
+    const auto issue = [&](int s) {
+        const uint32_t d_lds = (uint32_t)(uintptr_t)(lds_void*)(ring + s % Cfg::kRing * Cfg::kStepStage);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // (Rows behind the keys lie in their page still, or are those of page 0.)
+            const int key = k0 + s / kHalves * 32 + 16 * h;
+            const int id = key < sq.kn ? __builtin_amdgcn_readlane(ids, (key >> sh) - page0) : 0;
+            const size_t row = (((size_t)((unsigned)id < (unsigned)p.num_pages ? id : 0) * p.heads_kv + hk) << sh) +
+                               (key & ((1 << sh) - 1));
+            const char* const src = reinterpret_cast<const char*>(p.K) + row * (2 * D) + s % kHalves * kRowBytes;
+#pragma unroll
+            for (int i = 0; i < kHalfInstr; ++i)
+                lds_copy16(d_lds + (h * kHalfInstr + i) * 1024, src, lane_off[i]);
+        }
+    };
+    // The rows, those past the last as the last, and what their exponents are less by: those and
+    // rows without a key add nothing.  Loads in front of the stages', which are counted.
+    X8 q[kNKK];
+    const int row = min(lane & 31, R - 1);
+    {
+        const uint16_t* Qr = p.Q + (size_t)(sq.q0 + row / ratio) * p.q_token + (size_t)(hk * ratio + row % ratio) * p.q_head;
+#pragma unroll
+        for (int kk = 0; kk < kNKK; ++kk) q[kk] = *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8);
+    }
+    const float e = p.row_lse[((size_t)(sq.q0 + row / ratio) * p.heads_kv + hk) * ratio + row % ratio];
+    // This lane's key of every tile: its weight.
+    float* to[Cfg::kStepTiles];
+    float sum[Cfg::kStepTiles];
+#pragma unroll
+    for (int t = 0; t < Cfg::kStepTiles; ++t) {
+        const int key = k0 + 32 * t + (lane & 31);
+        const int id = __shfl(ids, min((key >> sh) - page0, 63));
+        to[t] = key < sq.kn && (unsigned)id < (unsigned)p.num_pages
+                    ? p.weights + (((size_t)id * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1)) : nullptr;
+        sum[t] = to[t] && g == 0 ? *to[t] : 0.f;
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    const float less_row = (lane & 31) < R && e > -INFINITY ? -e * kLog2e : -INFINITY;
+    float less[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) less[r] = __shfl(less_row, 8 * (r >> 2) + (r & 3) + 4 * g);
+    const int before = sq.kn - sq.qn;
+#pragma unroll
+    for (int s = 0; s < Cfg::kRing - 1; ++s)
+        if (s < nst) issue(s);
+    int koff[kStageKK];
+#pragma unroll
+    for (int kk = 0; kk < kStageKK; ++kk) {
+        const int r = lane & 31;
+        koff[kk] = r * kRowBytes + (((2 * kk + g) ^ SW::h(r)) % kChunks) * 16;
+    }
+#pragma unroll
+    for (int t = 0; t < Cfg::kStepTiles; ++t) {
+        if (t >= ntiles) break;
+        f32x16 x = {};
+#pragma unroll
+        for (int hf = 0; hf < kHalves; ++hf) {
+            const int s = t * kHalves + hf;
+            if (s + Cfg::kRing - 1 < nst) {
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage there has been read
+                issue(s + Cfg::kRing - 1);
+            }
+            // This stage has landed where no more than the later ones' copies are on their way.
+            const int ahead = min(Cfg::kRing - 1, nst - 1 - s);
+            asm volatile("" ::: "memory");
+            if (ahead >= 3) __builtin_amdgcn_s_waitcnt(0x0f70 | (6 * kHalfInstr & 15) | (6 * kHalfInstr >> 4) << 14);
+            else if (ahead == 2) __builtin_amdgcn_s_waitcnt(0x0f70 | (4 * kHalfInstr & 15) | (4 * kHalfInstr >> 4) << 14);
+            else if (ahead == 1) __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * kHalfInstr & 15) | (2 * kHalfInstr >> 4) << 14);
+            else __builtin_amdgcn_s_waitcnt(0x0f70);
+            asm volatile("" ::: "memory");
+            const char* const stage = ring + s % Cfg::kRing * Cfg::kStepStage;
+#pragma unroll
+            for (int kk = 0; kk < kStageKK; ++kk)
+                x = E::mfma32(q[hf * kStageKK + kk], *reinterpret_cast<const X8*>(stage + koff[kk]), x);
+        }
+        // The last key of the tile that row 0 sees too: from there on rows have limits.
+        const int key = k0 + 32 * t + (lane & 31);
+        const bool whole = !p.causal || k0 + 32 * t + 32 <= before + 1;
+        float add = 0.f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            if (8 * b >= R) break;
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = exp2_hw(fmaf(x[4 * b + i], p.scale_log2, less[4 * b + i]));
+            if (!whole) {
+                asm volatile("" ::: "memory");       // a branch, not selects in every tile
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key > before + (8 * b + 4 * g + i) / ratio) w[i] = 0.f;
+            }
+            add += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+        sum[t] += add + __shfl_xor(add, 32);
+    }
+#pragma unroll
+    for (int t = 0; t < Cfg::kStepTiles; ++t)
+        if (to[t] && g == 0) *to[t] = sum[t];
+}
 
 template <bool kBF, int D>
-__global__ __launch_bounds__(kWeighThreads)
+__global__ __launch_bounds__(kWeighThreads, WeighCfg<D>::kWavesPerSimd)
 void kf_kv_weigh_kernel(PagedParams p) {
     using E = Elem<kBF>;
     using X8 = typename E::x8;
-    constexpr int kNKK = D / 16;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
-    const int hk = blockIdx.x % p.heads_kv, sh = p.page_shift;
-    const int blocks = (p.kv_len + kWeighKeys - 1) / kWeighKeys;
-    const int seq = blockIdx.x / p.heads_kv / blocks, block = blockIdx.x / p.heads_kv % blocks;
-    const PagedSeq sq = paged_seq(p, seq);
-    const int R = sq.qn * p.ratio, k0 = block * kWeighKeys + wave * 32;
-    if (k0 >= sq.kn || R == 0) return;
-    const int* const table = p.block_table + (size_t)seq * p.max_pages;
-    // This lane's key of the A operand.  Past the keys, or on no valid page, any row will do:
-    // it reaches no other key's sum, and its own is dropped.
-    const auto page_of = [&](int key) { return key < sq.kn ? table[key >> sh] : -1; };
-    const auto valid = [&](int id) { return (unsigned)id < (unsigned)p.num_pages; };
-    const int key = k0 + (lane & 31), id = page_of(key);
-    const uint16_t* Kr = p.K + ((((size_t)(valid(id) ? id : 0) * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))) * D;
-    X8 kf[kNKK];
-#pragma unroll
-    for (int kk = 0; kk < kNKK; ++kk) kf[kk] = *reinterpret_cast<const X8*>(Kr + (2 * kk + g) * 8);
-    f32x16 sum = {};
-    // Causal: query i sees keys j <= i + before; the first that sees any of these.
-    const int before = sq.kn - sq.qn;
-    const int first = p.causal ? max(k0 - before, 0) : 0;
-    for (int r0 = first * p.ratio / 32 * 32; r0 < R; r0 += 32) {
-        const int row = min(r0 + (lane & 31), R - 1), q = row / p.ratio;
-        const uint16_t* Qr = p.Q + (size_t)(sq.q0 + q) * p.q_token + (size_t)(hk * p.ratio + row % p.ratio) * p.q_head;
-        const float e = p.row_lse[((size_t)(sq.q0 + q) * p.heads_kv + hk) * p.ratio + row % p.ratio];
-        f32x16 s = {};
-#pragma unroll
-        for (int kk = 0; kk < kNKK; ++kk) s = E::mfma32(kf[kk], *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8), s);
-        // Rows past the last, and those without a key, add nothing.
-        const float off = r0 + (lane & 31) < R && e > -INFINITY ? -e * kLog2e : -INFINITY;
-        const int lim = (p.causal ? q + before + 1 : sq.kn) - k0 - 4 * g;   // keys of this lane that the row sees
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float w = exp2_hw(fmaf(s[r], p.scale_log2, off));
-            sum[r] += 8 * (r >> 2) + (r & 3) < lim ? w : 0.f;
+    using SW = SwizzleRow<D>;
+    constexpr int kNKK = D / 16, kChunks = D / 8, kRowBytes = 2 * D, kRowsPerInstr = 1024 / kRowBytes;
+    constexpr int kWaves = kWeighThreads / 64, kInstr = kWeighRows / kRowsPerInstr / kWaves;  // of a wave and stage
+    constexpr int kTiles = WeighCfg<D>::kTiles, kWaveKeys = WeighCfg<D>::kWaveKeys, kKeys = WeighCfg<D>::kKeys;
+    constexpr bool kXorOff = D >= 128;
+    __shared__ __attribute__((aligned(1024))) char lds[WeighCfg<D>::kLds];
+    const auto buf = [&](int s) { return lds + (s & 1) * (kWeighRows * kRowBytes); };
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hk = blockIdx.x % p.heads_kv, sh = p.page_shift, ratio = p.ratio;
+    for (int j = blockIdx.x / p.heads_kv;; j += p.stride) {
+        // (An opaque lane: nothing that is derived from it lives across the items.)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int g = lane >> 5;
+        PagedItem it;
+        if (!paged_find<false, false>(p, lane, j, it, [&](int i) { return weigh_count<D>(p, i); })) return;
+        PagedSeq sq = paged_seq(p, it.seq);
+        sq.q0 = __builtin_amdgcn_readfirstlane(sq.q0);
+        sq.qn = __builtin_amdgcn_readfirstlane(sq.qn);
+        sq.kn = __builtin_amdgcn_readfirstlane(sq.kn);
+        const int R = sq.qn * ratio;
+        // (Of starts in no order the sums by which the item was found may wrap.)
+        const bool step = R <= 32;
+        const int kb = it.tile * (step ? WeighCfg<D>::kStepKeys : kKeys), k0 = kb + wave * kWaveKeys;
+        if ((unsigned)kb >= (unsigned)sq.kn || R == 0) continue;
+        if (step) {
+            weigh_step<kBF, D>(p, sq, it.seq, kb, hk, wave, lane, lds);
+            __syncthreads();  // every wave is done with its stages
+            continue;
         }
-    }
-    // Over the 32 rows: with every exchange a lane keeps half of its keys, in the end
-    // lane l (and l ^ 16) the one of register l % 16.
+        // LDS-DMA, as in the attention kernels: lane l of an instruction fills row l / kChunks of
+        // its rows, physical chunk l % kChunks.
+        const auto row_of = [&](int l, int i) { return (wave * kInstr + i) * kRowsPerInstr + l / kChunks; };
+        const auto chunk_off = [&](int l, int i) {
+            return (uint32_t)((((l % kChunks) ^ SW::h(row_of(l, i))) % kChunks) * 16);
+        };
+        // Whole stages begin at a token, and their lanes' offsets from it have 32 bits.
+        const bool plain = kWeighRows % ratio == 0 &&
+                           kWeighRows / ratio * p.q_token + ratio * p.q_head < (1LL << 30);
+        uint32_t off[kInstr], lse_off[2];
 #pragma unroll
-    for (int b = 3; b >= 0; --b)
-#pragma unroll
-        for (int r = 0; r < 1 << b; ++r) {
-            const bool up = (lane >> b & 1) != 0;
-            const float give = up ? sum[r] : sum[r + (1 << b)];
-            sum[r] = (up ? sum[r + (1 << b)] : sum[r]) + __shfl_xor(give, 1 << b);
+        for (int i = 0; i < kInstr; ++i) {
+            const int row = row_of(lane, i), q = row / ratio;
+            off[i] = (uint32_t)((q * p.q_token + (row - q * ratio) * p.q_head) * 2) + chunk_off(lane, i);
         }
-    const float total = sum[0] + __shfl_xor(sum[0], 16);
-    const int to = k0 + acc_row(lane & 15, lane), to_id = page_of(to);
-    if ((lane & 16) == 0 && valid(to_id)) {
-        float* const w = p.weights + (((size_t)to_id * p.heads_kv + hk) << sh) + (to & ((1 << sh) - 1));
-        *w += total;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = 32 * h + (lane & 31), q = row / ratio;
+            lse_off[h] = (uint32_t)(q * p.heads_kv * ratio + (row - q * ratio)) * 4;
+        }
+        int koff[kNKK];
+#pragma unroll
+        for (int kk = 0; kk < kNKK; ++kk) {
+            const int r = lane & 31;
+            koff[kk] = r * kRowBytes + (((2 * kk + g) ^ SW::h(r)) % kChunks) * 16;
+        }
+        const int* const table = p.block_table + (size_t)it.seq * p.max_pages;
+        const auto page_of = [&](int key) { return key < sq.kn ? table[key >> sh] : -1; };
+        const auto valid = [&](int id) { return (unsigned)id < (unsigned)p.num_pages; };
+        // The keys of the A operand.  Past the last, or on no valid page, any row will do: it
+        // reaches no other key's sum, and its own is dropped.
+        X8 kf[kTiles][kNKK];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int key = k0 + 32 * t + (lane & 31), id = page_of(key);
+            const uint16_t* Kr = p.K + ((((size_t)(valid(id) ? id : 0) * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))) * D;
+#pragma unroll
+            for (int kk = 0; kk < kNKK; ++kk) kf[t][kk] = *reinterpret_cast<const X8*>(Kr + (2 * kk + g) * 8);
+        }
+        // Causal: query i sees keys j <= i + before.  Rows in front of the first that sees any
+        // of the block's do not count.
+        const int before = sq.kn - sq.qn;
+        const int first = p.causal ? max(kb - before, 0) * ratio : 0;
+        const int s_first = first / kWeighRows, stages = (R + kWeighRows - 1) / kWeighRows;
+        const int per = (stages - s_first + it.parts - 1) / it.parts;
+        const int s0 = s_first + it.part * per, s1 = min(s0 + per, stages);
+        const char* const Qh = reinterpret_cast<const char*>(p.Q + (size_t)sq.q0 * p.q_token + (size_t)hk * ratio * p.q_head);
+        const float* const lse = p.row_lse + ((size_t)sq.q0 * p.heads_kv + hk) * ratio;
+        const size_t stage_bytes = (size_t)(kWeighRows / ratio) * p.q_token * 2;
+        // Requests a stage, and this lane's row of each half of it: what its exponents are less
+        // by.  (Other stages than whole ones from an opaque lane.)
+        const auto issue_stage = [&](int s, float (&e)[2]) {
+            const int r0 = s * kWeighRows;
+            const uint32_t d_lds = (uint32_t)(uintptr_t)(lds_void*)(buf(s) + wave * kInstr * 1024);
+            if (plain && r0 + kWeighRows <= R) {
+                const char* const src = Qh + s * stage_bytes;
+#pragma unroll
+                for (int i = 0; i < kInstr; ++i) lds_copy16(d_lds + i * 1024, src, off[i]);
+                const char* const at = reinterpret_cast<const char*>(lse + (size_t)r0 * p.heads_kv);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) e[h] = *reinterpret_cast<const float*>(at + lse_off[h]);
+            } else {
+                int l = lane;
+                asm volatile("" : "+v"(l));
+#pragma unroll
+                for (int i = 0; i < kInstr; ++i) {
+                    const int row = min(r0 + row_of(l, i), R - 1), q = row / ratio;
+                    lds_copy16(d_lds + i * 1024, Qh + ((size_t)q * p.q_token + (size_t)(row - q * ratio) * p.q_head) * 2 +
+                                                     chunk_off(l, i));
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = min(r0 + 32 * h + (l & 31), R - 1), q = row / ratio;
+                    e[h] = lse[(size_t)q * p.heads_kv * ratio + (row - q * ratio)];
+                }
+            }
+        };
+        // Rows in front of this one do not see all keys of the wave.
+        const int whole = p.causal ? max(k0 + kWaveKeys - 1 - before, 0) * ratio : 0;
+        f32x16 sum[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) sum[t] = f32x16{};
+        // The scores of 32 rows, and beside their products the exponentials of `old` ones, the
+        // instructions in this order: a wave overlaps the two only as they stand in its stream.
+        const auto scores = [&](const char* rows, f32x16 (&x)[kTiles], const f32x16 (&old)[kTiles], float less) {
+            constexpr int kPer = 16 * kTiles / kNKK;
+            int kb0 = koff[0];
+            if constexpr (kXorOff) asm volatile("" : "+v"(kb0));  // derived per tile
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) x[t] = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < kNKK; ++kk) {
+                const X8 q = *reinterpret_cast<const X8*>(rows + (kXorOff ? kb0 ^ (32 * kk) : koff[kk]));
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) x[t] = E::mfma32(kf[t][kk], q, x[t]);
+#pragma unroll
+                for (int i = kk * kPer; i < (kk + 1) * kPer; ++i)
+                    sum[i / 16][i % 16] += exp2_hw(fmaf(old[i / 16][i % 16], p.scale_log2, less));
+                __builtin_amdgcn_sched_barrier(0x100);            // LDS reads may pass
+            }
+        };
+        const auto gather = [&](const f32x16 (&x)[kTiles], float less) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum[t][r] += exp2_hw(fmaf(x[t][r], p.scale_log2, less));
+        };
+        // Rows without a key add nothing.
+        const auto less_of = [&](float e) { return e > -INFINITY ? -e * kLog2e : -INFINITY; };
+        float e_next[2] = {0.f, 0.f};
+        if (s0 < s1) issue_stage(s0, e_next);
+        // The second half's scores wait for their exponentials until the next products: every
+        // product then runs beside other rows' exponentials.
+        f32x16 late[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) late[t] = f32x16{};
+        float late_less = -INFINITY;
+        for (int s = s0; s < s1; ++s) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const float e[2] = {e_next[0], e_next[1]};
+            if (s + 1 < s1) issue_stage(s + 1, e_next);
+            const char* const rows = buf(s);
+            const int r0 = s * kWeighRows;
+            f32x16 x[kTiles];
+            if (r0 >= whole && r0 + kWeighRows <= R) {
+                scores(rows, x, late, late_less);
+                scores(rows + 32 * kRowBytes, late, x, less_of(e[0]));
+                late_less = less_of(e[1]);
+                continue;
+            }
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                const int rh = r0 + 32 * h, row = rh + (lane & 31);
+                if (rh >= R || rh + 32 <= first) continue;
+                scores(rows + h * 32 * kRowBytes, x, late, late_less);
+                late_less = -INFINITY;
+                const float less = row < R ? less_of(h ? e[1] : e[0]) : -INFINITY;
+                // Keys of this lane that the row sees.
+                const int lim = p.causal ? min(row, R - 1) / ratio + before + 1 - k0 - 4 * g : INT_MAX;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float w = exp2_hw(fmaf(x[t][r], p.scale_log2, less));
+                        sum[t][r] += 32 * t + 8 * (r >> 2) + (r & 3) < lim ? w : 0.f;
+                    }
+            }
+        }
+        gather(late, late_less);
+        // Over the 32 rows: with every exchange a lane keeps half of its keys, in the end
+        // lane l (and l ^ 16) the one of register l % 16.
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+            for (int b = 3; b >= 0; --b)
+#pragma unroll
+                for (int r = 0; r < 1 << b; ++r) {
+                    const bool up = (lane >> b & 1) != 0;
+                    const float give = up ? sum[t][r] : sum[t][r + (1 << b)];
+                    sum[t][r] = (up ? sum[t][r + (1 << b)] : sum[t][r]) + __shfl_xor(give, 1 << b);
+                }
+            const float total = sum[t][0] + __shfl_xor(sum[t][0], 16);
+            const int at = wave * kWaveKeys + 32 * t + acc_row(lane & 15, lane), key = kb + at, id = page_of(key);
+            if ((lane & 16) != 0) continue;
+            if (it.parts > 1)
+                p.Opart[((size_t)it.slot * p.heads_kv + hk) * kKeys + at] = total;
+            else if (valid(id))
+                p.weights[(((size_t)id * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))] += total;
+        }
+        __syncthreads();  // every wave is done with the stages
     }
+}
+
+// The parts of the blocks that were cut, added up in their order: a thread per key.
+template <int D>
+__global__ __launch_bounds__(WeighCfg<D>::kKeys)
+void kf_kv_weigh_merge_kernel(PagedParams p) {
+    constexpr int kKeys = WeighCfg<D>::kKeys;
+    const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv, sh = p.page_shift;
+    PagedItem it;
+    if (!paged_find<true, false>(p, lane, blockIdx.x / p.heads_kv, it, [&](int i) { return weigh_count<D>(p, i); })) return;
+    const PagedSeq sq = paged_seq(p, it.seq);
+    const int key = it.tile * kKeys + threadIdx.x;
+    if ((unsigned)it.tile * (unsigned)kKeys >= (unsigned)sq.kn || key >= sq.kn) return;
+    const int id = p.block_table[(size_t)it.seq * p.max_pages + (key >> sh)];
+    if ((unsigned)id >= (unsigned)p.num_pages) return;
+    float total = 0.f;
+    for (int k = 0; k < it.parts; ++k)
+        total += p.Opart[((size_t)(it.slot + k) * p.heads_kv + hk) * kKeys + threadIdx.x];
+    p.weights[(((size_t)id * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))] += total;
 }
 
 }  // namespace kf

@@ -311,16 +311,22 @@ struct PagedPlan {
     kf::PagedParams prm;
 };
 
-int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, int max_pages, int num_pages,
-               PagedPlan* pl) {
+int check_paged(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, int max_pages, int num_pages,
+                kf::PagedParams* prm) {
     if (D != 64 && D != 128 && D != 256) return KF_ERR_HEAD_DIM;
     if (const int st = check_heads(H_q, H_kv); st != KF_OK) return st;
     if (n_seqs <= 0) return KF_ERR_SIZE;
     if (const int st = check_packed(tokens, H_q, D); st != KF_OK) return st;
-    kf::PagedParams& prm = pl->prm;
-    if (const int st = paged_geometry(page_size, max_pages, num_pages, &prm.page_shift, &prm.kv_len); st != KF_OK)
+    if (const int st = paged_geometry(page_size, max_pages, num_pages, &prm->page_shift, &prm->kv_len); st != KF_OK)
         return st;
-    if (prm.kv_len > kMaxIndex) return KF_ERR_SIZE;
+    return prm->kv_len > kMaxIndex ? KF_ERR_SIZE : KF_OK;
+}
+
+int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, int max_pages, int num_pages,
+               PagedPlan* pl) {
+    kf::PagedParams& prm = pl->prm;
+    if (const int st = check_paged(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages, num_pages, &prm); st != KF_OK)
+        return st;
     const long long rows = (long long)tokens * (H_q / H_kv);
     const double avg = (double)rows / n_seqs;
     pl->rows = D == 256 ? (avg > 32 ? 128 : 32) : avg > 64 ? 128 : avg > 32 ? 64 : 32;
@@ -393,20 +399,62 @@ void set_paged(kf::PagedParams& prm, const void* Q, const int64_t* strides, cons
     set_scales(prm, D);
 }
 
-template <bool kBF>
-int launch_weigh(const kf::PagedParams& prm, int D, hipStream_t stream) {
-    const long long blocks = ((long long)prm.kv_len + kf::kWeighKeys - 1) / kf::kWeighKeys;
-    if (!fits_grid(blocks * prm.n_seqs, kf::kWeighThreads) ||
-        !fits_grid(blocks * prm.n_seqs * prm.heads_kv, kf::kWeighThreads))
+// ---- Gathered weights. ----
+
+struct WeighPlan {
+    long long cut_blocks;                 // at most, of a KV head
+    size_t ws_bytes;
+    kf::PagedParams prm;
+};
+
+int weigh_keys(int D) { return D == 256 ? kf::WeighCfg<256>::kKeys : kf::WeighCfg<128>::kKeys; }
+
+int weigh_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, int max_pages, int num_pages,
+               WeighPlan* pl) {
+    kf::PagedParams& prm = pl->prm;
+    if (const int st = check_paged(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages, num_pages, &prm); st != KF_OK)
+        return st;
+    const int keys = weigh_keys(D);
+    const long long blocks = ((long long)prm.kv_len + keys - 1) / keys;  // of a sequence, at most
+    if (blocks * n_seqs > kMaxIndex) return KF_ERR_SIZE;
+    const long long rows = (long long)tokens * (H_q / H_kv), cus = current_device_shape().cus;
+    const long long stages = rows / kf::kWeighRows + std::min(n_seqs, tokens);
+    // Blocks of keys are cut along the rows where these are many.
+    const int wanted = std::max(1, (int)(8 * cus / H_kv));
+    prm.target = rows / n_seqs < 8 * kf::kWeighRows ? 0 : wanted;
+    prm.unit_shift = 0;
+    while (blocks * ((stages >> prm.unit_shift) + n_seqs) > INT_MAX && prm.unit_shift < 30) ++prm.unit_shift;
+    if (blocks * ((stages >> prm.unit_shift) + n_seqs) > INT_MAX) prm.target = 0;
+    prm.min_share = std::max(1, 4 >> prm.unit_shift);
+    // Workgroups for all blocks that the tables could hold, up to many rounds of the device.
+    prm.stride = (int)std::min<long long>(blocks * n_seqs + prm.target, std::max<long long>(1, 32 * cus / H_kv));
+    pl->cut_blocks = std::min<long long>(blocks * n_seqs, prm.target);
+    pl->ws_bytes = align_up((size_t)2 * prm.target * H_kv * keys * sizeof(float), kWsAlign);
+    if (!fits_grid((long long)prm.stride * H_kv, kf::kWeighThreads) ||
+        !fits_grid(pl->cut_blocks * H_kv, keys))
         return KF_ERR_SIZE;
-    const dim3 grid((unsigned)(blocks * prm.n_seqs * prm.heads_kv)), block(kf::kWeighThreads);
+    return KF_OK;
+}
+
+template <bool kBF, int D>
+int launch_weigh(const WeighPlan& pl, hipStream_t stream) {
+    const kf::PagedParams& prm = pl.prm;
     (void)hipGetLastError();
-    switch (D) {
-        case 64: kf::kf_kv_weigh_kernel<kBF, 64><<<grid, block, 0, stream>>>(prm); break;
-        case 128: kf::kf_kv_weigh_kernel<kBF, 128><<<grid, block, 0, stream>>>(prm); break;
-        default: kf::kf_kv_weigh_kernel<kBF, 256><<<grid, block, 0, stream>>>(prm);
-    }
+    kf::kf_kv_weigh_kernel<kBF, D>
+        <<<dim3((unsigned)((long long)prm.stride * prm.heads_kv)), dim3(kf::kWeighThreads), 0, stream>>>(prm);
+    if (const int st = launched(); st != KF_OK || prm.target == 0) return st;
+    kf::kf_kv_weigh_merge_kernel<D>
+        <<<dim3((unsigned)(pl.cut_blocks * prm.heads_kv)), dim3(kf::WeighCfg<D>::kKeys), 0, stream>>>(prm);
     return launched();
+}
+
+template <bool kBF>
+int launch_weigh_dim(const WeighPlan& pl, int D, hipStream_t stream) {
+    switch (D) {
+        case 64: return launch_weigh<kBF, 64>(pl, stream);
+        case 128: return launch_weigh<kBF, 128>(pl, stream);
+        default: return launch_weigh<kBF, 256>(pl, stream);
+    }
 }
 
 // ---- The 16-bit cache: new tokens, eviction. ----
@@ -729,11 +777,18 @@ int kf_attn_paged(const void* Q, const int64_t* strides, const void* K_pages, co
     return (flags & KF_BF16) ? launch_paged_dim<true>(pl, D, s) : launch_paged_dim<false>(pl, D, s);
 }
 
+size_t kf_kv_weigh_workspace_bytes(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size,
+                                   int max_pages_per_seq) {
+    WeighPlan pl{};
+    return weigh_plan(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq, 1, &pl) == KF_OK ? pl.ws_bytes : 0;
+}
+
 int kf_kv_weigh(const void* Q, const int64_t* strides, const void* K_pages, float* weights, const int* block_table,
                 const int* seq_starts, const int* kv_lens, const float* lse, int n_seqs, int tokens, int H_q, int H_kv,
-                int D, int page_size, int max_pages_per_seq, int num_pages, int flags, void* stream) {
-    PagedPlan pl{};
-    if (const int st = paged_plan(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq, num_pages, &pl);
+                int D, int page_size, int max_pages_per_seq, int num_pages, int flags, void* workspace,
+                size_t workspace_bytes, void* stream) {
+    WeighPlan pl{};
+    if (const int st = weigh_plan(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq, num_pages, &pl);
         st != KF_OK)
         return st;
     if ((flags & ~(KF_ATTN_CAUSAL | KF_BF16)) != 0) return KF_ERR_FLAGS;
@@ -743,12 +798,17 @@ int kf_kv_weigh(const void* Q, const int64_t* strides, const void* K_pages, floa
         return KF_ERR_ALIGN;
     if (strides)
         if (const int st = check_strides(strides, 2); st != KF_OK) return st;
+    if (pl.ws_bytes > 0) {
+        if (!workspace || workspace_bytes < pl.ws_bytes) return KF_ERR_WORKSPACE;
+        if ((reinterpret_cast<uintptr_t>(workspace) & (kWsAlign - 1)) != 0) return KF_ERR_ALIGN;
+    }
     set_paged(pl.prm, Q, strides, K_pages, block_table, seq_starts, kv_lens, n_seqs, tokens, H_q, H_kv, D,
               max_pages_per_seq, num_pages, flags);
     pl.prm.row_lse = lse;
     pl.prm.weights = weights;
+    pl.prm.Opart = static_cast<float*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return (flags & KF_BF16) ? launch_weigh<true>(pl.prm, D, s) : launch_weigh<false>(pl.prm, D, s);
+    return (flags & KF_BF16) ? launch_weigh_dim<true>(pl, D, s) : launch_weigh_dim<false>(pl, D, s);
 }
 
 size_t kf_kv_evict_workspace_bytes(int n_seqs, int H_kv, int D, int page_size, int max_pages_per_seq) {

@@ -502,6 +502,12 @@ def paged_attn_workspace_bytes(n_seqs, tokens, H_q, H_kv, D, page_size, max_page
                                                             max_pages_per_seq))
 
 
+def weigh_workspace_bytes(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages_per_seq) -> int:
+    """Workspace of kv_weigh (kf_kv_weigh_workspace_bytes)."""
+    return int(load_library().kf_kv_weigh_workspace_bytes(n_seqs, tokens, H_q, H_kv, D, page_size,
+                                                          max_pages_per_seq))
+
+
 def evict_workspace_bytes(n_seqs, H_kv, D, page_size, max_pages_per_seq) -> int:
     """Workspace of kv_evict (kf_kv_evict_workspace_bytes)."""
     return int(load_library().kf_kv_evict_workspace_bytes(n_seqs, H_kv, D, page_size, max_pages_per_seq))
@@ -572,13 +578,15 @@ def attn_paged(Q, K_pages, V_pages, block_table, seq_starts, kv_lens, out=None, 
     return (out, lse) if return_lse else out
 
 
-def kv_weigh(Q, K_pages, weights, block_table, seq_starts, kv_lens, lse, *, causal=False, stream=None):
+def kv_weigh(Q, K_pages, weights, block_table, seq_starts, kv_lens, lse, *, causal=False, workspace=None,
+             stream=None):
     """Add the attention weight that keys of a paged 16-bit cache get from new tokens.
 
     weights[j] (float32 [num_pages, H_kv, page_size], by the pages of the keys) += the sum of
     exp(q . k_j / sqrt(D) - lse) over the tokens that see key j and the query heads of
     its KV head.  ``lse`` float32 [T, H_q] as attn_paged returns it (a row of -inf adds
     nothing), the other arguments as attn_paged's.  Sequences must not share pages.
+    ``workspace``: a buffer of weigh_workspace_bytes to use instead of a new one.
     """
     import torch
 
@@ -596,11 +604,14 @@ def kv_weigh(Q, K_pages, weights, block_table, seq_starts, kv_lens, lse, *, caus
         raise _too_many()
     if lse.dtype is not torch.float32 or lse.shape != (T, H_q) or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous float32 [T, H_q] tensor")
+    need = _need(weigh_workspace_bytes, device.index, n, T, H_q, H_kv, D, page_size, max_pages)
+    workspace = _workspace_at(torch, workspace, need, Q, stream)
     if causal:
         flags |= KF_ATTN_CAUSAL
     _launch(torch, device, stream, load_library().kf_kv_weigh,
             Q.data_ptr(), strides, K_pages.data_ptr(), _weights(torch, weights, pools), table, starts, lens,
-            lse.data_ptr(), n, T, H_q, H_kv, D, page_size, max_pages, num_pages, flags)
+            lse.data_ptr(), n, T, H_q, H_kv, D, page_size, max_pages, num_pages, flags,
+            workspace.data_ptr() if workspace is not None else None, need)
 
 
 def kv_evict(K_pages, V_pages, weights, block_table, kv_lens, budgets, out=None, *, recent=0, workspace=None,

@@ -26,8 +26,9 @@ def attend(lib, Q=FAKE, strides=None, Kp=FAKE, Vp=FAKE, table=FAKE, starts=FAKE,
 
 
 def weigh(lib, Q=FAKE, strides=None, Kp=FAKE, w=FAKE, table=FAKE, starts=FAKE, lens=FAKE, lse=FAKE, n=2, T=4, H_q=8,  # noqa: F811
-          H_kv=2, D=128, ps=16, mp=4, np_=8, flags=0):
-    return lib.kf_kv_weigh(Q, _strides(strides), Kp, w, table, starts, lens, lse, n, T, H_q, H_kv, D, ps, mp, np_, flags, None)
+          H_kv=2, D=128, ps=16, mp=4, np_=8, flags=0, ws=FAKE, ws_bytes=1 << 50):
+    return lib.kf_kv_weigh(Q, _strides(strides), Kp, w, table, starts, lens, lse, n, T, H_q, H_kv, D, ps, mp, np_, flags, ws,
+                           ws_bytes, None)
 
 
 def evict(lib, Kp=FAKE, Vp=FAKE, w=FAKE, table=FAKE, lens=FAKE, budgets=FAKE, kept=FAKE, n=2, H_kv=2, D=128, ps=16,  # noqa: F811
@@ -122,6 +123,11 @@ def test_workspaces(lib):  # noqa: F811
     # Tiles enough for the device, or few keys: none is cut.
     assert kf.paged_attn_workspace_bytes(8, 1 << 15, 32, 8, 128, 16, 1024) == 0
     assert kf.paged_attn_workspace_bytes(8, 8, 32, 8, 128, 16, 4) == 0
+    need = kf.weigh_workspace_bytes(1, 2048, 32, 8, 128, 16, 256)
+    assert need > 0 and need % 256 == 0 and kf.weigh_workspace_bytes(64, 64, 32, 8, 128, 16, 256) == 0
+    many = dict(n=1, T=2048, H_q=32, H_kv=8, mp=256)
+    assert weigh(lib, ws=None, **many) == weigh(lib, ws_bytes=need - 1, **many) == kf.KF_ERR_WORKSPACE
+    assert weigh(lib, ws=FAKE + 16, **many) == kf.KF_ERR_ALIGN
     need = kf.evict_workspace_bytes(2, 2, 128, 16, 4)
     assert need == 256 + 256 + 2 * 2 * 64 * 4
     assert evict(lib, ws=None) == evict(lib, ws_bytes=need - 1) == kf.KF_ERR_WORKSPACE
@@ -163,7 +169,7 @@ def test_no_kernel_uses_scratch(tmp_path):
     mine = {n: v for n, v in found.items() if re.search("kf_attn_paged|kf_kv_append|kf_kv_weigh|kf_kv_evict", n)}
     assert {re.search(r"kf_[a-z0-9_]+?_kernel", n).group(0) for n in mine} >= {
         "kf_attn_paged_kernel", "kf_attn_paged_merge_kernel", "kf_kv_append_kernel", "kf_kv_weigh_kernel",
-        "kf_kv_evict_select_kernel", "kf_kv_evict_move_kernel"}
+        "kf_kv_weigh_merge_kernel", "kf_kv_evict_select_kernel", "kf_kv_evict_move_kernel"}
     assert not {n: v for n, v in mine.items() if v != (0, 0)}
 
 
@@ -193,8 +199,13 @@ int kf_attn_paged(const void* Q, const int64_t* s, const void* Kp, const void* V
     ws_bytes = have;
     return take(P(Q), P(s), P(Kp), P(Vp), P(t), P(b), P(l), P(O), P(m), P(u), n, T, hq, hk, D, ps, mp, np, f, P(st));
 }
+size_t kf_kv_weigh_workspace_bytes(int, int, int, int, int, int, int) { return need; }
 int kf_kv_weigh(const void* Q, const int64_t* s, const void* Kp, float* w, const int* t, const int* b, const int* l,
-                const float* e, int n, int T, int hq, int hk, int D, int ps, int mp, int np, int f, void* st) {
+                const float* e, int n, int T, int hq, int hk, int D, int ps, int mp, int np, int f, void* ws, size_t have,
+                void* st) {
+    if (need && (!ws || have < need)) return KF_ERR_WORKSPACE;
+    ws_seen = ws;
+    ws_bytes = have;
     return take(P(Q), P(s), P(Kp), P(w), P(t), P(b), P(l), P(e), n, T, hq, hk, D, ps, mp, np, f, P(st));
 }
 size_t kf_kv_evict_workspace_bytes(int, int, int, int, int) { return need; }
@@ -218,9 +229,10 @@ int main() {
     REQUIRE(kf::kv_append(p<H>(1), p<H>(2), p<int64_t>(3), p<H>(4), p<H>(5), p<float>(6), p<int>(7), p<int>(8), p<int>(9), 10,
                           11, 12, 13, 14, 15, 16, 17, s1) == hipSuccess);
     REQUIRE(run(0, 16, 1) && seen[17] == 901 && count == 18);
-    REQUIRE(kf::kv_weigh(p<H>(1), p<int64_t>(2), p<H>(3), p<float>(4), p<int>(5), p<int>(6), p<int>(7), p<float>(8), 9, 10, 11,
-                         12, 13, 14, 15, 16, 17, s1) == hipSuccess);
-    REQUIRE(run(0, 16, 1) && seen[17] == 901 && count == 18);
+    auto weigh = [&](hipStream_t s) {
+        return kf::kv_weigh(p<H>(1), p<int64_t>(2), p<H>(3), p<float>(4), p<int>(5), p<int>(6), p<int>(7), p<float>(8), 9, 10, 11,
+                            12, 13, 14, 15, 16, 17, s);
+    };
     auto attend = [&](hipStream_t s) {
         return kf::attn_paged(p<H>(1), p<int64_t>(2), p<H>(3), p<H>(4), p<int>(5), p<int>(6), p<int>(7), p<void>(8), 11, 12, 13,
                               14, 15, 16, 17, 18, 19, s, p<float>(9), p<float>(10));
@@ -231,10 +243,12 @@ int main() {
     // During a capture no workspace can be had: refused, nothing allocated.
     g_capturing = true;
     REQUIRE(attend(s1) == hipErrorStreamCaptureUnsupported && evict(s1) == hipErrorStreamCaptureUnsupported && g_mallocs == 0);
+    REQUIRE(weigh(s1) == hipErrorStreamCaptureUnsupported && g_mallocs == 0);
     g_capturing = false;
     REQUIRE(attend(s1) == hipSuccess && run(0, 18, 1) && seen[19] == 901 && g_mallocs == 1 && ws_bytes >= need);
     void* first = ws_seen;
     REQUIRE(evict(s1) == hipSuccess && run(0, 13, 1) && seen[14] == 901 && ws_seen == first && g_mallocs == 1);
+    REQUIRE(weigh(s1) == hipSuccess && run(0, 16, 1) && seen[17] == 901 && count == 18 && ws_seen == first && g_mallocs == 1);
     REQUIRE(evict(s2) == hipSuccess && ws_seen != first && g_mallocs == 2);     // streams share none
     g_capturing = true;
     REQUIRE(attend(s1) == hipSuccess && ws_seen == first);                      // captured with what there is
@@ -244,6 +258,7 @@ int main() {
     for (int i = 0; i < g_frees; ++i) REQUIRE(g_freed[i] != first);             // a graph holds it
     need = 0;                                                                   // a call that is not cut
     REQUIRE(attend(p<S>(903)) == hipSuccess && ws_seen == nullptr);
+    REQUIRE(weigh(p<S>(903)) == hipSuccess && ws_seen == nullptr);
     status = KF_ERR_SIZE;
     REQUIRE(kf::kv_append(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0, 0, 0, 0, 0,
                           s1) == hipErrorInvalidValue);
