@@ -22,7 +22,7 @@ struct PagedParams : AttnParams {  // Q, K, V, O, Mi (LSE), scales, causal, head
     int target, min_share, unit_shift;
     const float* row_lse;          // kf_kv_weigh: [tokens_q][H_q]
     float* weights;                // kf_kv_weigh: [num_pages][H_kv][page_size]
-    int stride;                    // kf_kv_weigh: workgroups of a KV head
+    int cut;                       // kf_kv_weigh: blocks of keys may be cut
 };
 
 // One sequence's new tokens and keys.
@@ -482,58 +482,151 @@ void kf_attn_paged_merge_kernel(PagedParams p) {
 // stages of 64 that the workgroup's waves share; lane l has row l % 32 of 16 keys a
 // product, and adds their weights up in registers.  At the end the lanes' sums of a
 // key are added, and the one wave that has the key adds them to its weight: no
-// atomics, always the same order.  Blocks of keys with many rows may be cut along the
-// rows (paged_find); the parts' sums then go through the workspace.
+// atomics, always the same order.
 //
 // A sequence of up to 32 rows, a step's, is read once from the pages: there the wave
 // holds the rows, and its keys go by through LDS stages of its own (weigh_step).
+//
+// The work of a KV head is a line of units, 64 rows that meet a block of keys or a
+// run of a step's keys, of which every workgroup has an equal share.  Where a block's
+// units lie in several shares, their sums go through the workspace and a second kernel.
 // ---------------------------------------------------------------------------
-constexpr int kWeighThreads = 256;
 constexpr int kWeighRows = 64;                                      // query rows of a stage
 template <int D> struct WeighCfg {
+    static constexpr int kThreads = 256, kWaves = kThreads / 64;
     // 32-key tiles of a wave: two of 256 channels would not fit its registers.
     static constexpr int kTiles = D == 256 ? 1 : 2;
     static constexpr int kWaveKeys = 32 * kTiles;
-    static constexpr int kKeys = kWaveKeys * kWeighThreads / 64;    // of a workgroup: a block
+    static constexpr int kKeys = kWaveKeys * kWaves;                // of a block
     static constexpr int kWavesPerSimd = 2;
-    // Steps: 32-key tiles of a wave, channels of a stage, and the stages of a ring.
-    static constexpr int kStepTiles = 4, kStepKeys = kStepTiles * 32 * kWeighThreads / 64;
+    // Steps: a run has a tile of 32 keys for every wave, and counts as much as so many
+    // units; channels of an LDS stage and the stages of a wave; tiles whose sums wait
+    // in LDS.
+    static constexpr int kStepKeys = 32 * kWaves, kStepUnits = 2;
     static constexpr int kStepWidth = D < 128 ? D : 128, kRing = D == 64 ? 4 : 2;
-    static constexpr int kStepStage = 32 * kStepWidth * 2;
-    static constexpr int kRowsBytes = 2 * kWeighRows * 2 * D, kRingBytes = kWeighThreads / 64 * kRing * kStepStage;
+    static constexpr int kStepStage = 32 * kStepWidth * 2, kStepSums = 16;
+    static constexpr int kRowsBytes = 2 * kWeighRows * 2 * D, kRingBytes = kWaves * kRing * kStepStage;
     static constexpr int kLds = kRowsBytes > kRingBytes ? kRowsBytes : kRingBytes;
 };
 
-// Tiles are blocks of keys, units 64 << unit_shift query rows.
-template <int D>
-__device__ __forceinline__ PagedCount weigh_count(const PagedParams& p, int i) {
-    using Cfg = WeighCfg<D>;
-    const PagedSeq s = paged_seq(p, i);
-    const long long rows = (long long)s.qn * p.ratio;
-    const int stages = (int)((rows + kWeighRows - 1) / kWeighRows), keys = rows <= 32 ? Cfg::kStepKeys : Cfg::kKeys;
-    return PagedCount{stages > 0 ? (s.kn + keys - 1) / keys : 0, (stages + (1 << p.unit_shift) - 1) >> p.unit_shift};
+// The blocks of one sequence's keys.  Causal: query i sees keys j <= i + before, and the rows in
+// front of the first that sees any of a block's have no units there.
+template <int D> struct WeighSeq {
+    int q0, qn, kn, rows, stages;
+    bool step;
+    __device__ __forceinline__ WeighSeq(const PagedParams& p, int i) {
+        const PagedSeq s = paged_seq(p, i);
+        q0 = s.q0, qn = s.qn, kn = s.kn;
+        rows = qn * p.ratio;
+        stages = (int)(((unsigned)rows + kWeighRows - 1) / kWeighRows);
+        step = rows <= 32;
+    }
+    __device__ __forceinline__ int before() const { return kn - qn; }
+    __device__ __forceinline__ int tiles() const {
+        const int keys = step ? WeighCfg<D>::kStepKeys : WeighCfg<D>::kKeys;
+        return rows == 0 ? 0 : (kn + keys - 1) / keys;
+    }
+    // The first stage of block t, and the units of the t blocks in front of it.
+    __device__ __forceinline__ int first(const PagedParams& p, int t) const {
+        return !p.causal || step ? 0 : (int)((long long)max(t * WeighCfg<D>::kKeys - before(), 0) * p.ratio / kWeighRows);
+    }
+    __device__ __forceinline__ long long units(const PagedParams& p, int t) const {
+        if (step) return (long long)t * WeighCfg<D>::kStepUnits;
+        long long u = (long long)t * stages;
+        // From block t0 on first() is m t - c: a block has a whole number m of stages' rows.
+        const int t0 = before() < 0 ? 0 : before() / WeighCfg<D>::kKeys + 1;
+        if (p.causal && t > t0) {
+            const long long m = WeighCfg<D>::kKeys / kWeighRows * p.ratio, b = (long long)before() * p.ratio;
+            const long long c = b >= 0 ? (b + kWeighRows - 1) / kWeighRows : -(-b / kWeighRows);
+            u -= m * (((long long)t * (t - 1) - (long long)t0 * (t0 - 1)) / 2) - c * (t - t0);
+        }
+        return u;
+    }
+    __device__ __forceinline__ long long units(const PagedParams& p) const { return units(p, tiles()); }
+    // The block of unit u.
+    __device__ __forceinline__ int tile_of(const PagedParams& p, long long u) const {
+        int lo = 0, hi = tiles();   // units(lo) <= u < units(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (units(p, mid) <= u) lo = mid; else hi = mid;
+        }
+        return lo;
+    }
+};
+
+__device__ __forceinline__ long long weigh_scan(long long v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+__device__ __forceinline__ long long weigh_lane(long long v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (long long)((uint64_t)hi << 32 | lo);
 }
 
-// A block of a sequence of R <= 32 rows.  S = Q K^T: lane l has key l % 32 and 16 of the
+// Share j of a KV head's units: from unit u0 of the line on, `share` of them but for the last;
+// the sequence of the first, and its place among the sequence's units.  By the lanes
+// of a wave; false past the last unit.
+struct WeighShare {
+    long long u0, u1, share, at;
+    int seq;
+};
+template <int D>
+__device__ __forceinline__ bool weigh_find(const PagedParams& p, int lane, int j, WeighShare& w) {
+    const int per = (p.n_seqs + 63) / 64, first = min(lane * per, p.n_seqs), last = min(first + per, p.n_seqs);
+    long long mine = 0;
+    for (int i = first; i < last; ++i) mine += WeighSeq<D>(p, i).units(p);
+    long long inc = weigh_scan(mine, lane);
+    const long long total = weigh_lane(inc, 63);
+    w.share = max((total + p.target - 1) / p.target, (long long)p.min_share);
+    w.u0 = j * w.share;
+    w.u1 = min(w.u0 + w.share, total);
+    if (w.u0 >= total) return false;
+    const int run = __builtin_ctzll(__ballot(inc > w.u0));
+    w.at = w.u0 - (weigh_lane(inc, run) - weigh_lane(mine, run));
+    w.seq = run;
+    if (per == 1) return true;
+    const int end = min((run + 1) * per, p.n_seqs);
+    for (int i0 = run * per; i0 < end; i0 += 64) {
+        mine = i0 + lane < end ? WeighSeq<D>(p, i0 + lane).units(p) : 0;
+        inc = weigh_scan(mine, lane);
+        const uint64_t over = __ballot(inc > w.at);
+        if (over != 0) {
+            const int at = __builtin_ctzll(over);
+            w.seq = i0 + at;
+            w.at -= weigh_lane(inc, at) - weigh_lane(mine, at);
+            return true;
+        }
+        w.at -= weigh_lane(inc, 63);
+    }
+    return false;  // not reached
+}
+
+// Runs r0 .. r1 - 1 of a step's keys.  S = Q K^T: lane l has key l % 32 and 16 of the
 // rows, the sum over which needs one exchange; of fewer rows only those groups of eight
 // that there are have exponentials.  Every wave copies its own stages, 32 keys or half of
 // their 256 channels, and waits for itself alone.
 template <bool kBF, int D>
-__device__ __forceinline__ void weigh_step(const PagedParams& p, const PagedSeq& sq, int seq, int kb, int hk, int wave,
-                                           int lane, char* lds) {
+__device__ __forceinline__ void weigh_step(const PagedParams& p, const WeighSeq<D>& sq, int seq, int r0, int r1, int hk,
+                                           int wave, int lane, char* lds, float* sums) {
     using Cfg = WeighCfg<D>;
     using E = Elem<kBF>;
     using X8 = typename E::x8;
     constexpr int W = Cfg::kStepWidth, kChunks = W / 8, kRowBytes = 2 * W, kRowsPerInstr = 1024 / kRowBytes;
     using SW = SwizzleRow<W>;
     constexpr int kNKK = D / 16, kStageKK = W / 16, kHalves = D / W, kHalfInstr = 16 / kRowsPerInstr;
-    const int g = lane >> 5, sh = p.page_shift, ratio = p.ratio, R = sq.qn * ratio;
-    const int k0 = kb + wave * (32 * Cfg::kStepTiles), keys = sq.kn - k0;
-    if (keys <= 0) return;
-    const int ntiles = min((keys + 31) / 32, Cfg::kStepTiles), nst = ntiles * kHalves;
-    // The ids of the wave's pages, one to a lane: no more than 9.
-    const int page0 = k0 >> sh;
-    const int ids = p.block_table[(size_t)seq * p.max_pages + min(page0 + lane, (sq.kn - 1) >> sh)];
+    const int g = lane >> 5, sh = p.page_shift, ratio = p.ratio, R = sq.rows;
+    // Tile t of the wave begins at key k0 + t kStepKeys.
+    const int k0 = r0 * Cfg::kStepKeys + wave * 32, left = min(r1 * Cfg::kStepKeys, sq.kn) - k0;
+    if (left <= 0) return;
+    const int ntiles = (left + Cfg::kStepKeys - 1) / Cfg::kStepKeys, nst = ntiles * kHalves;
+    // The ids of 64 pages from page0 on, one to a lane; stages come in order.
+    const int* const table = p.block_table + (size_t)seq * p.max_pages;
+    const int last_page = (sq.kn - 1) >> sh;
+    int page0 = k0 >> sh, ids = table[min(page0 + lane, last_page)];
     const int lr = lane / kChunks;
     uint32_t lane_off[kHalfInstr];
 #pragma unroll
@@ -547,8 +640,15 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const PagedSeq&
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             // (Rows behind the keys lie in their page still, or are those of page 0.)
-            const int key = k0 + s / kHalves * 32 + 16 * h;
-            const int id = key < sq.kn ? __builtin_amdgcn_readlane(ids, (key >> sh) - page0) : 0;
+            const int key = k0 + s / kHalves * Cfg::kStepKeys + 16 * h;
+            int id = -1;
+            if (key < sq.kn) {
+                if ((key >> sh) - page0 >= 64) {
+                    page0 = key >> sh;
+                    ids = table[min(page0 + lane, last_page)];
+                }
+                id = __builtin_amdgcn_readlane(ids, (key >> sh) - page0);
+            }
             const size_t row = (((size_t)((unsigned)id < (unsigned)p.num_pages ? id : 0) * p.heads_kv + hk) << sh) +
                                (key & ((1 << sh) - 1));
             const char* const src = reinterpret_cast<const char*>(p.K) + row * (2 * D) + s % kHalves * kRowBytes;
@@ -558,7 +658,7 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const PagedSeq&
         }
     };
     // The rows, those past the last as the last, and what their exponents are less by: those and
-    // rows without a key add nothing.  Loads in front of the stages', which are counted.
+    // rows without a key add nothing.
     X8 q[kNKK];
     const int row = min(lane & 31, R - 1);
     {
@@ -567,146 +667,161 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const PagedSeq&
         for (int kk = 0; kk < kNKK; ++kk) q[kk] = *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8);
     }
     const float e = p.row_lse[((size_t)(sq.q0 + row / ratio) * p.heads_kv + hk) * ratio + row % ratio];
-    // This lane's key of every tile: its weight.
-    float* to[Cfg::kStepTiles];
-    float sum[Cfg::kStepTiles];
 #pragma unroll
-    for (int t = 0; t < Cfg::kStepTiles; ++t) {
-        const int key = k0 + 32 * t + (lane & 31);
-        const int id = __shfl(ids, min((key >> sh) - page0, 63));
-        to[t] = key < sq.kn && (unsigned)id < (unsigned)p.num_pages
-                    ? p.weights + (((size_t)id * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1)) : nullptr;
-        sum[t] = to[t] && g == 0 ? *to[t] : 0.f;
-    }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-    asm volatile("" ::: "memory");
+    for (int s = 0; s < Cfg::kRing - 1; ++s)
+        if (s < nst) issue(s);
     const float less_row = (lane & 31) < R && e > -INFINITY ? -e * kLog2e : -INFINITY;
     float less[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) less[r] = __shfl(less_row, 8 * (r >> 2) + (r & 3) + 4 * g);
-    const int before = sq.kn - sq.qn;
-#pragma unroll
-    for (int s = 0; s < Cfg::kRing - 1; ++s)
-        if (s < nst) issue(s);
+    const int before = sq.before();
     int koff[kStageKK];
 #pragma unroll
     for (int kk = 0; kk < kStageKK; ++kk) {
         const int r = lane & 31;
         koff[kk] = r * kRowBytes + (((2 * kk + g) ^ SW::h(r)) % kChunks) * 16;
     }
+    for (int t0 = 0; t0 < ntiles; t0 += Cfg::kStepSums) {
+        const int n = min(Cfg::kStepSums, ntiles - t0);
+        for (int t = t0; t < t0 + n; ++t) {
+            f32x16 x = {};
 #pragma unroll
-    for (int t = 0; t < Cfg::kStepTiles; ++t) {
-        if (t >= ntiles) break;
-        f32x16 x = {};
-#pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf) {
-            const int s = t * kHalves + hf;
-            if (s + Cfg::kRing - 1 < nst) {
+            for (int hf = 0; hf < kHalves; ++hf) {
+                const int s = t * kHalves + hf;
+                if (s + Cfg::kRing - 1 < nst) {
+                    asm volatile("" ::: "memory");
+                    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage there has been read
+                    issue(s + Cfg::kRing - 1);
+                }
+                // This stage has landed where no more than the later ones' copies are on their way.
+                const int ahead = min(Cfg::kRing - 1, nst - 1 - s);
                 asm volatile("" ::: "memory");
-                __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage there has been read
-                issue(s + Cfg::kRing - 1);
+                if (ahead >= 3) __builtin_amdgcn_s_waitcnt(0x0f70 | (6 * kHalfInstr & 15) | (6 * kHalfInstr >> 4) << 14);
+                else if (ahead == 2) __builtin_amdgcn_s_waitcnt(0x0f70 | (4 * kHalfInstr & 15) | (4 * kHalfInstr >> 4) << 14);
+                else if (ahead == 1) __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * kHalfInstr & 15) | (2 * kHalfInstr >> 4) << 14);
+                else __builtin_amdgcn_s_waitcnt(0x0f70);
+                asm volatile("" ::: "memory");
+                const char* const stage = ring + s % Cfg::kRing * Cfg::kStepStage;
+#pragma unroll
+                for (int kk = 0; kk < kStageKK; ++kk)
+                    x = E::mfma32(q[hf * kStageKK + kk], *reinterpret_cast<const X8*>(stage + koff[kk]), x);
             }
-            // This stage has landed where no more than the later ones' copies are on their way.
-            const int ahead = min(Cfg::kRing - 1, nst - 1 - s);
-            asm volatile("" ::: "memory");
-            if (ahead >= 3) __builtin_amdgcn_s_waitcnt(0x0f70 | (6 * kHalfInstr & 15) | (6 * kHalfInstr >> 4) << 14);
-            else if (ahead == 2) __builtin_amdgcn_s_waitcnt(0x0f70 | (4 * kHalfInstr & 15) | (4 * kHalfInstr >> 4) << 14);
-            else if (ahead == 1) __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * kHalfInstr & 15) | (2 * kHalfInstr >> 4) << 14);
-            else __builtin_amdgcn_s_waitcnt(0x0f70);
-            asm volatile("" ::: "memory");
-            const char* const stage = ring + s % Cfg::kRing * Cfg::kStepStage;
+            // Where row 0 does not see the last key of the tile rows have limits.
+            const int kt = k0 + t * Cfg::kStepKeys, key = kt + (lane & 31);
+            const bool whole = !p.causal || kt + 32 <= before + 1;
+            float add = 0.f;
 #pragma unroll
-            for (int kk = 0; kk < kStageKK; ++kk)
-                x = E::mfma32(q[hf * kStageKK + kk], *reinterpret_cast<const X8*>(stage + koff[kk]), x);
-        }
-        // The last key of the tile that row 0 sees too: from there on rows have limits.
-        const int key = k0 + 32 * t + (lane & 31);
-        const bool whole = !p.causal || k0 + 32 * t + 32 <= before + 1;
-        float add = 0.f;
+            for (int b = 0; b < 4; ++b) {
+                if (8 * b >= R) break;
+                float w[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            if (8 * b >= R) break;
-            float w[4];
+                for (int i = 0; i < 4; ++i) w[i] = exp2_hw(fmaf(x[4 * b + i], p.scale_log2, less[4 * b + i]));
+                if (!whole) {
+                    asm volatile("" ::: "memory");       // a branch, not selects in every tile
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = exp2_hw(fmaf(x[4 * b + i], p.scale_log2, less[4 * b + i]));
-            if (!whole) {
-                asm volatile("" ::: "memory");       // a branch, not selects in every tile
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (key > before + (8 * b + 4 * g + i) / ratio) w[i] = 0.f;
+                    for (int i = 0; i < 4; ++i)
+                        if (key > before + (8 * b + 4 * g + i) / ratio) w[i] = 0.f;
+                }
+                add += (w[0] + w[1]) + (w[2] + w[3]);
             }
-            add += (w[0] + w[1]) + (w[2] + w[3]);
+            add += __shfl_xor(add, 32);
+            if (g == 0) sums[(t - t0) * 32 + lane] = add;
         }
-        sum[t] += add + __shfl_xor(add, 32);
+        // The wave's own sums, two tiles at a time.
+        for (int t = t0 + g; t < t0 + n; t += 2) {
+            const int key = k0 + t * Cfg::kStepKeys + (lane & 31);
+            const int id = key < sq.kn ? table[key >> sh] : -1;
+            if ((unsigned)id < (unsigned)p.num_pages)
+                p.weights[(((size_t)id * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))] += sums[(t - t0) * 32 + (lane & 31)];
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): later waits count copies alone
+        asm volatile("" ::: "memory");
     }
-#pragma unroll
-    for (int t = 0; t < Cfg::kStepTiles; ++t)
-        if (to[t] && g == 0) *to[t] = sum[t];
 }
 
 template <bool kBF, int D>
-__global__ __launch_bounds__(kWeighThreads, WeighCfg<D>::kWavesPerSimd)
+__global__ __launch_bounds__(WeighCfg<D>::kThreads, WeighCfg<D>::kWavesPerSimd)
 void kf_kv_weigh_kernel(PagedParams p) {
+    using Cfg = WeighCfg<D>;
     using E = Elem<kBF>;
     using X8 = typename E::x8;
     using SW = SwizzleRow<D>;
     constexpr int kNKK = D / 16, kChunks = D / 8, kRowBytes = 2 * D, kRowsPerInstr = 1024 / kRowBytes;
-    constexpr int kWaves = kWeighThreads / 64, kInstr = kWeighRows / kRowsPerInstr / kWaves;  // of a wave and stage
-    constexpr int kTiles = WeighCfg<D>::kTiles, kWaveKeys = WeighCfg<D>::kWaveKeys, kKeys = WeighCfg<D>::kKeys;
+    constexpr int kWaves = Cfg::kWaves, kInstr = kWeighRows / kRowsPerInstr / kWaves;  // of a wave and stage
+    constexpr int kTiles = Cfg::kTiles, kWaveKeys = Cfg::kWaveKeys, kKeys = Cfg::kKeys;
     constexpr bool kXorOff = D >= 128;
-    __shared__ __attribute__((aligned(1024))) char lds[WeighCfg<D>::kLds];
+    __shared__ __attribute__((aligned(1024))) char lds[Cfg::kLds];
+    __shared__ float step_sums[kWaves][Cfg::kStepSums * 32];
+    __shared__ uint32_t off[kInstr][Cfg::kThreads];       // this thread's offsets of a whole stage
     const auto buf = [&](int s) { return lds + (s & 1) * (kWeighRows * kRowBytes); };
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hk = blockIdx.x % p.heads_kv, sh = p.page_shift, ratio = p.ratio;
-    for (int j = blockIdx.x / p.heads_kv;; j += p.stride) {
-        // (An opaque lane: nothing that is derived from it lives across the items.)
+    const int hk = blockIdx.x % p.heads_kv, sh = p.page_shift, ratio = p.ratio, share = blockIdx.x / p.heads_kv;
+    // LDS-DMA, as in the attention kernels: lane l of an instruction fills row l / kChunks of
+    // its rows, physical chunk l % kChunks.
+    const auto row_of = [&](int l, int i) { return (wave * kInstr + i) * kRowsPerInstr + l / kChunks; };
+    const auto chunk_off = [&](int l, int i) { return (uint32_t)((((l % kChunks) ^ SW::h(row_of(l, i))) % kChunks) * 16); };
+    // Whole stages begin at a token, and their lanes' offsets from it have 32 bits.
+    const bool plain = kWeighRows % ratio == 0 && kWeighRows / ratio * p.q_token + ratio * p.q_head < (1LL << 30);
+    const size_t stage_bytes = (size_t)(kWeighRows / ratio) * p.q_token * 2;
+    WeighShare w;
+    {
+        const int l = threadIdx.x & 63;
+        if (!weigh_find<D>(p, l, share, w)) return;
+#pragma unroll
+        for (int i = 0; i < kInstr; ++i) {
+            const int row = row_of(l, i), q = row / ratio;
+            off[i][threadIdx.x] = (uint32_t)((q * p.q_token + (row - q * ratio) * p.q_head) * 2) + chunk_off(l, i);
+        }
+    }
+    int seq = w.seq;
+    long long at = w.at, left = w.u1 - w.u0;
+    while (left > 0 && seq < p.n_seqs) {
+        // (An opaque lane: nothing that is derived from it lives across the blocks.)
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
         const int g = lane >> 5;
-        PagedItem it;
-        if (!paged_find<false, false>(p, lane, j, it, [&](int i) { return weigh_count<D>(p, i); })) return;
-        PagedSeq sq = paged_seq(p, it.seq);
+        WeighSeq<D> sq(p, seq);
         sq.q0 = __builtin_amdgcn_readfirstlane(sq.q0);
         sq.qn = __builtin_amdgcn_readfirstlane(sq.qn);
         sq.kn = __builtin_amdgcn_readfirstlane(sq.kn);
-        const int R = sq.qn * ratio;
-        // (Of starts in no order the sums by which the item was found may wrap.)
-        const bool step = R <= 32;
-        const int kb = it.tile * (step ? WeighCfg<D>::kStepKeys : kKeys), k0 = kb + wave * kWaveKeys;
-        if ((unsigned)kb >= (unsigned)sq.kn || R == 0) continue;
-        if (step) {
-            weigh_step<kBF, D>(p, sq, it.seq, kb, hk, wave, lane, lds);
+        sq.rows = __builtin_amdgcn_readfirstlane(sq.rows);
+        sq.stages = __builtin_amdgcn_readfirstlane(sq.stages);
+        sq.step = sq.rows <= 32;
+        const long long all = sq.units(p);
+        if (at >= all) {
+            at -= all;
+            ++seq;
+            continue;
+        }
+        if (sq.step) {
+            // The runs that begin in this share.
+            const long long n = min(all - at, left);
+            const int r0 = (int)((at + Cfg::kStepUnits - 1) / Cfg::kStepUnits);
+            const int r1 = (int)((at + n + Cfg::kStepUnits - 1) / Cfg::kStepUnits);
+            if (r0 < r1) weigh_step<kBF, D>(p, sq, seq, r0, r1, hk, wave, lane, lds, step_sums[wave]);
+            at += n;
+            left -= n;
             __syncthreads();  // every wave is done with its stages
             continue;
         }
-        // LDS-DMA, as in the attention kernels: lane l of an instruction fills row l / kChunks of
-        // its rows, physical chunk l % kChunks.
-        const auto row_of = [&](int l, int i) { return (wave * kInstr + i) * kRowsPerInstr + l / kChunks; };
-        const auto chunk_off = [&](int l, int i) {
-            return (uint32_t)((((l % kChunks) ^ SW::h(row_of(l, i))) % kChunks) * 16);
-        };
-        // Whole stages begin at a token, and their lanes' offsets from it have 32 bits.
-        const bool plain = kWeighRows % ratio == 0 &&
-                           kWeighRows / ratio * p.q_token + ratio * p.q_head < (1LL << 30);
-        uint32_t off[kInstr], lse_off[2];
-#pragma unroll
-        for (int i = 0; i < kInstr; ++i) {
-            const int row = row_of(lane, i), q = row / ratio;
-            off[i] = (uint32_t)((q * p.q_token + (row - q * ratio) * p.q_head) * 2) + chunk_off(lane, i);
+        const int R = sq.rows, tile = __builtin_amdgcn_readfirstlane(sq.tile_of(p, at));
+        const long long begin = sq.units(p, tile);
+        const int s_first = sq.first(p, tile), n_units = sq.stages - s_first;
+        // Stages of this share.  Without a second kernel a block goes to the share of its first unit.
+        int s0 = s_first + (int)(at - begin), s1 = (int)min((long long)sq.stages, s0 + left);
+        const int skip = s0;
+        if (!p.cut) {
+            s1 = sq.stages;
+            if (s0 > s_first) s0 = s1;
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = 32 * h + (lane & 31), q = row / ratio;
-            lse_off[h] = (uint32_t)(q * p.heads_kv * ratio + (row - q * ratio)) * 4;
-        }
-        int koff[kNKK];
-#pragma unroll
-        for (int kk = 0; kk < kNKK; ++kk) {
-            const int r = lane & 31;
-            koff[kk] = r * kRowBytes + (((2 * kk + g) ^ SW::h(r)) % kChunks) * 16;
-        }
-        const int* const table = p.block_table + (size_t)it.seq * p.max_pages;
+        const bool whole_block = s0 == s_first && s1 == sq.stages;
+        const int slot = 2 * share + (s0 == s_first ? 1 : 0);
+        at = begin + (s1 - s_first);
+        left -= s1 - skip;
+        if (s0 >= s1 || n_units <= 0) continue;
+        const int kb = tile * kKeys, k0 = kb + wave * kWaveKeys, before = sq.before();
+        const int* const table = p.block_table + (size_t)seq * p.max_pages;
         const auto page_of = [&](int key) { return key < sq.kn ? table[key >> sh] : -1; };
         const auto valid = [&](int id) { return (unsigned)id < (unsigned)p.num_pages; };
         // The keys of the A operand.  Past the last, or on no valid page, any row will do: it
@@ -719,28 +834,25 @@ void kf_kv_weigh_kernel(PagedParams p) {
 #pragma unroll
             for (int kk = 0; kk < kNKK; ++kk) kf[t][kk] = *reinterpret_cast<const X8*>(Kr + (2 * kk + g) * 8);
         }
-        // Causal: query i sees keys j <= i + before.  Rows in front of the first that sees any
-        // of the block's do not count.
-        const int before = sq.kn - sq.qn;
-        const int first = p.causal ? max(kb - before, 0) * ratio : 0;
-        const int s_first = first / kWeighRows, stages = (R + kWeighRows - 1) / kWeighRows;
-        const int per = (stages - s_first + it.parts - 1) / it.parts;
-        const int s0 = s_first + it.part * per, s1 = min(s0 + per, stages);
+        int koff[kNKK];
+#pragma unroll
+        for (int kk = 0; kk < kNKK; ++kk) {
+            const int r = lane & 31;
+            koff[kk] = r * kRowBytes + (((2 * kk + g) ^ SW::h(r)) % kChunks) * 16;
+        }
         const char* const Qh = reinterpret_cast<const char*>(p.Q + (size_t)sq.q0 * p.q_token + (size_t)hk * ratio * p.q_head);
         const float* const lse = p.row_lse + ((size_t)sq.q0 * p.heads_kv + hk) * ratio;
-        const size_t stage_bytes = (size_t)(kWeighRows / ratio) * p.q_token * 2;
-        // Requests a stage, and this lane's row of each half of it: what its exponents are less
-        // by.  (Other stages than whole ones from an opaque lane.)
-        const auto issue_stage = [&](int s, float (&e)[2]) {
+        const uint32_t lse_off = (uint32_t)(lane / ratio * p.heads_kv * ratio + lane % ratio) * 4;
+        // Requests a stage, and the log-sum-exp of a row of it.  (Other stages than whole ones
+        // from an opaque lane.)
+        const auto issue_stage = [&](int s, float& e) {
             const int r0 = s * kWeighRows;
             const uint32_t d_lds = (uint32_t)(uintptr_t)(lds_void*)(buf(s) + wave * kInstr * 1024);
             if (plain && r0 + kWeighRows <= R) {
                 const char* const src = Qh + s * stage_bytes;
 #pragma unroll
-                for (int i = 0; i < kInstr; ++i) lds_copy16(d_lds + i * 1024, src, off[i]);
-                const char* const at = reinterpret_cast<const char*>(lse + (size_t)r0 * p.heads_kv);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) e[h] = *reinterpret_cast<const float*>(at + lse_off[h]);
+                for (int i = 0; i < kInstr; ++i) lds_copy16(d_lds + i * 1024, src, off[i][threadIdx.x]);
+                e = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(lse + (size_t)r0 * p.heads_kv) + lse_off);
             } else {
                 int l = lane;
                 asm volatile("" : "+v"(l));
@@ -750,50 +862,57 @@ void kf_kv_weigh_kernel(PagedParams p) {
                     lds_copy16(d_lds + i * 1024, Qh + ((size_t)q * p.q_token + (size_t)(row - q * ratio) * p.q_head) * 2 +
                                                      chunk_off(l, i));
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = min(r0 + 32 * h + (l & 31), R - 1), q = row / ratio;
-                    e[h] = lse[(size_t)q * p.heads_kv * ratio + (row - q * ratio)];
-                }
+                const int row = min(r0 + l, R - 1), q = row / ratio;
+                e = lse[(size_t)q * p.heads_kv * ratio + (row - q * ratio)];
             }
         };
-        // Rows in front of this one do not see all keys of the wave.
+        // Rows in front of `first` see no key of the wave, those in front of `whole` not all.
+        const int first = p.causal ? max(k0 - before, 0) * ratio : 0;
         const int whole = p.causal ? max(k0 + kWaveKeys - 1 - before, 0) * ratio : 0;
         f32x16 sum[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) sum[t] = f32x16{};
-        // The scores of 32 rows, and beside their products the exponentials of `old` ones, the
-        // instructions in this order: a wave overlaps the two only as they stand in its stream.
+        // The scores x of 32 rows, and beside their products the exponentials of `old` ones, the
+        // instructions in this order and the rows read a step ahead: a wave overlaps them
+        // only as they stand in its stream.
         const auto scores = [&](const char* rows, f32x16 (&x)[kTiles], const f32x16 (&old)[kTiles], float less) {
             constexpr int kPer = 16 * kTiles / kNKK;
             int kb0 = koff[0];
             if constexpr (kXorOff) asm volatile("" : "+v"(kb0));  // derived per tile
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) x[t] = f32x16{};
+            const auto read = [&](int kk) { return *reinterpret_cast<const X8*>(rows + (kXorOff ? kb0 ^ (32 * kk) : koff[kk])); };
+            X8 q[2] = {read(0)};
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int kk = 0; kk < kNKK; ++kk) {
-                const X8 q = *reinterpret_cast<const X8*>(rows + (kXorOff ? kb0 ^ (32 * kk) : koff[kk]));
+                if (kk + 1 < kNKK) q[(kk + 1) % 2] = read(kk + 1);
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t) x[t] = E::mfma32(kf[t][kk], q, x[t]);
+                for (int t = 0; t < kTiles; ++t) x[t] = E::mfma32(kf[t][kk], q[kk % 2], kk == 0 ? f32x16{} : x[t]);
 #pragma unroll
-                for (int i = kk * kPer; i < (kk + 1) * kPer; ++i)
-                    sum[i / 16][i % 16] += exp2_hw(fmaf(old[i / 16][i % 16], p.scale_log2, less));
-                __builtin_amdgcn_sched_barrier(0x100);            // LDS reads may pass
+                for (int e = kk * kPer; e < (kk + 1) * kPer; ++e)
+                    sum[e / 16][e % 16] += exp2_hw(fmaf(old[e / 16][e % 16], p.scale_log2, less));
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        const auto gather = [&](const f32x16 (&x)[kTiles], float less) {
+        // Keys that a row does not see -> -inf.
+        const auto hide = [&](f32x16 (&x)[kTiles], int r0) {
+            if (r0 >= whole) return;
+            asm volatile("" ::: "memory");                        // a branch, not selects in every tile
+            const int lim = min(r0 + (lane & 31), R - 1) / ratio + before + 1 - k0 - 4 * g;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum[t][r] += exp2_hw(fmaf(x[t][r], p.scale_log2, less));
+                for (int r = 0; r < 16; ++r)
+                    if (32 * t + 8 * (r >> 2) + (r & 3) >= lim) x[t][r] = -INFINITY;
         };
-        // Rows without a key add nothing.
-        const auto less_of = [&](float e) { return e > -INFINITY ? -e * kLog2e : -INFINITY; };
-        float e_next[2] = {0.f, 0.f};
+        // What the exponents of a row are less by; rows past the last, and those without a key,
+        // add nothing.
+        const auto less_of = [&](float e, int r0) {
+            return r0 + (lane & 31) < R && e > -INFINITY ? -e * kLog2e : -INFINITY;
+        };
+        float e_next = 0.f;
         if (s0 < s1) issue_stage(s0, e_next);
-        // The second half's scores wait for their exponentials until the next products: every
-        // product then runs beside other rows' exponentials.
-        f32x16 late[kTiles];
+        // The second half's scores wait for their exponentials until the next products.
+        f32x16 x[kTiles], late[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) late[t] = f32x16{};
         float late_less = -INFINITY;
@@ -802,36 +921,21 @@ void kf_kv_weigh_kernel(PagedParams p) {
             __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            const float e[2] = {e_next[0], e_next[1]};
+            const float e = e_next;
             if (s + 1 < s1) issue_stage(s + 1, e_next);
             const char* const rows = buf(s);
             const int r0 = s * kWeighRows;
-            f32x16 x[kTiles];
-            if (r0 >= whole && r0 + kWeighRows <= R) {
-                scores(rows, x, late, late_less);
-                scores(rows + 32 * kRowBytes, late, x, less_of(e[0]));
-                late_less = less_of(e[1]);
-                continue;
-            }
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                const int rh = r0 + 32 * h, row = rh + (lane & 31);
-                if (rh >= R || rh + 32 <= first) continue;
-                scores(rows + h * 32 * kRowBytes, x, late, late_less);
-                late_less = -INFINITY;
-                const float less = row < R ? less_of(h ? e[1] : e[0]) : -INFINITY;
-                // Keys of this lane that the row sees.
-                const int lim = p.causal ? min(row, R - 1) / ratio + before + 1 - k0 - 4 * g : INT_MAX;
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float w = exp2_hw(fmaf(x[t][r], p.scale_log2, less));
-                        sum[t][r] += 32 * t + 8 * (r >> 2) + (r & 3) < lim ? w : 0.f;
-                    }
-            }
+            if (r0 + kWeighRows <= first) continue;
+            scores(rows, x, late, late_less);
+            hide(x, r0);
+            scores(rows + 32 * kRowBytes, late, x, less_of(__shfl(e, lane & 31), r0));
+            hide(late, r0 + 32);
+            late_less = less_of(__shfl(e, 32 + (lane & 31)), r0 + 32);
         }
-        gather(late, late_less);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[t][r] += exp2_hw(fmaf(late[t][r], p.scale_log2, late_less));
         // Over the 32 rows: with every exchange a lane keeps half of its keys, in the end
         // lane l (and l ^ 16) the one of register l % 16.
 #pragma unroll
@@ -845,10 +949,10 @@ void kf_kv_weigh_kernel(PagedParams p) {
                     sum[t][r] = (up ? sum[t][r + (1 << b)] : sum[t][r]) + __shfl_xor(give, 1 << b);
                 }
             const float total = sum[t][0] + __shfl_xor(sum[t][0], 16);
-            const int at = wave * kWaveKeys + 32 * t + acc_row(lane & 15, lane), key = kb + at, id = page_of(key);
+            const int place = wave * kWaveKeys + 32 * t + acc_row(lane & 15, lane), key = kb + place, id = page_of(key);
             if ((lane & 16) != 0) continue;
-            if (it.parts > 1)
-                p.Opart[((size_t)it.slot * p.heads_kv + hk) * kKeys + at] = total;
+            if (!whole_block)
+                p.Opart[((size_t)slot * p.heads_kv + hk) * kKeys + place] = total;
             else if (valid(id))
                 p.weights[(((size_t)id * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))] += total;
         }
@@ -856,22 +960,43 @@ void kf_kv_weigh_kernel(PagedParams p) {
     }
 }
 
-// The parts of the blocks that were cut, added up in their order: a thread per key.
+// The sums of the blocks that were cut, added up: the first share that begins inside a
+// block sees to it.  A thread per key and quarter of the parts, eight loads on their
+// way, and the quarters in order.
 template <int D>
-__global__ __launch_bounds__(WeighCfg<D>::kKeys)
+__global__ __launch_bounds__(4 * WeighCfg<D>::kKeys)
 void kf_kv_weigh_merge_kernel(PagedParams p) {
-    constexpr int kKeys = WeighCfg<D>::kKeys;
-    const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv, sh = p.page_shift;
-    PagedItem it;
-    if (!paged_find<true, false>(p, lane, blockIdx.x / p.heads_kv, it, [&](int i) { return weigh_count<D>(p, i); })) return;
-    const PagedSeq sq = paged_seq(p, it.seq);
-    const int key = it.tile * kKeys + threadIdx.x;
-    if ((unsigned)it.tile * (unsigned)kKeys >= (unsigned)sq.kn || key >= sq.kn) return;
-    const int id = p.block_table[(size_t)it.seq * p.max_pages + (key >> sh)];
-    if ((unsigned)id >= (unsigned)p.num_pages) return;
+    constexpr int kKeys = WeighCfg<D>::kKeys, kRuns = 4;
+    __shared__ float sums[kRuns][kKeys];
+    const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv, share = blockIdx.x / p.heads_kv + 1, sh = p.page_shift;
+    WeighShare w;
+    if (!weigh_find<D>(p, lane, share, w)) return;
+    const WeighSeq<D> sq(p, w.seq);
+    if (sq.step) return;
+    const int tile = sq.tile_of(p, w.at);
+    const long long in_front = w.at - sq.units(p, tile), behind = sq.units(p, tile + 1) - w.at;
+    if (in_front <= 0 || in_front > w.share) return;
+    // The block's parts: the last of the share in front, the first of this and the later ones.
+    const int parts = 1 + (int)((behind + w.share - 1) / w.share);
+    const auto slot = [&](int k) { return k == 0 ? 2 * share - 1 : 2 * (share + k - 1); };
+    const int at = threadIdx.x % kKeys, run = threadIdx.x / kKeys, key = tile * kKeys + at;
+    const int per = (parts + kRuns - 1) / kRuns, k1 = min((run + 1) * per, parts);
     float total = 0.f;
-    for (int k = 0; k < it.parts; ++k)
-        total += p.Opart[((size_t)(it.slot + k) * p.heads_kv + hk) * kKeys + threadIdx.x];
+    for (int k = run * per; k < k1; k += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            v[u] = p.Opart[((size_t)slot(min(k + u, k1 - 1)) * p.heads_kv + hk) * kKeys + at];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) total += k + u < k1 ? v[u] : 0.f;
+    }
+    sums[run][at] = total;
+    __syncthreads();
+    if (run > 0 || key >= sq.kn) return;
+    const int id = p.block_table[(size_t)w.seq * p.max_pages + (key >> sh)];
+    if ((unsigned)id >= (unsigned)p.num_pages) return;
+#pragma unroll
+    for (int r = 1; r < kRuns; ++r) total += sums[r][at];
     p.weights[(((size_t)id * p.heads_kv + hk) << sh) + (key & ((1 << sh) - 1))] += total;
 }
 

@@ -402,49 +402,37 @@ void set_paged(kf::PagedParams& prm, const void* Q, const int64_t* strides, cons
 // ---- Gathered weights. ----
 
 struct WeighPlan {
-    long long cut_blocks;                 // at most, of a KV head
     size_t ws_bytes;
     kf::PagedParams prm;
 };
-
-int weigh_keys(int D) { return D == 256 ? kf::WeighCfg<256>::kKeys : kf::WeighCfg<128>::kKeys; }
 
 int weigh_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, int max_pages, int num_pages,
                WeighPlan* pl) {
     kf::PagedParams& prm = pl->prm;
     if (const int st = check_paged(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages, num_pages, &prm); st != KF_OK)
         return st;
-    const int keys = weigh_keys(D);
-    const long long blocks = ((long long)prm.kv_len + keys - 1) / keys;  // of a sequence, at most
-    if (blocks * n_seqs > kMaxIndex) return KF_ERR_SIZE;
-    const long long rows = (long long)tokens * (H_q / H_kv), cus = current_device_shape().cus;
-    const long long stages = rows / kf::kWeighRows + std::min(n_seqs, tokens);
-    // Blocks of keys are cut along the rows where these are many.
-    const int wanted = std::max(1, (int)(8 * cus / H_kv));
-    prm.target = rows / n_seqs < 8 * kf::kWeighRows ? 0 : wanted;
-    prm.unit_shift = 0;
-    while (blocks * ((stages >> prm.unit_shift) + n_seqs) > INT_MAX && prm.unit_shift < 30) ++prm.unit_shift;
-    if (blocks * ((stages >> prm.unit_shift) + n_seqs) > INT_MAX) prm.target = 0;
-    prm.min_share = std::max(1, 4 >> prm.unit_shift);
-    // Workgroups for all blocks that the tables could hold, up to many rounds of the device.
-    prm.stride = (int)std::min<long long>(blocks * n_seqs + prm.target, std::max<long long>(1, 32 * cus / H_kv));
-    pl->cut_blocks = std::min<long long>(blocks * n_seqs, prm.target);
-    pl->ws_bytes = align_up((size_t)2 * prm.target * H_kv * keys * sizeof(float), kWsAlign);
-    if (!fits_grid((long long)prm.stride * H_kv, kf::kWeighThreads) ||
-        !fits_grid(pl->cut_blocks * H_kv, keys))
-        return KF_ERR_SIZE;
-    return KF_OK;
+    const int keys = D == 256 ? kf::WeighCfg<256>::kKeys : kf::WeighCfg<128>::kKeys;
+    const long long rows = (long long)tokens * (H_q / H_kv);
+    // A share for every workgroup that the device holds.
+    prm.target = std::max(1, 2 * current_device_shape().cus / H_kv);
+    prm.min_share = 4;
+    // Blocks are cut where sequences have, on average, more than a stage of rows; a
+    // batch of steps is spared the second launch.
+    prm.cut = rows / n_seqs > kf::kWeighRows ? 1 : 0;
+    pl->ws_bytes = prm.cut ? align_up((size_t)2 * prm.target * H_kv * keys * sizeof(float), kWsAlign) : 0;
+    return fits_grid((long long)prm.target * H_kv, 4 * keys) ? KF_OK : KF_ERR_SIZE;
 }
 
 template <bool kBF, int D>
 int launch_weigh(const WeighPlan& pl, hipStream_t stream) {
+    using Cfg = kf::WeighCfg<D>;
     const kf::PagedParams& prm = pl.prm;
     (void)hipGetLastError();
     kf::kf_kv_weigh_kernel<kBF, D>
-        <<<dim3((unsigned)((long long)prm.stride * prm.heads_kv)), dim3(kf::kWeighThreads), 0, stream>>>(prm);
-    if (const int st = launched(); st != KF_OK || prm.target == 0) return st;
+        <<<dim3((unsigned)(prm.target * prm.heads_kv)), dim3(Cfg::kThreads), 0, stream>>>(prm);
+    if (const int st = launched(); st != KF_OK || !prm.cut || prm.target == 1) return st;
     kf::kf_kv_weigh_merge_kernel<D>
-        <<<dim3((unsigned)(pl.cut_blocks * prm.heads_kv)), dim3(kf::WeighCfg<D>::kKeys), 0, stream>>>(prm);
+        <<<dim3((unsigned)((prm.target - 1) * prm.heads_kv)), dim3(4 * Cfg::kKeys), 0, stream>>>(prm);
     return launched();
 }
 
