@@ -873,23 +873,29 @@ void kf_kv_weigh_kernel(PagedParams p) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) sum[t] = f32x16{};
         // The scores x of 32 rows, and beside their products the exponentials of `old` ones, the
-        // instructions in this order and the rows read a step ahead: a wave overlaps them
-        // only as they stand in its stream.
-        const auto scores = [&](const char* rows, f32x16 (&x)[kTiles], const f32x16 (&old)[kTiles], float less) {
+        // instructions in this order: a wave overlaps them only as they stand in its stream.
+        // Rows are read kAhead steps before they are used, also the first of the next 32.
+        constexpr int kAhead = 3;
+        X8 q[kAhead + 1];
+        int kb0 = koff[0];
+        const auto read = [&](const char* rows, int kk) {
+            return *reinterpret_cast<const X8*>(rows + (kXorOff ? kb0 ^ (32 * kk) : koff[kk]));
+        };
+        const auto scores = [&](const char* rows, const char* next, f32x16 (&x)[kTiles], const f32x16 (&old)[kTiles], float less) {
             constexpr int kPer = 16 * kTiles / kNKK;
-            int kb0 = koff[0];
             if constexpr (kXorOff) asm volatile("" : "+v"(kb0));  // derived per tile
-            const auto read = [&](int kk) { return *reinterpret_cast<const X8*>(rows + (kXorOff ? kb0 ^ (32 * kk) : koff[kk])); };
-            X8 q[2] = {read(0)};
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int kk = 0; kk < kNKK; ++kk) {
-                if (kk + 1 < kNKK) q[(kk + 1) % 2] = read(kk + 1);
+                if (kk + kAhead < kNKK) q[(kk + kAhead) % (kAhead + 1)] = read(rows, kk + kAhead);
+                else if (next) q[(kk + kAhead) % (kAhead + 1)] = read(next, kk + kAhead - kNKK);
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t) x[t] = E::mfma32(kf[t][kk], q[kk % 2], kk == 0 ? f32x16{} : x[t]);
+                for (int t = 0; t < kTiles; ++t) x[t] = E::mfma32(kf[t][kk], q[kk % (kAhead + 1)], kk == 0 ? f32x16{} : x[t]);
 #pragma unroll
-                for (int e = kk * kPer; e < (kk + 1) * kPer; ++e)
-                    sum[e / 16][e % 16] += exp2_hw(fmaf(old[e / 16][e % 16], p.scale_log2, less));
+                for (int e = kk * kPer; e < (kk + 1) * kPer; ++e) {
+                    float v = sum[e / 16][e % 16] + exp2_hw(fmaf(old[e / 16][e % 16], p.scale_log2, less));
+                    asm volatile("" : "+v"(v));                   // here, not behind later branches
+                    sum[e / 16][e % 16] = v;
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
@@ -926,9 +932,11 @@ void kf_kv_weigh_kernel(PagedParams p) {
             const char* const rows = buf(s);
             const int r0 = s * kWeighRows;
             if (r0 + kWeighRows <= first) continue;
-            scores(rows, x, late, late_less);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) q[i] = read(rows, i);
+            scores(rows, rows + 32 * kRowBytes, x, late, late_less);
             hide(x, r0);
-            scores(rows + 32 * kRowBytes, late, x, less_of(__shfl(e, lane & 31), r0));
+            scores(rows + 32 * kRowBytes, nullptr, late, x, less_of(__shfl(e, lane & 31), r0));
             hide(late, r0 + 32);
             late_less = less_of(__shfl(e, 32 + (lane & 31)), r0 + 32);
         }
