@@ -67,9 +67,9 @@ void kf_kv_append_kernel(KvAppendParams p) {
 // freed, the i-th to the i-th, and the last r to k .. m - 1, in order.  (Closing
 // the gaps in order would move half a head's keys where one of them goes.)
 //
-// Select: a workgroup per (sequence, KV head) finds the k-th largest weight by four
-// counts of 8 bits each, writes the moves to the workspace and moves the weights.
-// Move: the rows of K and V, by these lists.
+// Select: a workgroup per (sequence, KV head) finds the k-th largest weight by three
+// counts of 12, 10 and 10 bits and writes the moves to the workspace.  Move: the rows of K
+// and V and the weights, by these lists.
 // ---------------------------------------------------------------------------
 struct EvictParams {
     uint8_t* pages[2];          // K, V
@@ -79,8 +79,9 @@ struct EvictParams {
     const int* budgets;         // [n_seqs]
     int* kept;                  // [n_seqs], may be kv_lens or budgets
     int n_seqs, heads, recent, max_pages, page_shift, num_pages, capacity;
-    int* counts;                // [n_seqs * heads]: moves among the old keys, -1: none of the head's rows move
-    int* cuts;                  // [n_seqs * heads][2]: n, m
+    int parts;                  // workgroups of a head that move keys behind the new end
+    int* cuts;                  // [n_seqs * heads][4]: n, m, moves among the old keys (-1: none of the head's
+                                // rows move), how many of them are from places below m
     int* moves;                 // [n_seqs * heads][capacity]: where to, from the middle on where from
 };
 
@@ -88,9 +89,10 @@ struct EvictParams {
 struct EvictTable {
     const int* table;
     int heads, head, shift;
-    __device__ __forceinline__ size_t row(int key) const {   // of a pool seen as [rows]
-        return (((size_t)table[key >> shift] * heads + head) << shift) + (key & ((1 << shift) - 1));
+    __device__ __forceinline__ size_t at(int page, int key) const {   // of a pool seen as [rows]
+        return (((size_t)page * heads + head) << shift) + (key & ((1 << shift) - 1));
     }
+    __device__ __forceinline__ size_t row(int key) const { return at(table[key >> shift], key); }
     // Of a key that the workspace names, one of n (of weights that change while they are
     // looked through, it may hold none).
     __device__ __forceinline__ size_t listed(int key, int n) const { return row(min(max(key, 0), n - 1)); }
@@ -106,11 +108,24 @@ __device__ __forceinline__ uint32_t evict_order(uint32_t u) {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kSelectAhead = 8;       // weights of a thread on their way at a time
 
+// f(std::integral_constant<int, i>) for i = 0 .. n - 1, whatever the size of f.
+template <class F, int... I>
+__device__ __forceinline__ void evict_unrolled(const F& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+// kPer: up to so many old keys of a thread are read once, into registers; 0: read anew by
+// every pass.
+template <int kPer>
 __global__ __launch_bounds__(kSelectThreads)
 void kf_kv_evict_select_kernel(EvictParams p) {
-    __shared__ int hist[kSelectWaves][256];
-    __shared__ int wave_sums[3][kSelectWaves];
+    constexpr int kHeld = kPer > 0 ? kPer : 1, kPages = kHeld * kSelectThreads / 16;
+    static_assert(kHeld == 1 || kHeld % kSelectAhead == 0, "whole batches");
+    __shared__ int hist[1 << 12];
+    __shared__ int pages[kPages];     // of the old keys
+    __shared__ int wave_sums[4][kSelectWaves];
     __shared__ int found[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = blockIdx.x, b = grp / p.heads, head = grp % p.heads;
@@ -119,89 +134,135 @@ void kf_kv_evict_select_kernel(EvictParams p) {
     // A key on no valid page has no place: the sequence is left as it is.
     bool bad = false;
     if (m < n)
-        for (int i = tid; i <= (n - 1) >> p.page_shift; i += kSelectThreads)
-            bad |= (unsigned)tb.table[i] >= (unsigned)p.num_pages;
+        for (int i = tid; i <= (n - 1) >> p.page_shift; i += kSelectThreads) {
+            const int id = tb.table[i];
+            bad |= (unsigned)id >= (unsigned)p.num_pages;
+            if (kPer > 0 && i < kPages) pages[i] = id;
+        }
     const bool left = __syncthreads_or(bad) != 0 || m == n;
     const int r = min(p.recent, m), k = m - r, old = n - r;
+    int* const cuts = p.cuts + 4 * (size_t)grp;
     if (tid == 0) {
-        p.cuts[2 * grp] = n;
-        p.cuts[2 * grp + 1] = m;
-        if (left) p.counts[grp] = -1;
+        cuts[0] = n;
+        cuts[1] = m;
+        if (left) cuts[2] = -1;
     }
     // (kept may be the array that the other heads' workgroups still read: the mover
     // writes it.)
     if (left) return;
-    const auto order_at = [&](int i) { return evict_order(p.weights[tb.row(i)]); };
+    // Every wave has a run of the old keys, 64 at a time.
+    const int its = (old + kSelectThreads - 1) / kSelectThreads, i0 = wave * its * 64;
+    const auto place = [&](int i) { return i0 + 64 * i + lane; };
+    uint32_t held[kHeld];
+    if constexpr (kPer > 0) {
+        evict_unrolled([&](auto batch) {
+            constexpr int j = decltype(batch)::value * kSelectAhead;
+            if (j >= its) return;
+            uint32_t raw[kSelectAhead];
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u) {
+                const int at = min(place(j + u), old - 1);
+                raw[u] = p.weights[tb.at(pages[at >> p.page_shift], at)];
+            }
+#pragma unroll
+            for (int u = 0; u < kSelectAhead; ++u) held[j + u] = evict_order(raw[u]);
+        }, std::make_integer_sequence<int, kPer / kSelectAhead>{});
+    }
+    // f(place, its weight's order, whether there is such a key) for all of the wave's, in order.
+    const auto each = [&](auto f) {
+        if constexpr (kPer > 0) {
+            evict_unrolled([&](auto index) {
+                constexpr int i = decltype(index)::value;
+                if (i < its) f(place(i), held[i], place(i) < old);
+            }, std::make_integer_sequence<int, kPer>{});
+        } else {
+            for (int i = 0; i < its; ++i) {
+                const int at = min(place(i), old - 1);
+                f(place(i), evict_order(p.weights[tb.row(at)]), place(i) < old);
+            }
+        }
+    };
 
     // The k-th largest of the old weights: `top` so far of its bits, `need` how many of
     // those that share them are kept.
     uint32_t top = 0;
     int need = k;
     if (k > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < kSelectWaves * 256; i += kSelectThreads) (&hist[0][0])[i] = 0;
+        const auto count_digit = [&](auto shift_c, auto bits_c) {
+            constexpr int shift = decltype(shift_c)::value, bits = decltype(bits_c)::value, kBins = 1 << bits;
+            constexpr int kOwn = kBins / kSelectThreads;       // bins of a thread, the last first
+            for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
             __syncthreads();
-            for (int i = tid; i < old; i += kSelectThreads) {
-                const uint32_t u = order_at(i);
-                if (shift == 24 || (u >> (shift + 8)) == (top >> (shift + 8))) atomicAdd(&hist[wave][u >> shift & 255], 1);
+            each([&](int, uint32_t u, bool in) {
+                bool add = in;
+                if constexpr (shift + bits < 32) add = in && (u >> (shift + bits)) == (top >> (shift + bits));
+                const int bin = u >> shift & (kBins - 1);
+                // Those of the first lane's bin in one, however many are alike.
+                const uint64_t adds = __ballot(add);
+                if (adds == 0) return;
+                const int lead = __builtin_ctzll(adds), lead_bin = __builtin_amdgcn_readlane(bin, lead);
+                const uint64_t same = __ballot(add && bin == lead_bin);
+                if (lane == lead) atomicAdd(&hist[lead_bin], __popcll(same));
+                else if (add && bin != lead_bin) atomicAdd(&hist[bin], 1);
+            });
+            __syncthreads();
+            int bins[kOwn], sum = 0;
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e) {
+                bins[e] = hist[kBins - 1 - kOwn * tid - e];
+                sum += bins[e];
             }
+            const int inc = wave_scan(sum);
+            if (lane == 63) wave_sums[0][wave] = inc;
             __syncthreads();
-            if (wave == 0) {
-                // Lane l has the bins 255 - 4 l down to 252 - 4 l.
-                int bins[4], sum = 0;
-                for (int e = 0; e < 4; ++e) {
-                    bins[e] = 0;
-                    for (int w = 0; w < kSelectWaves; ++w) bins[e] += hist[w][255 - 4 * lane - e];
-                    sum += bins[e];
-                }
-                int above = wave_scan(sum) - sum;
-                if (above < need && above + sum >= need) {
-                    int e = 0;
-                    while (above + bins[e] < need) above += bins[e++];
-                    found[0] = 255 - 4 * lane - e;
-                    found[1] = need - above;
-                }
+            int above = inc - sum;
+            for (int w = 0; w < wave; ++w) above += wave_sums[0][w];
+            if (above < need && above + sum >= need) {
+                int e = 0;
+#pragma unroll
+                for (int o = 0; o + 1 < kOwn; ++o)
+                    if (e == o && above + bins[o] < need) above += bins[o], ++e;
+                found[0] = kBins - 1 - kOwn * tid - e;
+                found[1] = need - above;
             }
             __syncthreads();
             top |= (uint32_t)found[0] << shift;
             need = found[1];
-        }
+        };
+        count_digit(std::integral_constant<int, 20>{}, std::integral_constant<int, 12>{});
+        count_digit(std::integral_constant<int, 10>{}, std::integral_constant<int, 10>{});
+        count_digit(std::integral_constant<int, 0>{}, std::integral_constant<int, 10>{});
     }
-    // Every wave has a run of the old keys.  First the ones of the k-th weight, of which the
-    // first `need` are kept, then the places that are freed and the keys that move.
-    const int run = (old + kSelectThreads - 1) / kSelectThreads * 64, i0 = min(wave * run, old), i1 = min(i0 + run, old);
+    // Of the keys of the k-th weight the first `need` are kept.
     int equal = 0;
-    if (k > 0)
-        for (int i = i0; i < i1; i += 64) {
-            const bool in = i + lane < i1;
-            equal += __popcll(__ballot(in && order_at(min(i + lane, old - 1)) == top));
-        }
+    each([&](int, uint32_t u, bool in) { equal += __popcll(__ballot(in && u == top)); });
     if (lane == 0) wave_sums[0][wave] = equal;
     __syncthreads();
     int before = 0;
     for (int w = 0; w < wave; ++w) before += wave_sums[0][w];
     const uint64_t below = (1ull << lane) - 1;
     // Of 64 keys which are kept; `ties` counts those of the k-th weight.
-    const auto kept_of = [&](int i, int& ties) {
-        const bool in = i + lane < i1;
-        const uint32_t u = k > 0 ? order_at(min(i + lane, old - 1)) : 0;
+    const auto kept_of = [&](uint32_t u, bool in, int& ties) {
         const uint64_t same = __ballot(in && u == top);
         const bool keep = in && k > 0 && (u > top || (u == top && ties + __popcll(same & below) < need));
         ties += __popcll(same);
         return keep;
     };
-    int freed = 0, moved = 0, ties = before;
-    for (int i = i0; i < i1; i += 64) {
-        const bool keep = kept_of(i, ties);
-        freed += __popcll(__ballot(i + lane < min(i1, k) && !keep));
-        moved += __popcll(__ballot(i + lane >= k && keep));
-    }
+    // The places that are freed, the keys that move, and those of them below the new end.
+    int freed = 0, moved = 0, near = 0, ties = before;
+    each([&](int at, uint32_t u, bool in) {
+        const bool keep = kept_of(u, in, ties);
+        freed += __popcll(__ballot(in && at < k && !keep));
+        moved += __popcll(__ballot(keep && at >= k));
+        near += __popcll(__ballot(keep && at >= k && at < m));
+    });
     if (lane == 0) {
         wave_sums[1][wave] = freed;
         wave_sums[2][wave] = moved;
+        wave_sums[3][wave] = near;
     }
     __syncthreads();
-    int to = 0, from = 0, all_freed = 0, all_moved = 0;
+    int to = 0, from = 0, all_freed = 0, all_moved = 0, all_near = 0;
     for (int w = 0; w < kSelectWaves; ++w) {
         if (w < wave) {
             to += wave_sums[1][w];
@@ -209,6 +270,7 @@ void kf_kv_evict_select_kernel(EvictParams p) {
         }
         all_freed += wave_sums[1][w];
         all_moved += wave_sums[2][w];
+        all_near += wave_sums[3][w];
     }
     // As many places are freed as keys move, no more than half of the old keys (of weights
     // that change meanwhile, as of a page that two sequences share, perhaps not).
@@ -216,68 +278,107 @@ void kf_kv_evict_select_kernel(EvictParams p) {
     int* const list = p.moves + (size_t)grp * p.capacity;
     int* const sources = list + half;
     ties = before;
-    for (int i = i0; i < i1; i += 64) {
-        const bool keep = kept_of(i, ties);
-        const bool f = i + lane < min(i1, k) && !keep, v = i + lane >= k && keep;
+    each([&](int at, uint32_t u, bool in) {
+        const bool keep = kept_of(u, in, ties);
+        const bool f = in && at < k && !keep, v = keep && at >= k;
         const uint64_t fs = __ballot(f), vs = __ballot(v);
         const int f_at = to + __popcll(fs & below), v_at = from + __popcll(vs & below);
-        if (f && f_at < half) list[f_at] = i + lane;
-        if (v && v_at < half) sources[v_at] = i + lane;
+        if (f && f_at < half) list[f_at] = at;
+        if (v && v_at < half) sources[v_at] = at;
         to += __popcll(fs);
         from += __popcll(vs);
-    }
-    if (tid == 0) p.counts[grp] = count;
-    __syncthreads();
-    // The weights: first the moves, whose places lie in front of all sources, then the last r.
-    for (int i = tid; i < count; i += kSelectThreads) p.weights[tb.listed(list[i], n)] = p.weights[tb.listed(sources[i], n)];
-    __syncthreads();
-    for (int i = 0; i < r; i += kSelectThreads) {
-        const uint32_t w = i + tid < r ? p.weights[tb.row(old + i + tid)] : 0;
-        __syncthreads();
-        if (i + tid < r) p.weights[tb.row(k + i + tid)] = w;
+    });
+    if (tid == 0) {
+        cuts[2] = count;
+        cuts[3] = min(all_near, count);
     }
 }
 
-// A workgroup per (sequence, KV head), tensor and 128 bytes of a row; rows of other
-// segments lie elsewhere, so that only its own loads and stores have to be in order.
+// Keys from below the new end m have to be read before the last r are written over them:
+// these, and the last r in order, are moved by a workgroup per (sequence, KV head), tensor and
+// 128 bytes of a row, in which rows of other segments lie elsewhere.  The others are
+// from places that are not written and go to freed ones that are not read: whole rows
+// by `parts` more workgroups of the head, in any order.
 constexpr int kMoveThreads = 256;
-constexpr int kMoveAhead = 4;          // rows of a thread in flight
+constexpr int kMoveAhead = 4;          // rows of a thread on their way
 
 template <int D>
 __global__ __launch_bounds__(kMoveThreads)
 void kf_kv_evict_move_kernel(EvictParams p) {
-    constexpr int kSegments = D / 64, kRows = kMoveThreads / 8;   // 8 lanes of 16 bytes a row
-    const int tid = threadIdx.x, seg = blockIdx.x % (2 * kSegments), grp = blockIdx.x / (2 * kSegments);
-    const int b = grp / p.heads, head = grp % p.heads;
-    const int count = p.counts[grp], n = p.cuts[2 * grp], m = p.cuts[2 * grp + 1];
-    if (head == 0 && seg == 0 && tid == 0) p.kept[b] = count < 0 ? n : m;
+    constexpr int kSegments = 2 * (D / 64);
+    const int tid = threadIdx.x, groups = p.n_seqs * p.heads;
+    const bool bulk = blockIdx.x >= (unsigned)(groups * kSegments);
+    const int item = bulk ? blockIdx.x - groups * kSegments : blockIdx.x, of = bulk ? p.parts : kSegments;
+    const int grp = item / of, seg = item % of, b = grp / p.heads, head = grp % p.heads;
+    const int* const cuts = p.cuts + 4 * (size_t)grp;
+    const int n = cuts[0], m = cuts[1], count = cuts[2];
+    if (!bulk && head == 0 && seg == 0 && tid == 0) p.kept[b] = count < 0 ? n : m;
     if (count < 0) return;
+    const int near = cuts[3];
     const EvictTable tb{p.block_table + (size_t)b * p.max_pages, p.heads, head, p.page_shift};
-    uint8_t* const pool = p.pages[seg / kSegments] + seg % kSegments * 128 + tid % 8 * 16;
-    const auto at = [&](size_t row) { return reinterpret_cast<u32x4*>(pool + row * (2 * D)); };
     const int r = min(p.recent, m), k = m - r, old = n - r;
     const int* const list = p.moves + (size_t)grp * p.capacity;
     const int* const sources = list + p.capacity / 2;
-    for (int i0 = tid / 8; i0 < count; i0 += kRows * kMoveAhead) {
-        u32x4 v[kMoveAhead];
+    if (bulk) {
+        constexpr int kLanes = D / 8, kRows = kMoveThreads / kLanes, kStep = kRows * kMoveAhead;
+        const int chunk = tid % kLanes;
+        const auto at = [&](int s, size_t row) { return reinterpret_cast<u32x4*>(p.pages[s] + row * (2 * D)) + chunk; };
+        for (int i0 = near + seg * kStep; i0 < count; i0 += p.parts * kStep) {
+            size_t from[kMoveAhead], to[kMoveAhead];
+            u32x4 v[kMoveAhead][2];
+            uint32_t w[kMoveAhead];
 #pragma unroll
-        for (int u = 0; u < kMoveAhead; ++u) v[u] = *at(tb.listed(sources[min(i0 + u * kRows, count - 1)], n));
+            for (int u = 0; u < kMoveAhead; ++u) {
+                const int i = min(i0 + u * kRows + tid / kLanes, count - 1);
+                from[u] = tb.listed(sources[i], n);
+                to[u] = tb.listed(list[i], n);
+            }
 #pragma unroll
-        for (int u = 0; u < kMoveAhead; ++u)
-            if (i0 + u * kRows < count) *at(tb.listed(list[i0 + u * kRows], n)) = v[u];
+            for (int u = 0; u < kMoveAhead; ++u) {
+                v[u][0] = *at(0, from[u]);
+                v[u][1] = *at(1, from[u]);
+                w[u] = chunk == 0 ? p.weights[from[u]] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < kMoveAhead; ++u) {
+                if (i0 + u * kRows + tid / kLanes >= count) continue;
+                *at(0, to[u]) = v[u][0];
+                *at(1, to[u]) = v[u][1];
+                if (chunk == 0) p.weights[to[u]] = w[u];
+            }
+        }
+        return;
     }
-    // The last r keys, over places that the moves have read.
+    constexpr int kRows = kMoveThreads / 8, kStep = kRows * kMoveAhead;   // 8 lanes of 16 bytes a row
+    uint8_t* const pool = p.pages[seg / (D / 64)] + seg % (D / 64) * 128 + tid % 8 * 16;
+    const auto at = [&](size_t row) { return reinterpret_cast<u32x4*>(pool + row * (2 * D)); };
+    const bool weigh = seg == 0 && tid % 8 == 0;          // moves the weights too
+    // `count` rows, from and to of the i-th; a place is written when all that is in front of it in
+    // the list, and kStep rows from it on, has been read.
+    const auto move = [&](int count, auto from_of, auto to_of) {
+        for (int i0 = 0; i0 < count; i0 += kStep) {
+            u32x4 v[kMoveAhead];
+            uint32_t w[kMoveAhead];
+#pragma unroll
+            for (int u = 0; u < kMoveAhead; ++u) {
+                const size_t from = from_of(min(i0 + u * kRows + tid / 8, count - 1));
+                v[u] = *at(from);
+                w[u] = weigh ? p.weights[from] : 0;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < kMoveAhead; ++u) {
+                const int i = i0 + u * kRows + tid / 8;
+                if (i >= count) continue;
+                const size_t to = to_of(i);
+                *at(to) = v[u];
+                if (weigh) p.weights[to] = w[u];
+            }
+        }
+    };
+    move(near, [&](int i) { return tb.listed(sources[i], n); }, [&](int i) { return tb.listed(list[i], n); });
     __syncthreads();
-    for (int i = 0; i < r; i += kRows * kMoveAhead) {
-        u32x4 v[kMoveAhead];
-#pragma unroll
-        for (int u = 0; u < kMoveAhead; ++u) v[u] = *at(tb.row(old + min(i + u * kRows + tid / 8, r - 1)));
-        // A place is written when it has been read; later rows are read behind all of these.
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < kMoveAhead; ++u)
-            if (const int j = i + u * kRows + tid / 8; j < r) *at(tb.row(k + j)) = v[u];
-    }
+    move(r, [&](int i) { return tb.row(old + i); }, [&](int i) { return tb.row(k + i); });
 }
 
 }  // namespace kf

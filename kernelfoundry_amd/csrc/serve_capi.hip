@@ -458,8 +458,8 @@ int launch_append(kf::KvAppendParams& prm, hipStream_t stream) {
 }
 
 struct EvictPlan {
-    int shift, capacity;
-    size_t counts_bytes, cuts_bytes, ws_bytes;
+    int shift, capacity, parts;
+    size_t cuts_bytes, ws_bytes;
 };
 
 int evict_plan(int n_seqs, int H_kv, int D, int page_size, int max_pages, int num_pages, EvictPlan* pl) {
@@ -467,22 +467,30 @@ int evict_plan(int n_seqs, int H_kv, int D, int page_size, int max_pages, int nu
     if (n_seqs <= 0 || H_kv <= 0) return KF_ERR_SIZE;
     if (const int st = paged_geometry(page_size, max_pages, num_pages, &pl->shift, &pl->capacity); st != KF_OK) return st;
     const long long groups = (long long)n_seqs * H_kv;
+    // Up to 32 workgroups a CU that move keys, each with a few rounds at least.
+    const long long rounds = pl->capacity / 2 / (kf::kMoveThreads * 8 / D * kf::kMoveAhead);
+    pl->parts = (int)std::max<long long>(1, std::min(32LL * current_device_shape().cus / groups, rounds / 4));
     if (pl->capacity > kMaxIndex || !fits_grid(groups, kf::kSelectThreads) ||
-        !fits_grid(groups * (D / 32), kf::kMoveThreads))
+        !fits_grid(groups * (D / 32 + pl->parts), kf::kMoveThreads))
         return KF_ERR_SIZE;
-    pl->counts_bytes = align_up((size_t)groups * sizeof(int), kWsAlign);
-    pl->cuts_bytes = align_up((size_t)groups * 2 * sizeof(int), kWsAlign);
-    pl->ws_bytes = pl->counts_bytes + pl->cuts_bytes + align_up((size_t)groups * pl->capacity * sizeof(int), kWsAlign);
+    pl->cuts_bytes = align_up((size_t)groups * 4 * sizeof(int), kWsAlign);
+    pl->ws_bytes = pl->cuts_bytes + align_up((size_t)groups * pl->capacity * sizeof(int), kWsAlign);
     return KF_OK;
 }
 
 template <int D>
 int launch_evict(const kf::EvictParams& prm, hipStream_t stream) {
     const int groups = prm.n_seqs * prm.heads;
+    const dim3 grid(groups), block(kf::kSelectThreads);
     (void)hipGetLastError();
-    kf::kf_kv_evict_select_kernel<<<dim3(groups), dim3(kf::kSelectThreads), 0, stream>>>(prm);
+    if (prm.capacity <= 16 * kf::kSelectThreads)
+        kf::kf_kv_evict_select_kernel<16><<<grid, block, 0, stream>>>(prm);
+    else if (prm.capacity <= 80 * kf::kSelectThreads)
+        kf::kf_kv_evict_select_kernel<80><<<grid, block, 0, stream>>>(prm);
+    else
+        kf::kf_kv_evict_select_kernel<0><<<grid, block, 0, stream>>>(prm);
     if (const int st = launched(); st != KF_OK) return st;
-    kf::kf_kv_evict_move_kernel<D><<<dim3(groups * (D / 32)), dim3(kf::kMoveThreads), 0, stream>>>(prm);
+    kf::kf_kv_evict_move_kernel<D><<<dim3(groups * (D / 32 + prm.parts)), dim3(kf::kMoveThreads), 0, stream>>>(prm);
     return launched();
 }
 
@@ -832,9 +840,9 @@ int kf_kv_evict(void* K_pages, void* V_pages, float* weights, const int* block_t
     prm.num_pages = num_pages;
     prm.capacity = pl.capacity;
     char* ws = static_cast<char*>(workspace);
-    prm.counts = reinterpret_cast<int*>(ws);
-    prm.cuts = reinterpret_cast<int*>(ws + pl.counts_bytes);
-    prm.moves = reinterpret_cast<int*>(ws + pl.counts_bytes + pl.cuts_bytes);
+    prm.parts = pl.parts;
+    prm.cuts = reinterpret_cast<int*>(ws);
+    prm.moves = reinterpret_cast<int*>(ws + pl.cuts_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (D) {
         case 64: return launch_evict<64>(prm, s);
