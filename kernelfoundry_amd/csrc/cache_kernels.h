@@ -108,8 +108,12 @@ __device__ __forceinline__ uint32_t evict_order(uint32_t u) {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kSelectAhead = 8;       // weights of a thread on their way at a time
+constexpr int kSelectAhead = 16;      // weights of a thread on their way at a time
 
+// Bits of lanes below this one.
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
 // f(std::integral_constant<int, i>) for i = 0 .. n - 1, whatever the size of f.
 template <class F, int... I>
 __device__ __forceinline__ void evict_unrolled(const F& f, std::integer_sequence<int, I...>) {
@@ -126,7 +130,7 @@ void kf_kv_evict_select_kernel(EvictParams p) {
     __shared__ int hist[1 << 12];
     __shared__ int pages[kPages];     // of the old keys
     __shared__ int wave_sums[4][kSelectWaves];
-    __shared__ int found[2];
+    __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = blockIdx.x, b = grp / p.heads, head = grp % p.heads;
     const EvictTable tb{p.block_table + (size_t)b * p.max_pages, p.heads, head, p.page_shift};
@@ -165,45 +169,46 @@ void kf_kv_evict_select_kernel(EvictParams p) {
                 raw[u] = p.weights[tb.at(pages[at >> p.page_shift], at)];
             }
 #pragma unroll
-            for (int u = 0; u < kSelectAhead; ++u) held[j + u] = evict_order(raw[u]);
+            for (int u = 0; u < kSelectAhead; ++u) held[j + u] = place(j + u) < old ? evict_order(raw[u]) : 0;
         }, std::make_integer_sequence<int, kPer / kSelectAhead>{});
     }
-    // f(place, its weight's order, whether there is such a key) for all of the wave's, in order.
+    // f(place of lane 0, a weight's order) for all of the wave's keys, 64 at a time and in order.  Lanes
+    // past the last key have 0, less than any weight's order.
     const auto each = [&](auto f) {
         if constexpr (kPer > 0) {
             evict_unrolled([&](auto index) {
                 constexpr int i = decltype(index)::value;
-                if (i < its) f(place(i), held[i], place(i) < old);
+                if (i < its) f(i0 + 64 * i, held[i]);
             }, std::make_integer_sequence<int, kPer>{});
         } else {
             for (int i = 0; i < its; ++i) {
                 const int at = min(place(i), old - 1);
-                f(place(i), evict_order(p.weights[tb.row(at)]), place(i) < old);
+                f(i0 + 64 * i, place(i) < old ? evict_order(p.weights[tb.row(at)]) : 0);
             }
         }
     };
 
     // The k-th largest of the old weights: `top` so far of its bits, `need` how many of
-    // those that share them are kept.
-    uint32_t top = 0;
-    int need = k;
+    // those that share them are kept, of `alike`.
+    uint32_t top = 0xffffffffu;
+    int need = 0, alike = 1;
     if (k > 0) {
+        top = 0;
+        need = k;
         const auto count_digit = [&](auto shift_c, auto bits_c) {
             constexpr int shift = decltype(shift_c)::value, bits = decltype(bits_c)::value, kBins = 1 << bits;
             constexpr int kOwn = kBins / kSelectThreads;       // bins of a thread, the last first
             for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
             __syncthreads();
-            each([&](int, uint32_t u, bool in) {
-                bool add = in;
-                if constexpr (shift + bits < 32) add = in && (u >> (shift + bits)) == (top >> (shift + bits));
+            each([&](int, uint32_t u) {
                 const int bin = u >> shift & (kBins - 1);
-                // Those of the first lane's bin in one, however many are alike.
-                const uint64_t adds = __ballot(add);
-                if (adds == 0) return;
-                const int lead = __builtin_ctzll(adds), lead_bin = __builtin_amdgcn_readlane(bin, lead);
-                const uint64_t same = __ballot(add && bin == lead_bin);
-                if (lane == lead) atomicAdd(&hist[lead_bin], __popcll(same));
-                else if (add && bin != lead_bin) atomicAdd(&hist[bin], 1);
+                if constexpr (shift + bits < 32) {
+                    if ((u >> (shift + bits)) == (top >> (shift + bits))) atomicAdd(&hist[bin], 1);
+                } else if (const int lead = __builtin_amdgcn_readfirstlane(bin); __all(bin == lead)) {
+                    if (lane == 0) atomicAdd(&hist[lead], 64);       // one place for 64 lanes is slow
+                } else {
+                    atomicAdd(&hist[bin], 1);
+                }
             });
             __syncthreads();
             int bins[kOwn], sum = 0;
@@ -218,43 +223,50 @@ void kf_kv_evict_select_kernel(EvictParams p) {
             int above = inc - sum;
             for (int w = 0; w < wave; ++w) above += wave_sums[0][w];
             if (above < need && above + sum >= need) {
-                int e = 0;
+                int e = 0, of = bins[0];
 #pragma unroll
                 for (int o = 0; o + 1 < kOwn; ++o)
-                    if (e == o && above + bins[o] < need) above += bins[o], ++e;
+                    if (e == o && above + bins[o] < need) above += bins[o], ++e, of = bins[o + 1];
                 found[0] = kBins - 1 - kOwn * tid - e;
                 found[1] = need - above;
+                found[2] = of;
             }
             __syncthreads();
             top |= (uint32_t)found[0] << shift;
             need = found[1];
+            alike = found[2];
         };
         count_digit(std::integral_constant<int, 20>{}, std::integral_constant<int, 12>{});
         count_digit(std::integral_constant<int, 10>{}, std::integral_constant<int, 10>{});
         count_digit(std::integral_constant<int, 0>{}, std::integral_constant<int, 10>{});
     }
-    // Of the keys of the k-th weight the first `need` are kept.
-    int equal = 0;
-    each([&](int, uint32_t u, bool in) { equal += __popcll(__ballot(in && u == top)); });
-    if (lane == 0) wave_sums[0][wave] = equal;
-    __syncthreads();
+    // Of the keys of the k-th weight the first `need` are kept; mostly that is all of them.
+    const bool tie = need < alike;
     int before = 0;
-    for (int w = 0; w < wave; ++w) before += wave_sums[0][w];
-    const uint64_t below = (1ull << lane) - 1;
+    if (tie) {
+        int equal = 0;
+        each([&](int, uint32_t u) { equal += __popcll(__ballot(u == top)); });
+        if (lane == 0) wave_sums[0][wave] = equal;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) before += wave_sums[0][w];
+    }
     // Of 64 keys which are kept; `ties` counts those of the k-th weight.
-    const auto kept_of = [&](uint32_t u, bool in, int& ties) {
-        const uint64_t same = __ballot(in && u == top);
-        const bool keep = in && k > 0 && (u > top || (u == top && ties + __popcll(same & below) < need));
+    const auto kept_of = [&](uint32_t u, int& ties) {
+        if (!tie) return (uint64_t)__ballot(u >= top);
+        const uint64_t same = __ballot(u == top);
+        const uint64_t keep = __ballot(u > top || (u == top && ties + lanes_below(same) < need));
         ties += __popcll(same);
         return keep;
     };
+    // Those of 64 places from c on that are below x.
+    const auto low = [](int c, int x) { return c + 64 <= x ? ~0ull : c >= x ? 0ull : (1ull << (x - c)) - 1; };
     // The places that are freed, the keys that move, and those of them below the new end.
     int freed = 0, moved = 0, near = 0, ties = before;
-    each([&](int at, uint32_t u, bool in) {
-        const bool keep = kept_of(u, in, ties);
-        freed += __popcll(__ballot(in && at < k && !keep));
-        moved += __popcll(__ballot(keep && at >= k));
-        near += __popcll(__ballot(keep && at >= k && at < m));
+    each([&](int c, uint32_t u) {
+        const uint64_t keep = kept_of(u, ties), front = low(c, k);
+        freed += __popcll(front & ~keep);
+        moved += __popcll(keep & ~front);
+        near += __popcll(keep & ~front & low(c, m));
     });
     if (lane == 0) {
         wave_sums[1][wave] = freed;
@@ -278,13 +290,11 @@ void kf_kv_evict_select_kernel(EvictParams p) {
     int* const list = p.moves + (size_t)grp * p.capacity;
     int* const sources = list + half;
     ties = before;
-    each([&](int at, uint32_t u, bool in) {
-        const bool keep = kept_of(u, in, ties);
-        const bool f = in && at < k && !keep, v = keep && at >= k;
-        const uint64_t fs = __ballot(f), vs = __ballot(v);
-        const int f_at = to + __popcll(fs & below), v_at = from + __popcll(vs & below);
-        if (f && f_at < half) list[f_at] = at;
-        if (v && v_at < half) sources[v_at] = at;
+    each([&](int c, uint32_t u) {
+        const uint64_t keep = kept_of(u, ties), front = low(c, k), fs = front & ~keep, vs = keep & ~front;
+        const int f_at = to + lanes_below(fs), v_at = from + lanes_below(vs);
+        if ((fs >> lane & 1) && f_at < half) list[f_at] = c + lane;
+        if ((vs >> lane & 1) && v_at < half) sources[v_at] = c + lane;
         to += __popcll(fs);
         from += __popcll(vs);
     });
