@@ -127,14 +127,15 @@ __global__ __launch_bounds__(kSelectThreads)
 void kf_kv_evict_select_kernel(EvictParams p) {
     constexpr int kHeld = kPer > 0 ? kPer : 1, kPages = kHeld * kSelectThreads / 16;
     static_assert(kHeld == 1 || kHeld % kSelectAhead == 0, "whole batches");
-    __shared__ int hist[1 << 12];
+    constexpr int kHist = (1 << 12) + 2 * (1 << 10) + 3 * 256;
+    __shared__ __attribute__((aligned(16))) int hist[kHist];   // of all three counts
     __shared__ int pages[kPages];     // of the old keys
     __shared__ int wave_sums[4][kSelectWaves];
-    __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = blockIdx.x, b = grp / p.heads, head = grp % p.heads;
     const EvictTable tb{p.block_table + (size_t)b * p.max_pages, p.heads, head, p.page_shift};
     const int n = min(max(p.kv_lens[b], 0), p.capacity), m = min(max(p.budgets[b], 0), n);
+    for (int i = tid; i < kHist; i += kSelectThreads) hist[i] = 0;
     // A key on no valid page has no place: the sequence is left as it is.
     bool bad = false;
     if (m < n)
@@ -165,8 +166,11 @@ void kf_kv_evict_select_kernel(EvictParams p) {
             uint32_t raw[kSelectAhead];
 #pragma unroll
             for (int u = 0; u < kSelectAhead; ++u) {
-                const int at = min(place(j + u), old - 1);
-                raw[u] = p.weights[tb.at(pages[at >> p.page_shift], at)];
+                raw[u] = 0;
+                if (j + u < its) {
+                    const int at = min(place(j + u), old - 1);
+                    raw[u] = p.weights[tb.at(pages[at >> p.page_shift], at)];
+                }
             }
 #pragma unroll
             for (int u = 0; u < kSelectAhead; ++u) held[j + u] = place(j + u) < old ? evict_order(raw[u]) : 0;
@@ -195,50 +199,42 @@ void kf_kv_evict_select_kernel(EvictParams p) {
     if (k > 0) {
         top = 0;
         need = k;
-        const auto count_digit = [&](auto shift_c, auto bits_c) {
+        const auto count_digit = [&](auto shift_c, auto bits_c, int* hist) {
+            // Bins lie in 64 runs, each padded by four: the reads below go to all banks.
             constexpr int shift = decltype(shift_c)::value, bits = decltype(bits_c)::value, kBins = 1 << bits;
-            constexpr int kOwn = kBins / kSelectThreads;       // bins of a thread, the last first
-            for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
-            __syncthreads();
+            constexpr int kRun = kBins / 64;
+            const auto slot = [](int bin) { return bin + bin / kRun * 4; };
             each([&](int, uint32_t u) {
                 const int bin = u >> shift & (kBins - 1);
                 if constexpr (shift + bits < 32) {
-                    if ((u >> (shift + bits)) == (top >> (shift + bits))) atomicAdd(&hist[bin], 1);
+                    if ((u >> (shift + bits)) == (top >> (shift + bits))) atomicAdd(&hist[slot(bin)], 1);
                 } else if (const int lead = __builtin_amdgcn_readfirstlane(bin); __all(bin == lead)) {
-                    if (lane == 0) atomicAdd(&hist[lead], 64);       // one place for 64 lanes is slow
+                    if (lane == 0) atomicAdd(&hist[slot(lead)], 64);       // one place for 64 lanes is slow
                 } else {
-                    atomicAdd(&hist[bin], 1);
+                    atomicAdd(&hist[slot(bin)], 1);
                 }
             });
             __syncthreads();
-            int bins[kOwn], sum = 0;
+            // Every wave finds the bin: its run, of which lane l has the one 63 - l, and then it in the run.
+            int sum = 0;
 #pragma unroll
-            for (int e = 0; e < kOwn; ++e) {
-                bins[e] = hist[kBins - 1 - kOwn * tid - e];
-                sum += bins[e];
+            for (int e = 0; e < kRun; e += 4) {
+                const int4 v = *reinterpret_cast<const int4*>(&hist[slot((63 - lane) * kRun) + e]);
+                sum += (v.x + v.y) + (v.z + v.w);
             }
-            const int inc = wave_scan(sum);
-            if (lane == 63) wave_sums[0][wave] = inc;
-            __syncthreads();
-            int above = inc - sum;
-            for (int w = 0; w < wave; ++w) above += wave_sums[0][w];
-            if (above < need && above + sum >= need) {
-                int e = 0, of = bins[0];
-#pragma unroll
-                for (int o = 0; o + 1 < kOwn; ++o)
-                    if (e == o && above + bins[o] < need) above += bins[o], ++e, of = bins[o + 1];
-                found[0] = kBins - 1 - kOwn * tid - e;
-                found[1] = need - above;
-                found[2] = of;
-            }
-            __syncthreads();
-            top |= (uint32_t)found[0] << shift;
-            need = found[1];
-            alike = found[2];
+            int inc = wave_scan(sum);
+            const int run = __builtin_ctzll(__ballot(inc >= need));
+            need -= __builtin_amdgcn_readlane(inc, run) - __builtin_amdgcn_readlane(sum, run);
+            sum = lane < kRun ? hist[slot((63 - run) * kRun) + kRun - 1 - lane] : 0;
+            inc = wave_scan(sum);
+            const int e = __builtin_ctzll(__ballot(inc >= need));
+            alike = __builtin_amdgcn_readlane(sum, e);
+            need -= __builtin_amdgcn_readlane(inc, e) - alike;
+            top |= (uint32_t)((63 - run) * kRun + kRun - 1 - e) << shift;
         };
-        count_digit(std::integral_constant<int, 20>{}, std::integral_constant<int, 12>{});
-        count_digit(std::integral_constant<int, 10>{}, std::integral_constant<int, 10>{});
-        count_digit(std::integral_constant<int, 0>{}, std::integral_constant<int, 10>{});
+        count_digit(std::integral_constant<int, 20>{}, std::integral_constant<int, 12>{}, hist);
+        count_digit(std::integral_constant<int, 10>{}, std::integral_constant<int, 10>{}, hist + (1 << 12) + 256);
+        count_digit(std::integral_constant<int, 0>{}, std::integral_constant<int, 10>{}, hist + (1 << 12) + (1 << 10) + 512);
     }
     // Of the keys of the k-th weight the first `need` are kept; mostly that is all of them.
     const bool tie = need < alike;
