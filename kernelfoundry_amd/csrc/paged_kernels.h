@@ -138,6 +138,79 @@ __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j
     return it.parts == 1 || (unsigned)it.slot + (kCut ? it.parts : 1u) <= 2u * (unsigned)p.target;
 }
 
+// The work of a KV head as a line of units, its sequences one after the other, of which every
+// workgroup has an equal share.  Share j: from unit u0 of the line on to u1; the sequence
+// of u0 and its place among the sequence's units.  By the lanes of a wave; false past the last
+// unit.
+struct LineShare {
+    long long u0, u1, share, at;
+    int seq;
+};
+__device__ __forceinline__ long long line_scan(long long v, int lane) {
+    if (__all(v < 1 << 24)) return wave_scan((int)v);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+__device__ __forceinline__ long long line_lane(long long v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (long long)((uint64_t)hi << 32 | lo);
+}
+// a / b, a not negative, mostly by 32 bits.
+__device__ __forceinline__ long long line_div(long long a, int b) {
+    return a < INT_MAX ? (int)((unsigned)a / (unsigned)b) : a / b;
+}
+template <class UnitsOf>
+__device__ __forceinline__ bool line_find(const PagedParams& p, int lane, int j, LineShare& w, const UnitsOf& units_of) {
+    const int per = (p.n_seqs + 63) / 64, first = min(lane * per, p.n_seqs), last = min(first + per, p.n_seqs);
+    long long mine = 0;
+    for (int i = first; i < last; ++i) mine += units_of(i);
+    long long inc = line_scan(mine, lane);
+    const long long total = line_lane(inc, 63);
+    w.share = max(line_div(total + p.target - 1, p.target), (long long)p.min_share);
+    w.u0 = j * w.share;
+    w.u1 = min(w.u0 + w.share, total);
+    if (w.u0 >= total) return false;
+    const int run = __builtin_ctzll(__ballot(inc > w.u0));
+    w.at = w.u0 - (line_lane(inc, run) - line_lane(mine, run));
+    w.seq = run;
+    if (per == 1) return true;
+    const int end = min((run + 1) * per, p.n_seqs);
+    for (int i0 = run * per; i0 < end; i0 += 64) {
+        mine = i0 + lane < end ? units_of(i0 + lane) : 0;
+        inc = line_scan(mine, lane);
+        const uint64_t over = __ballot(inc > w.at);
+        if (over != 0) {
+            const int at = __builtin_ctzll(over);
+            w.seq = i0 + at;
+            w.at -= line_lane(inc, at) - line_lane(mine, at);
+            return true;
+        }
+        w.at -= line_lane(inc, 63);
+    }
+    return false;  // not reached
+}
+// Where share `share` begins inside a tile, `in_front` of whose units lie in front of it and `behind`
+// from it on, and is the first that does: how many parts the tile has, else 0.  The
+// parts' slots: the last one of the share in front, the first of this and the later ones.
+__device__ __forceinline__ int line_parts(const LineShare& w, long long in_front, long long behind) {
+    if (in_front <= 0 || in_front > w.share) return 0;
+    return 1 + (int)((behind + w.share - 1) / w.share);
+}
+__device__ __forceinline__ int line_slot(int share, int k) { return k == 0 ? 2 * share - 1 : 2 * (share + k - 1); }
+
+// Attention of tiles of 32 rows: every tile of a sequence has its 32-key stages, and what
+// starting on one costs, as units.
+constexpr int kLineStart = 6;
+__device__ __forceinline__ int line_stages(const PagedSeq& s) { return kLineStart + key_stages(s.kn); }
+__device__ __forceinline__ long long line_units(const PagedParams& p, int i) {
+    const PagedSeq s = paged_seq(p, i);
+    return ((long long)s.qn * p.ratio + 31) / 32 * line_stages(s);
+}
+
 // A workgroup is NW waves of 32 query rows each; with KS > 1 they form KS groups that
 // take the same rows and a share of the keys each, merged through LDS at the end.
 template <int D, int NW, int KS> struct PagedCfg {
@@ -154,9 +227,10 @@ template <int D, int NW, int KS> struct PagedCfg {
 // rows of zeros.
 static __device__ const u32x4 paged_zeros[16 * 256 * 2 / 16] = {};
 
+// One tile, or the part of it from stage s0 on to s1 (of a line's: else those of it.part).
 template <bool kBF, int D, int NW, int KS>
-__global__ __launch_bounds__((PagedCfg<D, NW, KS>::kThreads), (PagedCfg<D, NW, KS>::kWavesPerSimd))
-void kf_attn_paged_kernel(PagedParams p) {
+__device__ __forceinline__ void paged_tile(const PagedParams& p, const PagedItem& it, int hk, int lane, int line_s0,
+                                           int line_s1) {
     using Cfg = PagedCfg<D, NW, KS>;
     using E = Elem<kBF>;
     using X8 = typename E::x8;
@@ -172,17 +246,8 @@ void kf_attn_paged_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(1024))) char buf0[kBuf];
     __shared__ __attribute__((aligned(1024))) char buf1[kBuf];
 
-    const int tid = threadIdx.x;
-    const int lane = tid & 63;
-    const int wave_id = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 5;
-    // KV heads next to each other: with ids dealt round-robin over the XCDs, 8
-    // heads have an XCD, and its L2, each.
-    const int hk = blockIdx.x % p.heads_kv;
-    PagedItem it;
-    // (Causal tiles see the more keys the later they are.)
-    if (!paged_find<false, true>(p, lane, blockIdx.x / p.heads_kv, it, [&](int i) { return paged_count<kRows>(p, i); }))
-        return;
     PagedSeq sq = paged_seq(p, it.seq);
     sq.q0 = __builtin_amdgcn_readfirstlane(sq.q0);
     sq.qn = __builtin_amdgcn_readfirstlane(sq.qn);
@@ -201,7 +266,8 @@ void kf_attn_paged_kernel(PagedParams p) {
     // This part's stages of those that the tile sees, and the groups' of these, as many
     // as any other's; row limits count from kv_base.
     const int seen = key_stages(blk_lim), per_part = (seen + it.parts - 1) / it.parts;
-    const int s0 = min(it.part * per_part, seen), s1 = min(s0 + per_part, seen);
+    const int s0 = min(kRows == 32 ? line_s0 : it.part * per_part, seen);
+    const int s1 = min(kRows == 32 ? line_s1 : s0 + per_part, seen);
     const int ntiles = (s1 - s0 + KS - 1) / KS;
     const int kv_base = (s0 + kgrp * ntiles) * BC, kv_end = min(min(kv_base + ntiles * BC, s1 * BC), blk_lim);
     const auto own = [&](int lim) { return min(lim, kv_end) - kv_base; };
@@ -264,7 +330,9 @@ void kf_attn_paged_kernel(PagedParams p) {
         chunk_off[i] = (((lane % kChunks) ^ SW::h(i * kRowsPerInstr + lr)) % kChunks) * 16;
     // Requests the stage that begins at key kv_base + kv0; returns which of its halves lie on
     // no valid page, bit 0 keys 0 .. 15, bit 1 the others.
-    auto issue_stage = [&](char* dst, int kv0) {
+    // kWhat: 1 K, 2 V, 3 both.
+    auto issue_stage = [&](char* dst, int kv0, auto what) {
+        constexpr int kWhat = decltype(what)::value;
         const int kv = kv_base + kv0;
         int id[2], bad = 0;
 #pragma unroll
@@ -276,6 +344,7 @@ void kf_attn_paged_kernel(PagedParams p) {
         for (int u = 0; u < kUnitsPerWave; ++u) {
             const int unit = copier * kUnitsPerWave + u, h = unit & 1;
             const bool is_v = unit >= 2;
+            if (kRowWaves == 1 && (kWhat >> (u >> 1) & 1) == 0) continue;
             const uint32_t d_lds = (uint32_t)(uintptr_t)(lds_void*)(dst + unit * (kTensorBytes / 2));
             const int key = kv + 16 * h;
             const int page = h ? id[1] : id[0];
@@ -320,7 +389,10 @@ void kf_attn_paged_kernel(PagedParams p) {
 
     char* const b0 = buf0 + kgrp * 2 * kTensorBytes;      // this group's stages
     char* const b1 = buf1 + kgrp * 2 * kTensorBytes;
-    int bad_next = issue_stage(b0, 0);
+    constexpr std::integral_constant<int, 1> kK{};
+    constexpr std::integral_constant<int, 2> kV{};
+    constexpr std::integral_constant<int, 3> kBoth{};
+    int bad_next = issue_stage(b0, 0, kBoth);
     X8 q[kNKK];
     {
         const int rc = min(w0 + (lane & 31), R - 1);
@@ -342,16 +414,20 @@ void kf_attn_paged_kernel(PagedParams p) {
         const f16x4 hi = lds_read_tr16(stage + vo1 + jj * 16 * kRowBytes);
         return __builtin_bit_cast(X8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto tile = [&](const char* stage, int t, int bad) {
-        if (t >= nt_w) return;
-        int kb = koff[0], vb = voff[0][0];
-        if constexpr (kXorOff) asm volatile("" : "+v"(kb), "+v"(vb));  // derived per tile
-        f32x16 s[1] = {f32x16{}};
+    // S of a tile, masked and rebased to the running maximum, and then O.
+    f32x16 s[1];
+    const auto scores = [&](const char* stage) {
+        int kb = koff[0];
+        if constexpr (kXorOff) asm volatile("" : "+v"(kb));  // derived per tile
+        s[0] = f32x16{};
 #pragma unroll
         for (int kk = 0; kk < kNKK; ++kk) {
             const X8 kf = *reinterpret_cast<const X8*>(stage + (kXorOff ? kb ^ (32 * kk) : koff[kk]));
             s[0] = E::mfma32(kf, q[kk], s[0]);
         }
+    };
+    X8 pp[2];
+    const auto weights = [&](int t, int bad) {
         if ((t + 1) * BC > wave_min || bad != 0) {      // keys that a row does not see -> -inf
             asm volatile("" ::: "memory");              // a branch, not selects in every tile
             const int lg = lim - t * BC - 4 * g;
@@ -359,31 +435,80 @@ void kf_attn_paged_kernel(PagedParams p) {
             for (int r = 0; r < 16; ++r)
                 if (8 * (r >> 2) + (r & 3) >= lg || (bad >> (r >> 3) & 1)) s[0][r] = -INFINITY;
         }
-        X8 pp[2];
         block_update_max<kNTD>(st, block_rowmax<1>(s), c, inv_c, o);
         // A row that has seen no key yet keeps m = -inf and must get P = 0, not NaN.
         packed_exp<kBF>(s[0], c, st.m == -INFINITY ? 0.f : -st.m, pp, st.l);
+    };
+    const auto outputs = [&](const char* stage) {
+        int vb = voff[0][0];
+        if constexpr (kXorOff) asm volatile("" : "+v"(vb));
 #pragma unroll
         for (int td = 0; td < kNTD; ++td)
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj) o[td] = E::mfma32(v_frag(stage, vb, td, jj), pp[jj], o[td]);
     };
-    for (int t0 = 0; t0 < ntiles; t0 += 2) {
+    if constexpr (kRowWaves == 1) {
+        // The wave copies its stages itself and waits for itself alone: K of the stage after the
+        // next as soon as this one's has been read, and V likewise, so that three of four
+        // half stages are on their way (64 contexts of 2048 keys, 32 / 8 heads of 128: 112 us
+        // with one stage, 108 with these).
+        constexpr int kHalf = 2 * kUnitInstr;             // copies of K or V of a stage
+        const auto landed = [](int halves) {              // but for so many younger halves
+            asm volatile("" ::: "memory");
+            const auto wait = [](auto n) {
+                constexpr int v = decltype(n)::value * kHalf;
+                static_assert(v < 64, "vmcnt");
+                __builtin_amdgcn_s_waitcnt(0x0f70 | (v & 15) | (v >> 4) << 14);
+            };
+            if (halves == 3) wait(std::integral_constant<int, 3>{});
+            else if (halves == 2) wait(std::integral_constant<int, 2>{});
+            else if (halves == 1) wait(std::integral_constant<int, 1>{});
+            else wait(std::integral_constant<int, 0>{});
+            asm volatile("" ::: "memory");
+        };
+        const auto read = [] {                            // all LDS reads have returned
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            asm volatile("" ::: "memory");
+        };
+        int bad = bad_next;
+        if (ntiles > 1) bad_next = issue_stage(b1, BC, kBoth);
+        for (int t = 0; t < ntiles; ++t) {
+            char* const stage = t & 1 ? b1 : b0;
+            const int later = min(ntiles - 1 - t, 2);     // stages behind this one, up to two
+            int bad_after = 0;
+            landed(later > 0 ? 3 : 1);
+            if (t < nt_w) scores(stage);
+            read();
+            if (later > 1) bad_after = issue_stage(stage, (t + 2) * BC, kK);
+            if (t < nt_w) weights(t, bad);
+            landed(later == 0 ? 0 : later + 1);
+            if (t < nt_w) outputs(stage);
+            read();
+            if (later > 1) issue_stage(stage, (t + 2) * BC, kV);
+            bad = bad_next;
+            bad_next = bad_after;
+        }
+    } else {
+        for (int t0 = 0; t0 < ntiles; t0 += 2) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int t = t0 + u;
-            if (t >= ntiles) break;
-            char* cur = u == 0 ? b0 : b1;
-            char* nxt = u == 0 ? b1 : b0;
-            // Stage t has landed for every wave; every wave is done with stage t - 1 (in
-            // nxt).  A wave that copies its stages itself waits for itself alone.
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-            if constexpr (kRowWaves > 1) __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            const int bad = bad_next;
-            if (t + 1 < ntiles) bad_next = issue_stage(nxt, (t + 1) * BC);
-            tile(cur, t, bad);
+            for (int u = 0; u < 2; ++u) {
+                const int t = t0 + u;
+                if (t >= ntiles) break;
+                char* cur = u == 0 ? b0 : b1;
+                char* nxt = u == 0 ? b1 : b0;
+                // Stage t has landed for every wave; every wave is done with stage t - 1 (in nxt).
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                const int bad = bad_next;
+                if (t + 1 < ntiles) bad_next = issue_stage(nxt, (t + 1) * BC, kBoth);
+                if (t >= nt_w) continue;
+                scores(cur);
+                weights(t, bad);
+                outputs(cur);
+            }
         }
     }
     if constexpr (KS > 1) {
@@ -391,8 +516,9 @@ void kf_attn_paged_kernel(PagedParams p) {
         static_assert(kRowWaves * kNTD * 4 * (KS - 1) * 1024 <= 2 * kBuf, "merge slots");
         __shared__ float merge_ml[2 * NW * 64];
         const auto slot_base = [&](int k) { return k < kBuf / 1024 ? buf0 + k * 1024 : buf1 + (k * 1024 - kBuf); };
-        p.n_splits = it.parts;
-        merge_kv_groups<D, KS, kRowWaves>(p, st, o, slot_base, merge_ml, wave, kgrp, lane, g, out_row(), part_row(),
+        AttnParams to = p;
+        to.n_splits = it.parts;
+        merge_kv_groups<D, KS, kRowWaves>(to, st, o, slot_base, merge_ml, wave, kgrp, lane, g, out_row(), part_row(),
                                           (lane & 31) < nrows);
         return;
     }
@@ -404,8 +530,9 @@ void kf_attn_paged_kernel(PagedParams p) {
         const bool none = st.rmax == -INFINITY;
         const float beta = none ? 0.f : rebase_factor(st.m, st.rmax, c);
         const size_t at = part_row();
-        p.O = p.Opart + (at - (lane & 31)) * D;
-        packed_store<kOutF32, D, 2 * kBuf / NW>(p, o, beta, mine, lane & 31, nrows, lane);
+        AttnParams to = p;
+        to.O = p.Opart + (at - (lane & 31)) * D;
+        packed_store<kOutF32, D, 2 * kBuf / NW>(to, o, beta, mine, lane & 31, nrows, lane);
         if (g == 0 && (lane & 31) < nrows) {
             p.Mpart[at] = none ? -INFINITY : st.rmax * p.scale;
             p.Lpart[at] = l * beta;
@@ -425,6 +552,51 @@ void kf_attn_paged_kernel(PagedParams p) {
         store_stats(p, at, st.rmax * p.scale, empty ? 0.f : l * rebase_factor(st.m, st.rmax, c));
 }
 
+template <bool kBF, int D, int NW, int KS>
+__global__ __launch_bounds__((PagedCfg<D, NW, KS>::kThreads), (PagedCfg<D, NW, KS>::kWavesPerSimd))
+void kf_attn_paged_kernel(PagedParams p) {
+    constexpr int kRows = PagedCfg<D, NW, KS>::kRows;
+    // KV heads next to each other: with ids dealt round-robin over the XCDs, 8
+    // heads have an XCD, and its L2, each.
+    const int hk = blockIdx.x % p.heads_kv, share = blockIdx.x / p.heads_kv;
+    int lane = threadIdx.x & 63;
+    PagedItem it;
+    if constexpr (kRows > 32) {
+        // (Causal tiles see the more keys the later they are.)
+        if (paged_find<false, true>(p, lane, share, it, [&](int i) { return paged_count<kRows>(p, i); }))
+            paged_tile<kBF, D, NW, KS>(p, it, hk, lane, 0, 0);
+    } else {
+        LineShare w;
+        if (!line_find(p, lane, share, w, [&](int i) { return line_units(p, i); })) return;
+        int seq = w.seq;
+        long long at = w.at, left = w.u1 - w.u0;
+        while (left > 0 && seq < p.n_seqs) {
+            // (An opaque lane: nothing that is derived from it lives across the tiles.)
+            lane = threadIdx.x & 63;
+            asm volatile("" : "+v"(lane));
+            const PagedSeq sq = paged_seq(p, seq);
+            const int stages = line_stages(sq);
+            const long long all = ((long long)sq.qn * p.ratio + 31) / 32 * stages;
+            if (at >= all) {
+                at -= all;
+                ++seq;
+                continue;
+            }
+            it.seq = seq;
+            it.tile = __builtin_amdgcn_readfirstlane((int)line_div(at, stages));
+            const int a = __builtin_amdgcn_readfirstlane((int)(at - (long long)it.tile * stages));
+            const int b = (int)min((long long)stages, a + left);
+            it.part = 0;
+            it.parts = b - a == stages ? 1 : 2;
+            it.slot = 2 * share + (a == 0 ? 1 : 0);
+            paged_tile<kBF, D, NW, KS>(p, it, hk, lane, max(a - kLineStart, 0), max(b - kLineStart, 0));
+            __syncthreads();  // every wave is done with the stages
+            at += b - a;
+            left -= b - a;
+        }
+    }
+}
+
 // The parts of the tiles that were cut, joined: a workgroup per tile and KV head, a
 // lane per 4 channels of a row.  O = sum_i w_i O_i / L, L = sum_i w_i l_i, w_i = exp(m_i - max m), in
 // the order of the keys; a part in which a row saw no key (m_i = -inf) wrote no O.
@@ -432,10 +604,20 @@ constexpr int kPagedMergeThreads = 256;
 template <int D, int kRows>
 __global__ __launch_bounds__(kPagedMergeThreads)
 void kf_attn_paged_merge_kernel(PagedParams p) {
-    const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv;
+    const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv, share = blockIdx.x / p.heads_kv + 1;
     PagedItem it;
-    if (!paged_find<true, true>(p, lane, blockIdx.x / p.heads_kv, it, [&](int i) { return paged_count<kRows>(p, i); }))
-        return;
+    if constexpr (kRows > 32) {
+        if (!paged_find<true, true>(p, lane, share - 1, it, [&](int i) { return paged_count<kRows>(p, i); })) return;
+    } else {
+        LineShare w;
+        if (!line_find(p, lane, share, w, [&](int i) { return line_units(p, i); })) return;
+        const int stages = line_stages(paged_seq(p, w.seq));
+        it.seq = w.seq;
+        it.tile = (int)line_div(w.at, stages);
+        const long long in_front = w.at - (long long)it.tile * stages;
+        it.parts = line_parts(w, in_front, stages - in_front);
+        if (it.parts == 0) return;
+    }
     const PagedSeq sq = paged_seq(p, it.seq);
     const int R = sq.qn * p.ratio, r0 = it.tile * kRows;
     if ((unsigned)it.tile * (unsigned)kRows >= (unsigned)R) return;
@@ -443,7 +625,9 @@ void kf_attn_paged_merge_kernel(PagedParams p) {
     constexpr int kUnroll = 4;
     for (int i = threadIdx.x; i < n; i += kPagedMergeThreads) {
         const int r = i / (D / 4), c4 = i % (D / 4) * 4;
-        const auto at = [&](int k) { return ((size_t)(it.slot + k) * p.heads_kv + hk) * kRows + r; };
+        const auto at = [&](int k) {
+            return ((size_t)(kRows > 32 ? it.slot + k : line_slot(share, k)) * p.heads_kv + hk) * kRows + r;
+        };
         float m = -INFINITY, l = 0.f;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
         for (int k0 = 0; k0 < it.parts; k0 += kUnroll) {
@@ -553,57 +737,6 @@ template <int D> struct WeighSeq {
         return lo;
     }
 };
-
-__device__ __forceinline__ long long weigh_scan(long long v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-__device__ __forceinline__ long long weigh_lane(long long v, int lane) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-    return (long long)((uint64_t)hi << 32 | lo);
-}
-
-// Share j of a KV head's units: from unit u0 of the line on, `share` of them but for the last;
-// the sequence of the first, and its place among the sequence's units.  By the lanes
-// of a wave; false past the last unit.
-struct WeighShare {
-    long long u0, u1, share, at;
-    int seq;
-};
-template <int D>
-__device__ __forceinline__ bool weigh_find(const PagedParams& p, int lane, int j, WeighShare& w) {
-    const int per = (p.n_seqs + 63) / 64, first = min(lane * per, p.n_seqs), last = min(first + per, p.n_seqs);
-    long long mine = 0;
-    for (int i = first; i < last; ++i) mine += WeighSeq<D>(p, i).units(p);
-    long long inc = weigh_scan(mine, lane);
-    const long long total = weigh_lane(inc, 63);
-    w.share = max((total + p.target - 1) / p.target, (long long)p.min_share);
-    w.u0 = j * w.share;
-    w.u1 = min(w.u0 + w.share, total);
-    if (w.u0 >= total) return false;
-    const int run = __builtin_ctzll(__ballot(inc > w.u0));
-    w.at = w.u0 - (weigh_lane(inc, run) - weigh_lane(mine, run));
-    w.seq = run;
-    if (per == 1) return true;
-    const int end = min((run + 1) * per, p.n_seqs);
-    for (int i0 = run * per; i0 < end; i0 += 64) {
-        mine = i0 + lane < end ? WeighSeq<D>(p, i0 + lane).units(p) : 0;
-        inc = weigh_scan(mine, lane);
-        const uint64_t over = __ballot(inc > w.at);
-        if (over != 0) {
-            const int at = __builtin_ctzll(over);
-            w.seq = i0 + at;
-            w.at -= weigh_lane(inc, at) - weigh_lane(mine, at);
-            return true;
-        }
-        w.at -= weigh_lane(inc, 63);
-    }
-    return false;  // not reached
-}
 
 // Runs r0 .. r1 - 1 of a step's keys.  S = Q K^T: lane l has key l % 32 and 16 of the
 // rows, the sum over which needs one exchange; of fewer rows only those groups of eight
@@ -764,10 +897,10 @@ void kf_kv_weigh_kernel(PagedParams p) {
     // Whole stages begin at a token, and their lanes' offsets from it have 32 bits.
     const bool plain = kWeighRows % ratio == 0 && kWeighRows / ratio * p.q_token + ratio * p.q_head < (1LL << 30);
     const size_t stage_bytes = (size_t)(kWeighRows / ratio) * p.q_token * 2;
-    WeighShare w;
+    LineShare w;
     {
         const int l = threadIdx.x & 63;
-        if (!weigh_find<D>(p, l, share, w)) return;
+        if (!line_find(p, l, share, w, [&](int i) { return WeighSeq<D>(p, i).units(p); })) return;
 #pragma unroll
         for (int i = 0; i < kInstr; ++i) {
             const int row = row_of(l, i), q = row / ratio;
@@ -977,16 +1110,14 @@ void kf_kv_weigh_merge_kernel(PagedParams p) {
     constexpr int kKeys = WeighCfg<D>::kKeys, kRuns = 4;
     __shared__ float sums[kRuns][kKeys];
     const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv, share = blockIdx.x / p.heads_kv + 1, sh = p.page_shift;
-    WeighShare w;
-    if (!weigh_find<D>(p, lane, share, w)) return;
+    LineShare w;
+    if (!line_find(p, lane, share, w, [&](int i) { return WeighSeq<D>(p, i).units(p); })) return;
     const WeighSeq<D> sq(p, w.seq);
     if (sq.step) return;
     const int tile = sq.tile_of(p, w.at);
     const long long in_front = w.at - sq.units(p, tile), behind = sq.units(p, tile + 1) - w.at;
-    if (in_front <= 0 || in_front > w.share) return;
-    // The block's parts: the last of the share in front, the first of this and the later ones.
-    const int parts = 1 + (int)((behind + w.share - 1) / w.share);
-    const auto slot = [&](int k) { return k == 0 ? 2 * share - 1 : 2 * (share + k - 1); };
+    const int parts = line_parts(w, in_front, behind);
+    if (parts == 0) return;
     const int at = threadIdx.x % kKeys, run = threadIdx.x / kKeys, key = tile * kKeys + at;
     const int per = (parts + kRuns - 1) / kRuns, k1 = min((run + 1) * per, parts);
     float total = 0.f;
@@ -994,7 +1125,7 @@ void kf_kv_weigh_merge_kernel(PagedParams p) {
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            v[u] = p.Opart[((size_t)slot(min(k + u, k1 - 1)) * p.heads_kv + hk) * kKeys + at];
+            v[u] = p.Opart[((size_t)line_slot(share, min(k + u, k1 - 1)) * p.heads_kv + hk) * kKeys + at];
 #pragma unroll
         for (int u = 0; u < 8; ++u) total += k + u < k1 ? v[u] : 0.f;
     }

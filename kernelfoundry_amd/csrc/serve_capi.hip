@@ -322,6 +322,13 @@ int check_paged(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size,
     return prm->kv_len > kMaxIndex ? KF_ERR_SIZE : KF_OK;
 }
 
+void paged_sizes(int D, int H_kv, PagedPlan* pl) {
+    const size_t parts = (size_t)pl->slots * H_kv * pl->rows;
+    pl->o_bytes = align_up(parts * D * sizeof(float), kWsAlign);
+    pl->s_bytes = align_up(parts * sizeof(float), kWsAlign);
+    pl->ws_bytes = pl->o_bytes + 2 * pl->s_bytes;
+}
+
 int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, int max_pages, int num_pages,
                PagedPlan* pl) {
     kf::PagedParams& prm = pl->prm;
@@ -330,6 +337,17 @@ int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, 
     const long long rows = (long long)tokens * (H_q / H_kv);
     const double avg = (double)rows / n_seqs;
     pl->rows = D == 256 ? (avg > 32 ? 128 : 32) : avg > 64 ? 128 : avg > 32 ? 64 : 32;
+    if (pl->rows == 32) {
+        // Equal shares of a line, for every workgroup that the device holds; no fewer than 8
+        // units each.
+        prm.target = std::max(1, current_device_shape().cus * (D == 64 ? 2 : 1) / H_kv);
+        prm.min_share = 8;
+        pl->items = prm.target;
+        pl->cut_tiles = prm.target - 1;
+        pl->slots = prm.target > 1 ? 2 * prm.target : 0;
+        paged_sizes(D, H_kv, pl);
+        return fits_grid(pl->items * H_kv, 256) ? KF_OK : KF_ERR_SIZE;
+    }
     const long long least = (rows + pl->rows - 1) / pl->rows;
     const long long tiles = rows / pl->rows + std::min<long long>(n_seqs, tokens);
     const long long stages = ((long long)prm.kv_len + 31) / 32;
@@ -341,10 +359,7 @@ int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, 
     pl->items = tiles + prm.target;
     pl->cut_tiles = std::min<long long>(tiles, prm.target);
     pl->slots = 2 * prm.target;
-    const size_t parts = (size_t)pl->slots * H_kv * pl->rows;
-    pl->o_bytes = align_up(parts * D * sizeof(float), kWsAlign);
-    pl->s_bytes = align_up(parts * sizeof(float), kWsAlign);
-    pl->ws_bytes = pl->o_bytes + 2 * pl->s_bytes;
+    paged_sizes(D, H_kv, pl);
     if (!fits_grid(pl->items * H_kv, 256)) return KF_ERR_SIZE;
     return KF_OK;
 }
@@ -356,7 +371,7 @@ int launch_paged(const PagedPlan& pl, hipStream_t stream) {
     (void)hipGetLastError();
     kf::kf_attn_paged_kernel<kBF, D, NW, KS>
         <<<dim3((unsigned)(pl.items * prm.heads_kv)), dim3(Cfg::kThreads), 0, stream>>>(prm);
-    if (const int st = launched(); st != KF_OK || prm.target == 0) return st;
+    if (const int st = launched(); st != KF_OK || pl.cut_tiles == 0) return st;
     kf::kf_attn_paged_merge_kernel<D, Cfg::kRows>
         <<<dim3((unsigned)(pl.cut_tiles * prm.heads_kv)), dim3(kf::kPagedMergeThreads), 0, stream>>>(prm);
     return launched();
