@@ -22,7 +22,7 @@ struct PagedParams : AttnParams {  // Q, K, V, O, Mi (LSE), scales, causal, head
     int target, min_share, unit_shift;
     const float* row_lse;          // kf_kv_weigh: [tokens_q][H_q]
     float* weights;                // kf_kv_weigh: [num_pages][H_kv][page_size]
-    int cut;                       // kf_kv_weigh: blocks of keys may be cut
+    int cut;                       // where shares cut a line: whether they cut tiles of it, too
 };
 
 // One sequence's new tokens and keys.
@@ -585,7 +585,13 @@ void kf_attn_paged_kernel(PagedParams p) {
             it.seq = seq;
             it.tile = __builtin_amdgcn_readfirstlane((int)line_div(at, stages));
             const int a = __builtin_amdgcn_readfirstlane((int)(at - (long long)it.tile * stages));
-            const int b = (int)min((long long)stages, a + left);
+            // Without a second kernel a tile goes to the share of its first unit.
+            const int b = p.cut ? (int)min((long long)stages, a + left) : stages;
+            if (!p.cut && a > 0) {
+                at += b - a;
+                left -= b - a;
+                continue;
+            }
             it.part = 0;
             it.parts = b - a == stages ? 1 : 2;
             it.slot = 2 * share + (a == 0 ? 1 : 0);

@@ -342,9 +342,11 @@ int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, 
         // units each.
         prm.target = std::max(1, current_device_shape().cus * (D == 64 ? 2 : 1) / H_kv);
         prm.min_share = 8;
+        // (Few keys: no second launch.)
+        prm.cut = prm.target > 1 && prm.kv_len > 256 ? 1 : 0;
         pl->items = prm.target;
-        pl->cut_tiles = prm.target - 1;
-        pl->slots = prm.target > 1 ? 2 * prm.target : 0;
+        pl->cut_tiles = prm.cut ? prm.target - 1 : 0;
+        pl->slots = prm.cut ? 2 * prm.target : 0;
         paged_sizes(D, H_kv, pl);
         return fits_grid(pl->items * H_kv, 256) ? KF_OK : KF_ERR_SIZE;
     }

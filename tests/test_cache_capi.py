@@ -79,7 +79,6 @@ def test_sizes(lib):  # noqa: F811
     # Grids of more threads than a launch can number.
     assert append(lib, T=1 << 27, H_kv=8, D=256) == kf.KF_ERR_SIZE
     assert evict(lib, n=1 << 22, H_kv=1) == kf.KF_ERR_SIZE
-    assert attend(lib, T=1 << 26, n=1 << 26, H_q=1, H_kv=1) == kf.KF_ERR_SIZE
 
 
 def test_flags(lib):  # noqa: F811
@@ -120,6 +119,8 @@ def test_workspaces(lib):  # noqa: F811
     assert attend(lib, ws=None) == attend(lib, ws_bytes=need - 1) == kf.KF_ERR_WORKSPACE
     assert attend(lib, ws=FAKE + 16) == kf.KF_ERR_ALIGN
     assert kf.paged_attn_workspace_bytes(2, 4, 8, 3, 128, 16, 64) == 0
+    # A share for every workgroup, however many sequences.
+    assert kf.paged_attn_workspace_bytes(1 << 26, 1 << 26, 8, 2, 128, 16, 64) == need
     # Tiles enough for the device, or few keys: none is cut.
     assert kf.paged_attn_workspace_bytes(8, 1 << 15, 32, 8, 128, 16, 1024) == 0
     assert kf.paged_attn_workspace_bytes(8, 8, 32, 8, 128, 16, 4) == 0
@@ -129,7 +130,7 @@ def test_workspaces(lib):  # noqa: F811
     assert weigh(lib, ws=None, **many) == weigh(lib, ws_bytes=need - 1, **many) == kf.KF_ERR_WORKSPACE
     assert weigh(lib, ws=FAKE + 16, **many) == kf.KF_ERR_ALIGN
     need = kf.evict_workspace_bytes(2, 2, 128, 16, 4)
-    assert need == 256 + 256 + 2 * 2 * 64 * 4
+    assert need == 256 + 2 * 2 * 64 * 4
     assert evict(lib, ws=None) == evict(lib, ws_bytes=need - 1) == kf.KF_ERR_WORKSPACE
     assert evict(lib, ws=FAKE + 16) == kf.KF_ERR_ALIGN
 
