@@ -223,11 +223,12 @@ void kf_kv_evict_select_kernel(EvictParams p) {
                 sum += (v.x + v.y) + (v.z + v.w);
             }
             int inc = wave_scan(sum);
-            const int run = __builtin_ctzll(__ballot(inc >= need));
+            // (Of weights that change meanwhile there may be none.)
+            const int run = __builtin_ctzll(__ballot(inc >= need) | 1ull << 63);
             need -= __builtin_amdgcn_readlane(inc, run) - __builtin_amdgcn_readlane(sum, run);
             sum = lane < kRun ? hist[slot((63 - run) * kRun) + kRun - 1 - lane] : 0;
             inc = wave_scan(sum);
-            const int e = __builtin_ctzll(__ballot(inc >= need));
+            const int e = __builtin_ctzll(__ballot(inc >= need) | 1ull << (kRun - 1));
             alike = __builtin_amdgcn_readlane(sum, e);
             need -= __builtin_amdgcn_readlane(inc, e) - alike;
             top |= (uint32_t)((63 - run) * kRun + kRun - 1 - e) << shift;

@@ -867,6 +867,8 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const WeighSeq<
             if (g == 0) sums[(t - t0) * 32 + lane] = add;
         }
         // The wave's own sums, two tiles at a time.
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
         for (int t = t0 + g; t < t0 + n; t += 2) {
             const int key = k0 + t * Cfg::kStepKeys + (lane & 31);
             const int id = key < sq.kn ? table[key >> sh] : -1;
@@ -1006,8 +1008,8 @@ void kf_kv_weigh_kernel(PagedParams p) {
             }
         };
         // Rows in front of `first` see no key of the wave, those in front of `whole` not all.
-        const int first = p.causal ? max(k0 - before, 0) * ratio : 0;
-        const int whole = p.causal ? max(k0 + kWaveKeys - 1 - before, 0) * ratio : 0;
+        const auto rows_to = [&](int key) { return (int)min((long long)max(key - before, 0) * ratio, (long long)R); };
+        const int first = p.causal ? rows_to(k0) : 0, whole = p.causal ? rows_to(k0 + kWaveKeys - 1) : 0;
         f32x16 sum[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) sum[t] = f32x16{};
@@ -1070,7 +1072,7 @@ void kf_kv_weigh_kernel(PagedParams p) {
             if (s + 1 < s1) issue_stage(s + 1, e_next);
             const char* const rows = buf(s);
             const int r0 = s * kWeighRows;
-            if (r0 + kWeighRows <= first) continue;
+            if (min(r0 + kWeighRows, R) <= first) continue;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) q[i] = read(rows, i);
             scores(rows, rows + 32 * kRowBytes, x, late, late_less);

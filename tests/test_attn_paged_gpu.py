@@ -124,6 +124,15 @@ def test_sequence_counts(n, long):
     run(news, before, (4, 2, 64))
 
 
+@pytest.mark.parametrize("heads", [(8, 2, 128), (300, 300, 64), (4, 2, 256)])
+@pytest.mark.parametrize("most", [250, 900])
+def test_shares_of_many_short_sequences(heads, most):
+    """Shares that begin inside tiles, several tiles and empty sequences in a share, few keys
+    and one share a KV head."""
+    news = [(7 * i) % 6 for i in range(40)]
+    run(news, [(37 * i) % (most - 10) for i in range(40)], heads)
+
+
 def test_many_sequences_of_one_token():
     run([1] * 3000, [i % 40 for i in range(3000)], (2, 1, 64))
 

@@ -151,6 +151,36 @@ def test_weights_of_a_long_prompt_of_one_kv_head():
     weigh(cache, Q, news, lse, True)
 
 
+@pytest.mark.parametrize("heads,keys,news", [
+    ((64, 64, 64), [70000, 40000, 3], [1, 2, 1]),                      # more runs of a wave than wait in LDS
+    ((32, 32, 128), [9000, 20, 9000, 500], [1, 20, 30, 400]),          # steps and chunks in a share
+    ((520, 520, 64), [300, 70, 900], [70, 1, 300]),                    # one share a KV head
+    ((16, 2, 128), [5000, 4000, 3900], [700, 0, 1000]),                # blocks that several shares cut
+    ((10, 2, 256), [1500, 1400], [37, 900])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_weights_over_shares(heads, keys, news, causal):
+    H_q, H_kv, D = heads
+    cache = ref.Cache(keys, H_kv, D, torch.float16, 16)
+    Q = queries(news, H_q, D, torch.float16)
+    _, lse = kf.attn_paged(Q, cache.K, cache.V, cache.table, ints(ref.starts_of(news)), cache.lens, causal=causal,
+                           return_lse=True)
+    weigh(cache, Q, news, lse, causal)
+
+
+def test_weights_repeat():
+    """The same sums every time."""
+    cache = ref.Cache([3000, 700, 5000], 2, 128, torch.bfloat16, 32)
+    news = [300, 1, 64]
+    Q, s = queries(news, 16, 128, torch.bfloat16), ints(ref.starts_of([300, 1, 64]))
+    _, lse = kf.attn_paged(Q, cache.K, cache.V, cache.table, s, cache.lens, causal=True, return_lse=True)
+    got = []
+    for _ in range(3):
+        w = cache.weights.clone()
+        kf.kv_weigh(Q, cache.K, w, cache.table, s, cache.lens, lse, causal=True)
+        got.append(w)
+    assert equal(got[0], got[1]) and equal(got[0], got[2])
+
+
 def test_weights_from_views_and_tokens_outside():
     cache = ref.Cache([300, 700], 2, 128, torch.float16, 16)
     x = torch.randn(60, 12 * 128, device="cuda").half()
@@ -209,6 +239,21 @@ def test_evict_ties_and_strange_weights():
     strange = torch.tensor([math.nan, math.inf, 0.0, -0.0, -math.inf, -1.0, 1e-45, -math.nan], device="cuda")
     w[page, :, row] = strange[torch.arange(400, device="cuda") % 8][:, None]
     evict(cache, [100, 270, 130, 1], 7)
+
+
+@pytest.mark.parametrize("values", [1, 2, 300])
+@pytest.mark.parametrize("wide", [0, 2000, 6000])
+def test_evict_ties_of_many_keys(values, wide):
+    """Few values among keys of many waves, in tables of up to 16384, 81920 and more places."""
+    cache = ref.Cache([5000, 3100, 1025], 2, 64, torch.float16, 16, wide=wide)
+    w = torch.randint(0, values, cache.weights.shape, generator=torch.Generator("cuda").manual_seed(values), device="cuda")
+    cache.weights.copy_(w.float() / 7 - 3)
+    evict(cache, [2100, 3000, 1], 40)
+
+
+def test_evict_more_keys_than_registers_hold():
+    cache = ref.Cache([90000, 100, 82500], 1, 64, torch.bfloat16, 64)
+    evict(cache, [30000, 90, 82400], 300)
 
 
 def test_evict_on_invalid_pages():
