@@ -603,8 +603,9 @@ void kf_attn_paged_kernel(PagedParams p) {
     }
 }
 
-// The parts of the tiles that were cut, joined: a workgroup per tile and KV head, a
-// lane per 4 channels of a row.  O = sum_i w_i O_i / L, L = sum_i w_i l_i, w_i = exp(m_i - max m), in
+// The parts of the tiles that were cut, joined: a workgroup per KV head and 32 rows of a
+// tile (32 contexts with 1 to 512 new tokens, 32 / 8 heads of 128, 9.4 us; 128 rows 18.8),
+// a lane per 4 channels of a row.  O = sum_i w_i O_i / L, L = sum_i w_i l_i, w_i = exp(m_i - max m), in
 // the order of the keys; a part in which a row saw no key (m_i = -inf) wrote no O.
 constexpr int kPagedMergeThreads = 256;
 template <int D, int kRows>
@@ -627,9 +628,10 @@ void kf_attn_paged_merge_kernel(PagedParams p) {
     const PagedSeq sq = paged_seq(p, it.seq);
     const int R = sq.qn * p.ratio, r0 = it.tile * kRows;
     if ((unsigned)it.tile * (unsigned)kRows >= (unsigned)R) return;
-    const int n = min(kRows, R - r0) * (D / 4);
     constexpr int kUnroll = 4;
-    for (int i = threadIdx.x; i < n; i += kPagedMergeThreads) {
+    // Rows 32 blockIdx.y and the next 31.
+    const int first = blockIdx.y * 32 * (D / 4), n = min(min(kRows, R - r0) * (D / 4), first + 32 * (D / 4));
+    for (int i = first + threadIdx.x; i < n; i += kPagedMergeThreads) {
         const int r = i / (D / 4), c4 = i % (D / 4) * 4;
         const auto at = [&](int k) {
             return ((size_t)(kRows > 32 ? it.slot + k : line_slot(share, k)) * p.heads_kv + hk) * kRows + r;

@@ -375,7 +375,7 @@ int launch_paged(const PagedPlan& pl, hipStream_t stream) {
         <<<dim3((unsigned)(pl.items * prm.heads_kv)), dim3(Cfg::kThreads), 0, stream>>>(prm);
     if (const int st = launched(); st != KF_OK || pl.cut_tiles == 0) return st;
     kf::kf_attn_paged_merge_kernel<D, Cfg::kRows>
-        <<<dim3((unsigned)(pl.cut_tiles * prm.heads_kv)), dim3(kf::kPagedMergeThreads), 0, stream>>>(prm);
+        <<<dim3((unsigned)(pl.cut_tiles * prm.heads_kv), Cfg::kRows / 32), dim3(kf::kPagedMergeThreads), 0, stream>>>(prm);
     return launched();
 }
 
