@@ -124,41 +124,29 @@ __device__ __forceinline__ void evict_unrolled(const F& f, std::integer_sequence
     (f(std::integral_constant<int, I>{}), ...);
 }
 
-// kPer: up to so many old keys of a thread are read once, into registers; 0: read anew by
-// every pass (65536 keys 220 us so, by four counts of 8 bits).
+constexpr int kSelectHist = (1 << 12) + 2 * (1 << 10) + 3 * 256;   // the bins of all three counts
+constexpr int kSelectMost = 80, kSelectPages = kSelectMost * kSelectThreads / 16;
+struct EvictShared {
+    __attribute__((aligned(16))) int hist[kSelectHist];
+    int pages[kSelectPages];          // of the first keys
+    int wave_sums[4][kSelectWaves];
+};
+
+// The cut of one head from n to m keys.  kPer: up to so many old keys of a thread are read
+// once, into registers; 0: read anew by every pass.
 template <int kPer>
-__global__ __launch_bounds__(kSelectThreads)
-void kf_kv_evict_select_kernel(EvictParams p) {
-    constexpr int kHeld = kPer > 0 ? kPer : 1, kPages = kHeld * kSelectThreads / 16;
-    static_assert(kHeld == 1 || kHeld % kSelectAhead == 0, "whole batches");
-    constexpr int kHist = (1 << 12) + 2 * (1 << 10) + 3 * 256;
-    __shared__ __attribute__((aligned(16))) int hist[kHist];   // of all three counts
-    __shared__ int pages[kPages];     // of the old keys
-    __shared__ int wave_sums[4][kSelectWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int grp = blockIdx.x, b = grp / p.heads, head = grp % p.heads;
-    const EvictTable tb{p.block_table + (size_t)b * p.max_pages, p.heads, head, p.page_shift};
-    const int n = min(max(p.kv_lens[b], 0), p.capacity), m = min(max(p.budgets[b], 0), n);
-    for (int i = tid; i < kHist; i += kSelectThreads) hist[i] = 0;
-    // A key on no valid page has no place: the sequence is left as it is.
-    bool bad = false;
-    if (m < n)
-        for (int i = tid; i <= (n - 1) >> p.page_shift; i += kSelectThreads) {
-            const int id = tb.table[i];
-            bad |= (unsigned)id >= (unsigned)p.num_pages;
-            if (kPer > 0 && i < kPages) pages[i] = id;
-        }
-    const bool left = __syncthreads_or(bad) != 0 || m == n;
+__device__ __forceinline__ void evict_select(const EvictParams& p, const EvictTable& tb, EvictShared& sh, int grp, int n, int m) {
+    constexpr int kHeld = kPer > 0 ? kPer : 1;
+    static_assert(kPer <= kSelectMost && (kHeld == 1 || kHeld % kSelectAhead == 0), "whole batches");
+    int* const hist = sh.hist;
+    const int* const pages = sh.pages;
+    auto& wave_sums = sh.wave_sums;
+    // (Opaque: nothing that is derived from it is made for the forms that are not taken.)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = min(p.recent, m), k = m - r, old = n - r;
     int* const cuts = p.cuts + 4 * (size_t)grp;
-    if (tid == 0) {
-        cuts[0] = n;
-        cuts[1] = m;
-        if (left) cuts[2] = -1;
-    }
-    // (kept may be the array that the other heads' workgroups still read: the mover
-    // writes it.)
-    if (left) return;
     // Every wave has a run of the old keys, 64 at a time.
     const int its = (old + kSelectThreads - 1) / kSelectThreads, i0 = wave * its * 64;
     const auto place = [&](int i) { return i0 + 64 * i + lane; };
@@ -303,6 +291,45 @@ void kf_kv_evict_select_kernel(EvictParams p) {
         cuts[2] = count;
         cuts[3] = min(all_near, count);
     }
+}
+
+// By how many old keys a thread has: up to 16 or 80 in registers (4097 keys of 256 heads 13.3 us
+// by 16 and 22.5 by 80, whose passes step over what they do not need; 65537 keys of one head 62,
+// and 135 without registers).
+__global__ __launch_bounds__(kSelectThreads)
+void kf_kv_evict_select_kernel(EvictParams p) {
+    __shared__ EvictShared sh;
+    const int tid = threadIdx.x;
+    const int grp = blockIdx.x, b = grp / p.heads, head = grp % p.heads;
+    const EvictTable tb{p.block_table + (size_t)b * p.max_pages, p.heads, head, p.page_shift};
+    const int n = __builtin_amdgcn_readfirstlane(min(max(p.kv_lens[b], 0), p.capacity));
+    const int m = __builtin_amdgcn_readfirstlane(min(max(p.budgets[b], 0), n));
+    for (int i = tid; i < kSelectHist; i += kSelectThreads) sh.hist[i] = 0;
+    // A key on no valid page has no place: the sequence is left as it is.
+    bool bad = false;
+    if (m < n)
+        for (int i = tid; i <= (n - 1) >> p.page_shift; i += kSelectThreads) {
+            const int id = tb.table[i];
+            bad |= (unsigned)id >= (unsigned)p.num_pages;
+            if (i < kSelectPages) sh.pages[i] = id;
+        }
+    const bool left = __syncthreads_or(bad) != 0 || m == n;
+    int* const cuts = p.cuts + 4 * (size_t)grp;
+    if (tid == 0) {
+        cuts[0] = n;
+        cuts[1] = m;
+        if (left) cuts[2] = -1;
+    }
+    // (kept may be the array that the other heads' workgroups still read: the mover
+    // writes it.)
+    if (left) return;
+    const int per = (n - min(p.recent, m) + kSelectThreads - 1) / kSelectThreads;
+    if (per <= 16)
+        evict_select<16>(p, tb, sh, grp, n, m);
+    else if (per <= kSelectMost)
+        evict_select<kSelectMost>(p, tb, sh, grp, n, m);
+    else
+        evict_select<0>(p, tb, sh, grp, n, m);
 }
 
 // Keys from below the new end m have to be read before the last r are written over them:

@@ -500,12 +500,7 @@ int launch_evict(const kf::EvictParams& prm, hipStream_t stream) {
     const int groups = prm.n_seqs * prm.heads;
     const dim3 grid(groups), block(kf::kSelectThreads);
     (void)hipGetLastError();
-    if (prm.capacity <= 16 * kf::kSelectThreads)
-        kf::kf_kv_evict_select_kernel<16><<<grid, block, 0, stream>>>(prm);
-    else if (prm.capacity <= 80 * kf::kSelectThreads)
-        kf::kf_kv_evict_select_kernel<80><<<grid, block, 0, stream>>>(prm);
-    else
-        kf::kf_kv_evict_select_kernel<0><<<grid, block, 0, stream>>>(prm);
+    kf::kf_kv_evict_select_kernel<<<grid, block, 0, stream>>>(prm);
     if (const int st = launched(); st != KF_OK) return st;
     kf::kf_kv_evict_move_kernel<D><<<dim3(groups * (D / 32 + prm.parts)), dim3(kf::kMoveThreads), 0, stream>>>(prm);
     return launched();
