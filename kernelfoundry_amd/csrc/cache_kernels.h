@@ -5,6 +5,8 @@
 // [num_pages][H_kv][page_size] in fp32.
 #pragma once
 
+#include <utility>
+
 #include "kv4_kernels.h"
 
 namespace kf {
@@ -112,7 +114,6 @@ __device__ __forceinline__ uint32_t evict_order(uint32_t u) {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kSelectAhead = 16;      // weights of a thread on their way at a time
 
 // Bits of lanes below this one.
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
@@ -125,7 +126,7 @@ __device__ __forceinline__ void evict_unrolled(const F& f, std::integer_sequence
 }
 
 constexpr int kSelectHist = (1 << 12) + 2 * (1 << 10) + 3 * 256;   // the bins of all three counts
-constexpr int kSelectMost = 80, kSelectPages = kSelectMost * kSelectThreads / 16;
+constexpr int kSelectMost = 72, kSelectPages = kSelectMost * kSelectThreads / 16;
 struct EvictShared {
     __attribute__((aligned(16))) int hist[kSelectHist];
     int pages[kSelectPages];          // of the first keys
@@ -136,8 +137,8 @@ struct EvictShared {
 // once, into registers; 0: read anew by every pass.
 template <int kPer>
 __device__ __forceinline__ void evict_select(const EvictParams& p, const EvictTable& tb, EvictShared& sh, int grp, int n, int m) {
-    constexpr int kHeld = kPer > 0 ? kPer : 1;
-    static_assert(kPer <= kSelectMost && (kHeld == 1 || kHeld % kSelectAhead == 0), "whole batches");
+    constexpr int kHeld = kPer > 0 ? kPer : 1, kSelectAhead = 8;   // weights of a thread on their way at a time
+    static_assert(kPer <= kSelectMost && kPer % kSelectAhead == 0, "whole batches");
     int* const hist = sh.hist;
     const int* const pages = sh.pages;
     auto& wave_sums = sh.wave_sums;
@@ -293,8 +294,8 @@ __device__ __forceinline__ void evict_select(const EvictParams& p, const EvictTa
     }
 }
 
-// By how many old keys a thread has: up to 16 or 80 in registers (4097 keys of 256 heads 13.3 us
-// by 16 and 22.5 by 80, whose passes step over what they do not need; 65537 keys of one head 62,
+// By how many old keys a thread has: up to 16 or 72 in registers (4097 keys of 256 heads 13.3 us
+// by 16 and 22.5 by 80 once, whose passes step over what they do not need; 65537 keys of one head 62,
 // and 135 without registers).
 __global__ __launch_bounds__(kSelectThreads)
 void kf_kv_evict_select_kernel(EvictParams p) {

@@ -61,8 +61,8 @@ struct PagedItem {
 // parts come out, and 2 target of tiles that are cut: more than one part means more
 // than `share` units, and fewer than twice as many parts as shares.  Up to 64 sequences have a
 // lane each, of more a lane has a run of consecutive ones.  kCut: j counts the tiles
-// that are cut, not the parts.  kLastFirst: a sequence's last tiles come first.
-template <bool kCut, bool kLastFirst, class CountOf>
+// that are cut, not the parts; of the parts, a sequence's last tiles, which see the most keys, come first.
+template <bool kCut, class CountOf>
 __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j, PagedItem& it, const CountOf& count) {
     using Count = PagedCount;
     const int per = (p.n_seqs + 63) / 64, first = min(lane * per, p.n_seqs), last = min(first + per, p.n_seqs);
@@ -131,7 +131,7 @@ __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j
         it.tile = left;
     } else {
         it.part = left % it.parts;
-        it.tile = kLastFirst ? tiles - 1 - left / it.parts : left / it.parts;
+        it.tile = tiles - 1 - left / it.parts;
     }
     it.slot = slot + it.tile * it.parts + it.part;
     // (Of starts in no order the sums may wrap: no partial outside the workspace.)
@@ -565,8 +565,7 @@ void kf_attn_paged_kernel(PagedParams p) {
     int lane = threadIdx.x & 63;
     PagedItem it;
     if constexpr (kRows > 32) {
-        // (Causal tiles see the more keys the later they are.)
-        if (paged_find<false, true>(p, lane, share, it, [&](int i) { return paged_count<kRows>(p, i); }))
+        if (paged_find<false>(p, lane, share, it, [&](int i) { return paged_count<kRows>(p, i); }))
             paged_tile<kBF, D, NW, KS>(p, it, hk, lane, 0, 0);
     } else {
         LineShare w;
@@ -617,7 +616,7 @@ void kf_attn_paged_merge_kernel(PagedParams p) {
     const int lane = threadIdx.x & 63, hk = blockIdx.x % p.heads_kv, share = blockIdx.x / p.heads_kv + 1;
     PagedItem it;
     if constexpr (kRows > 32) {
-        if (!paged_find<true, true>(p, lane, share - 1, it, [&](int i) { return paged_count<kRows>(p, i); })) return;
+        if (!paged_find<true>(p, lane, share - 1, it, [&](int i) { return paged_count<kRows>(p, i); })) return;
     } else {
         LineShare w;
         if (!line_find(p, lane, share, w, [&](int i) { return line_units(p, i); })) return;

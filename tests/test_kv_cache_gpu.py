@@ -244,7 +244,7 @@ def test_evict_ties_and_strange_weights():
 @pytest.mark.parametrize("values", [1, 2, 300])
 @pytest.mark.parametrize("wide", [0, 2000, 6000])
 def test_evict_ties_of_many_keys(values, wide):
-    """Few values among keys of many waves, in tables of up to 16384, 81920 and more places."""
+    """Few values among keys of many waves, in tables of different sizes."""
     cache = ref.Cache([5000, 3100, 1025], 2, 64, torch.float16, 16, wide=wide)
     w = torch.randint(0, values, cache.weights.shape, generator=torch.Generator("cuda").manual_seed(values), device="cuda")
     cache.weights.copy_(w.float() / 7 - 3)
