@@ -25,8 +25,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # Packed-fp32 VALU ops are kept out of every code object (-packed-fp32-ops).
 # -fno-honor-nans lets fmaxf skip NaN canonicalisation of MFMA results: the
-# kernels never produce or test NaN from finite inputs, and promise nothing
-# for a NaN among them.  Infinities keep their IEEE meaning, which the -inf
+# kernels never produce NaN from finite inputs.  Comparisons of floats count
+# on none, so what depends on whether a value is NaN is decided by its bits,
+# loaded as an integer (of a float loaded as one the compiler compares the float
+# again).  Infinities keep their IEEE meaning, which the -inf
 # score masking relies on.
 DEVICE_FLAGS = [
     f"--offload-arch={ARCH}",

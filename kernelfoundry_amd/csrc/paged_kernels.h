@@ -20,7 +20,7 @@ struct PagedParams : AttnParams {  // Q, K, V, O, Mi (LSE), scales, causal, head
     // paged_find): `target` parts of a KV head are aimed at (0: no cuts), none smaller
     // than min_share units.
     int target, min_share, unit_shift;
-    const float* row_lse;          // kf_kv_weigh: [tokens_q][H_q]
+    const uint32_t* row_lse;       // kf_kv_weigh: [tokens_q][H_q], bits of fp32
     float* weights;                // kf_kv_weigh: [num_pages][H_kv][page_size]
     int cut;                       // where shares cut a line: whether they cut tiles of it, too
 };
@@ -751,6 +751,12 @@ template <int D> struct WeighSeq {
     }
 };
 
+// A row's log-sum-exp, as bits: the compiler takes comparisons of floats to have no NaN.  -inf, of a
+// row without keys; NaN; and what the row's exponents are less by.
+__device__ __forceinline__ bool lse_none(uint32_t e) { return e == 0xff800000u; }
+__device__ __forceinline__ bool lse_nan(uint32_t e) { return (e & 0x7fffffffu) > 0x7f800000u; }
+__device__ __forceinline__ float lse_less(uint32_t e) { return -__uint_as_float(e) * kLog2e; }
+
 // Runs r0 .. r1 - 1 of a step's keys.  S = Q K^T: lane l has key l % 32 and 16 of the
 // rows, the sum over which needs one exchange; of fewer rows only those groups of eight
 // that there are have exponentials.  Every wave copies its own stages, 32 keys or half of
@@ -812,11 +818,12 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const WeighSeq<
 #pragma unroll
         for (int kk = 0; kk < kNKK; ++kk) q[kk] = *reinterpret_cast<const X8*>(Qr + (2 * kk + g) * 8);
     }
-    const float e = p.row_lse[((size_t)(sq.q0 + row / ratio) * p.heads_kv + hk) * ratio + row % ratio];
+    const uint32_t e = p.row_lse[((size_t)(sq.q0 + row / ratio) * p.heads_kv + hk) * ratio + row % ratio];
 #pragma unroll
     for (int s = 0; s < Cfg::kRing - 1; ++s)
         if (s < nst) issue(s);
-    const float less_row = (lane & 31) < R && e > -INFINITY ? -e * kLog2e : -INFINITY;
+    // (NaN stays NaN: the weights of keys that a row does not see are 0 whatever they would be.)
+    const float less_row = (lane & 31) >= R || lse_none(e) ? -INFINITY : __uint_as_float(lse_nan(e) ? e : __float_as_uint(lse_less(e)));
     float less[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) less[r] = __shfl(less_row, 8 * (r >> 2) + (r & 3) + 4 * g);
@@ -989,18 +996,18 @@ void kf_kv_weigh_kernel(PagedParams p) {
             koff[kk] = r * kRowBytes + (((2 * kk + g) ^ SW::h(r)) % kChunks) * 16;
         }
         const char* const Qh = reinterpret_cast<const char*>(p.Q + (size_t)sq.q0 * p.q_token + (size_t)hk * ratio * p.q_head);
-        const float* const lse = p.row_lse + ((size_t)sq.q0 * p.heads_kv + hk) * ratio;
+        const uint32_t* const lse = p.row_lse + ((size_t)sq.q0 * p.heads_kv + hk) * ratio;
         const uint32_t lse_off = (uint32_t)(lane / ratio * p.heads_kv * ratio + lane % ratio) * 4;
         // Requests a stage, and the log-sum-exp of a row of it.  (Other stages than whole ones
         // from an opaque lane.)
-        const auto issue_stage = [&](int s, float& e) {
+        const auto issue_stage = [&](int s, uint32_t& e) {
             const int r0 = s * kWeighRows;
             const uint32_t d_lds = (uint32_t)(uintptr_t)(lds_void*)(buf(s) + wave * kInstr * 1024);
             if (plain && r0 + kWeighRows <= R) {
                 const char* const src = Qh + s * stage_bytes;
 #pragma unroll
                 for (int i = 0; i < kInstr; ++i) lds_copy16(d_lds + i * 1024, src, off[i][threadIdx.x]);
-                e = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(lse + (size_t)r0 * p.heads_kv) + lse_off);
+                e = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(lse + (size_t)r0 * p.heads_kv) + lse_off);
             } else {
                 int l = lane;
                 asm volatile("" : "+v"(l));
@@ -1047,8 +1054,18 @@ void kf_kv_weigh_kernel(PagedParams p) {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // Keys that a row does not see -> -inf.
-        const auto hide = [&](f32x16 (&x)[kTiles], int r0) {
+        // The rows `half` of the 64 that lane l has row l's log-sum-exp e of: those whose e is NaN, as
+        // `strange` says, -> NaN, and then keys that a row does not see -> -inf.
+        const auto hide = [&](f32x16 (&x)[kTiles], int r0, uint64_t strange, uint32_t e, int half) {
+            if (strange != 0) {
+                asm volatile("" ::: "memory");
+                const uint32_t mine = __shfl(e, 32 * half + (lane & 31));
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        x[t][r] = __uint_as_float(lse_nan(mine) ? mine : __float_as_uint(x[t][r]));
+            }
             if (r0 >= whole) return;
             asm volatile("" ::: "memory");                        // a branch, not selects in every tile
             const int lim = min(r0 + (lane & 31), R - 1) / ratio + before + 1 - k0 - 4 * g;
@@ -1058,12 +1075,7 @@ void kf_kv_weigh_kernel(PagedParams p) {
                 for (int r = 0; r < 16; ++r)
                     if (32 * t + 8 * (r >> 2) + (r & 3) >= lim) x[t][r] = -INFINITY;
         };
-        // What the exponents of a row are less by; rows past the last, and those without a key,
-        // add nothing.
-        const auto less_of = [&](float e, int r0) {
-            return r0 + (lane & 31) < R && e > -INFINITY ? -e * kLog2e : -INFINITY;
-        };
-        float e_next = 0.f;
+        uint32_t e_next = 0;
         if (s0 < s1) issue_stage(s0, e_next);
         // The second half's scores wait for their exponentials until the next products.
         f32x16 x[kTiles], late[kTiles];
@@ -1075,18 +1087,23 @@ void kf_kv_weigh_kernel(PagedParams p) {
             __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            const float e = e_next;
+            const uint32_t e = e_next;
             if (s + 1 < s1) issue_stage(s + 1, e_next);
             const char* const rows = buf(s);
             const int r0 = s * kWeighRows;
             if (min(r0 + kWeighRows, R) <= first) continue;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) q[i] = read(rows, i);
+            // What the exponents of the stage's row `lane` are less by; rows past the last, and those without
+            // a key, add nothing.  (A NaN is in the scores that the row sees: here it would reach all.)
+            const uint64_t strange = __ballot(lse_nan(e));
+            float less = r0 + lane >= R || lse_none(e) ? -INFINITY : lse_less(e);
+            if (strange != 0) less = lse_nan(e) ? 0.f : less;
             scores(rows, rows + 32 * kRowBytes, x, late, late_less);
-            hide(x, r0);
-            scores(rows + 32 * kRowBytes, nullptr, late, x, less_of(__shfl(e, lane & 31), r0));
-            hide(late, r0 + 32);
-            late_less = less_of(__shfl(e, 32 + (lane & 31)), r0 + 32);
+            hide(x, r0, strange, e, 0);
+            scores(rows + 32 * kRowBytes, nullptr, late, x, __shfl(less, lane & 31));
+            hide(late, r0 + 32, strange, e, 1);
+            late_less = __shfl(less, 32 + (lane & 31));
         }
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)

@@ -812,7 +812,7 @@ int kf_kv_weigh(const void* Q, const int64_t* strides, const void* K_pages, floa
     }
     set_paged(pl.prm, Q, strides, K_pages, block_table, seq_starts, kv_lens, n_seqs, tokens, H_q, H_kv, D,
               max_pages_per_seq, num_pages, flags);
-    pl.prm.row_lse = lse;
+    pl.prm.row_lse = reinterpret_cast<const uint32_t*>(lse);
     pl.prm.weights = weights;
     pl.prm.Opart = static_cast<float*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
