@@ -752,9 +752,11 @@ template <int D> struct WeighSeq {
 };
 
 // A row's log-sum-exp, as bits: the compiler takes comparisons of floats to have no NaN.  -inf, of a
-// row without keys; NaN; and what the row's exponents are less by.
+// row that adds nothing whatever it and the keys hold; NaN; neither a number nor +inf; and what the
+// row's exponents are less by.
 __device__ __forceinline__ bool lse_none(uint32_t e) { return e == 0xff800000u; }
 __device__ __forceinline__ bool lse_nan(uint32_t e) { return (e & 0x7fffffffu) > 0x7f800000u; }
+__device__ __forceinline__ bool lse_strange(uint32_t e) { return lse_none(e) || lse_nan(e); }
 __device__ __forceinline__ float lse_less(uint32_t e) { return -__uint_as_float(e) * kLog2e; }
 
 // Runs r0 .. r1 - 1 of a step's keys.  S = Q K^T: lane l has key l % 32 and 16 of the
@@ -822,12 +824,19 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const WeighSeq<
 #pragma unroll
     for (int s = 0; s < Cfg::kRing - 1; ++s)
         if (s < nst) issue(s);
-    // (NaN stays NaN: the weights of keys that a row does not see are 0 whatever they would be.)
-    const float less_row = (lane & 31) >= R || lse_none(e) ? -INFINITY : __uint_as_float(lse_nan(e) ? e : __float_as_uint(lse_less(e)));
+    // (NaN stays NaN: the weights of keys that a row does not see, and those of rows that add nothing,
+    // are 0 whatever they would be.)
+    const float less_row = (lane & 31) >= R ? -INFINITY : __uint_as_float(lse_nan(e) ? e : __float_as_uint(lse_less(e)));
+    // The last key to which a row adds something: all of them up to one, or none.
+    const int last_row = lse_none(e) ? -1 : p.causal ? sq.before() + (lane & 31) / ratio : sq.kn;
+    const int clear = __any(lse_none(e)) ? 0 : p.causal ? sq.before() + 1 : INT_MAX;   // in front of it all rows do
     float less[16];
+    int last[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) less[r] = __shfl(less_row, 8 * (r >> 2) + (r & 3) + 4 * g);
-    const int before = sq.before();
+    for (int r = 0; r < 16; ++r) {
+        less[r] = __shfl(less_row, 8 * (r >> 2) + (r & 3) + 4 * g);
+        last[r] = __shfl(last_row, 8 * (r >> 2) + (r & 3) + 4 * g);
+    }
     int koff[kStageKK];
 #pragma unroll
     for (int kk = 0; kk < kStageKK; ++kk) {
@@ -859,9 +868,8 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const WeighSeq<
                 for (int kk = 0; kk < kStageKK; ++kk)
                     x = E::mfma32(q[hf * kStageKK + kk], *reinterpret_cast<const X8*>(stage + koff[kk]), x);
             }
-            // Where row 0 does not see the last key of the tile rows have limits.
             const int kt = k0 + t * Cfg::kStepKeys, key = kt + (lane & 31);
-            const bool whole = !p.causal || kt + 32 <= before + 1;
+            const bool whole = kt + 31 < clear;
             float add = 0.f;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -873,7 +881,7 @@ __device__ __forceinline__ void weigh_step(const PagedParams& p, const WeighSeq<
                     asm volatile("" ::: "memory");       // a branch, not selects in every tile
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (key > before + (8 * b + 4 * g + i) / ratio) w[i] = 0.f;
+                        if (key > last[4 * b + i]) w[i] = 0.f;
                 }
                 add += (w[0] + w[1]) + (w[2] + w[3]);
             }
@@ -1054,17 +1062,17 @@ void kf_kv_weigh_kernel(PagedParams p) {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // The rows `half` of the 64 that lane l has row l's log-sum-exp e of: those whose e is NaN, as
-        // `strange` says, -> NaN, and then keys that a row does not see -> -inf.
-        const auto hide = [&](f32x16 (&x)[kTiles], int r0, uint64_t strange, uint32_t e, int half) {
-            if (strange != 0) {
+        // The rows `half` of the 64 that lane l has row l's log-sum-exp e of: where e is NaN or -inf
+        // (`strange`: there are such) -> e, and then keys that a row does not see -> -inf.
+        const auto hide = [&](f32x16 (&x)[kTiles], int r0, bool strange, uint32_t e, int half) {
+            if (strange) {
                 asm volatile("" ::: "memory");
                 const uint32_t mine = __shfl(e, 32 * half + (lane & 31));
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        x[t][r] = __uint_as_float(lse_nan(mine) ? mine : __float_as_uint(x[t][r]));
+                        x[t][r] = __uint_as_float(lse_strange(mine) ? mine : __float_as_uint(x[t][r]));
             }
             if (r0 >= whole) return;
             asm volatile("" ::: "memory");                        // a branch, not selects in every tile
@@ -1094,11 +1102,11 @@ void kf_kv_weigh_kernel(PagedParams p) {
             if (min(r0 + kWeighRows, R) <= first) continue;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) q[i] = read(rows, i);
-            // What the exponents of the stage's row `lane` are less by; rows past the last, and those without
-            // a key, add nothing.  (A NaN is in the scores that the row sees: here it would reach all.)
-            const uint64_t strange = __ballot(lse_nan(e));
-            float less = r0 + lane >= R || lse_none(e) ? -INFINITY : lse_less(e);
-            if (strange != 0) less = lse_nan(e) ? 0.f : less;
+            // What the exponents of the stage's row `lane` are less by; rows past the last add nothing.  (NaN
+            // and -inf are in the scores that the row sees: here a NaN would reach all.)
+            const bool strange = __any(lse_strange(e));
+            float less = r0 + lane >= R ? -INFINITY : lse_less(e);
+            if (strange) less = lse_strange(e) ? 0.f : less;
             scores(rows, rows + 32 * kRowBytes, x, late, late_less);
             hide(x, r0, strange, e, 0);
             scores(rows + 32 * kRowBytes, nullptr, late, x, __shfl(less, lane & 31));

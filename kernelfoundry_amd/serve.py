@@ -585,7 +585,7 @@ def kv_weigh(Q, K_pages, weights, block_table, seq_starts, kv_lens, lse, *, caus
     weights[j] (float32 [num_pages, H_kv, page_size], by the pages of the keys) += the sum of
     exp(q . k_j / sqrt(D) - lse) over the tokens that see key j and the query heads of
     its KV head.  ``lse`` float32 [T, H_q] as attn_paged returns it (a row of -inf adds
-    nothing), the other arguments as attn_paged's.  Sequences must not share pages.
+    nothing, whatever it holds), the other arguments as attn_paged's.  Sequences must not share pages.
     ``workspace``: a buffer of weigh_workspace_bytes to use instead of a new one.
     """
     import torch

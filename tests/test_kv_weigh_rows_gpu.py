@@ -73,3 +73,30 @@ def test_nan_in_every_row():
         assert torch.isnan(got[page, :, row]).all()
         want[page, :, row] = got[page, :, row]
     assert equal(got, want)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("news,before", MIXES)
+def test_rows_of_minus_infinity_add_nothing(heads, dtype, causal, news, before):
+    """Whatever they hold themselves."""
+    call = Call(heads, dtype, news, before, causal)
+    lse, Q = call.lse.clone(), call.Q.clone()
+    for k, (b, i, h) in enumerate(call.rows()):
+        lse[call.starts[b] + i, h] = -math.inf
+        Q[call.starts[b] + i, h] = [math.nan, math.inf, -math.inf][k % 3]
+        Q[call.starts[b] + i, h, ::2] = 1.0
+    want = call(lse=lse)
+    assert torch.isfinite(want).all() and equal(call(Q=Q, lse=lse), want)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("news,before", MIXES)
+def test_rows_of_minus_infinity_add_nothing_to_strange_keys(heads, news, before):
+    """No row adds anything: keys that hold NaN and infinities keep their weights."""
+    call = Call(heads, torch.bfloat16, news, before, True)
+    K = call.cache.K.clone()
+    K[..., 3] = math.nan
+    K[:, :, ::3, 5] = math.inf
+    assert equal(call(K=K, lse=torch.full_like(call.lse, -math.inf)), call.cache.weights)
