@@ -7,6 +7,8 @@
 // token major: row r of a sequence is query r / ratio of group head r % ratio.
 #pragma once
 
+#include <cfloat>
+
 #include "elem.h"
 #include "packed_kernels.h"
 
@@ -757,6 +759,7 @@ template <int D> struct WeighSeq {
 __device__ __forceinline__ bool lse_none(uint32_t e) { return e == 0xff800000u; }
 __device__ __forceinline__ bool lse_nan(uint32_t e) { return (e & 0x7fffffffu) > 0x7f800000u; }
 __device__ __forceinline__ bool lse_strange(uint32_t e) { return lse_none(e) || lse_nan(e); }
+constexpr uint32_t kLseLow = 0xff300000u;   // -2.34e38; from -2.36e38 down lse_less passes fp32's range
 __device__ __forceinline__ float lse_less(uint32_t e) { return -__uint_as_float(e) * kLog2e; }
 
 // Runs r0 .. r1 - 1 of a step's keys.  S = Q K^T: lane l has key l % 32 and 16 of the
@@ -1063,7 +1066,7 @@ void kf_kv_weigh_kernel(PagedParams p) {
             }
         };
         // The rows `half` of the 64 that lane l has row l's log-sum-exp e of: where e is NaN or -inf
-        // (`strange`: there are such) -> e, and then keys that a row does not see -> -inf.
+        // (`strange`: there may be such) -> e, and then keys that a row does not see -> -inf.
         const auto hide = [&](f32x16 (&x)[kTiles], int r0, bool strange, uint32_t e, int half) {
             if (strange) {
                 asm volatile("" ::: "memory");
@@ -1104,9 +1107,9 @@ void kf_kv_weigh_kernel(PagedParams p) {
             for (int i = 0; i < kAhead; ++i) q[i] = read(rows, i);
             // What the exponents of the stage's row `lane` are less by; rows past the last add nothing.  (NaN
             // and -inf are in the scores that the row sees: here a NaN would reach all.)
-            const bool strange = __any(lse_strange(e));
+            const bool strange = __any(e >= kLseLow || lse_nan(e));
             float less = r0 + lane >= R ? -INFINITY : lse_less(e);
-            if (strange) less = lse_strange(e) ? 0.f : less;
+            if (strange) less = lse_strange(e) ? 0.f : fminf(less, FLT_MAX);   // -inf + inf would be NaN
             scores(rows, rows + 32 * kRowBytes, x, late, late_less);
             hide(x, r0, strange, e, 0);
             scores(rows + 32 * kRowBytes, nullptr, late, x, __shfl(less, lane & 31));

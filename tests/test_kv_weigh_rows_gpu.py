@@ -100,3 +100,62 @@ def test_rows_of_minus_infinity_add_nothing_to_strange_keys(heads, news, before)
     K[..., 3] = math.nan
     K[:, :, ::3, 5] = math.inf
     assert equal(call(K=K, lse=torch.full_like(call.lse, -math.inf)), call.cache.weights)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("value", [torch.finfo(torch.float32).min, -2.4e38, -1e30, 1e30, torch.finfo(torch.float32).max,
+                                   math.inf])
+@pytest.mark.parametrize("news,before", MIXES)
+def test_extreme_rows(heads, causal, value, news, before):
+    """exp(score - lse) is infinite, or 0; keys that the row does not see get nothing."""
+    call = Call(heads, torch.float16, news, before, causal)
+    want = call()
+    for b, i, h in call.rows():
+        lse = call.lse.clone()
+        lse[call.starts[b] + i, h] = value
+        got, expect = call(lse=lse), want.clone()
+        page, row = call.seen(b, i)
+        at = got[page, h // call.ratio, row]
+        assert (torch.isposinf(at) if value < 0 else torch.isfinite(at)).all(), (b, i, h)
+        expect[page, h // call.ratio, row] = at
+        assert equal(got, expect), (b, i, h)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("news,before", MIXES)
+def test_strange_queries_reach_the_keys_that_the_row_sees(heads, causal, value, news, before):
+    """One channel of a row with an ordinary log-sum-exp."""
+    call = Call(heads, torch.bfloat16, news, before, causal)
+    want = call()
+    for b, i, h in call.rows():
+        if not math.isfinite(float(call.lse[call.starts[b] + i, h])):
+            continue
+        Q = call.Q.clone()
+        Q[call.starts[b] + i, h, 7] = value
+        got, expect = call(Q=Q), want.clone()
+        page, row = call.seen(b, i)
+        at = got[page, h // call.ratio, row]
+        assert math.isinf(value) or torch.isnan(at).all(), (b, i, h)
+        expect[page, h // call.ratio, row] = at
+        assert equal(got, expect), (b, i, h)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("news,before", MIXES)
+def test_strange_keys_change_their_own_weight_alone(heads, news, before):
+    call = Call(heads, torch.bfloat16, news, before, True)
+    K, want = call.cache.K.clone(), call()
+    odd = torch.zeros_like(call.cache.weights, dtype=torch.bool)
+    for b, n in enumerate(call.cache.keys):
+        page, row = call.cache.slots(b, range(0, n, 7))
+        K[page, :, row, 3], odd[page, :, row] = math.nan, True
+        page, row = call.cache.slots(b, range(3, n, 14))
+        K[page, :, row, 9], odd[page, :, row] = math.inf, True
+    got = call(K=K)
+    assert equal(torch.where(odd, 0.0, got), torch.where(odd, 0.0, want))
+    for b, n in enumerate(call.cache.keys):
+        page, row = call.cache.slots(b, range(0, n, 7))
+        assert torch.isnan(got[page, :, row]).all()
