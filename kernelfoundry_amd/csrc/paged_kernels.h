@@ -64,6 +64,9 @@ struct PagedItem {
 // than `share` units, and fewer than twice as many parts as shares.  Up to 64 sequences have a
 // lane each, of more a lane has a run of consecutive ones.  kCut: j counts the tiles
 // that are cut, not the parts; of the parts, a sequence's last tiles, which see the most keys, come first.
+// Of starts in no order the counts have no bound: a lane's stop at kFindMost, which no j reaches (a grid
+// has less than 2^32 threads, 256 a workgroup), so that all in front of an item that is found are exact.
+constexpr int kFindMost = 1 << 24;
 template <bool kCut, class CountOf>
 __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j, PagedItem& it, const CountOf& count) {
     using Count = PagedCount;
@@ -72,26 +75,27 @@ __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j
     if (per == 1 && first < last) mine = count(first);
     int share = 0;
     if (p.target > 0) {
-        int sum = mine.tiles * mine.units;
+        unsigned sum = (unsigned)mine.tiles * (unsigned)mine.units;
         if (per > 1)
             for (int i = first; i < last; ++i) {
                 const Count c = count(i);
-                sum += c.tiles * c.units;
+                sum += (unsigned)c.tiles * (unsigned)c.units;
             }
-        const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-        share = max((int)((unsigned)total + (unsigned)p.target - 1u) / p.target, p.min_share);
+        const unsigned total = (unsigned)__builtin_amdgcn_readlane(wave_scan((int)sum), 63);
+        share = max((int)((total + (unsigned)p.target - 1u) / (unsigned)p.target), p.min_share);
     }
     const auto parts_of = [&](const Count& c) { return share > 0 ? max((c.units + share - 1) / share, 1) : 1; };
-    const auto items_of = [&](const Count& c, int parts) { return kCut ? (parts > 1 ? c.tiles : 0) : c.tiles * parts; };
-    const auto slots_of = [&](const Count& c, int parts) { return parts > 1 ? c.tiles * parts : 0; };
+    const auto all_parts = [](const Count& c, int parts) { return (int)min((long long)c.tiles * parts, (long long)kFindMost); };
+    const auto items_of = [&](const Count& c, int parts) { return kCut ? (parts > 1 ? c.tiles : 0) : all_parts(c, parts); };
+    const auto slots_of = [&](const Count& c, int parts) { return parts > 1 ? all_parts(c, parts) : 0; };
     int parts = parts_of(mine), items = items_of(mine, parts), slots = slots_of(mine, parts);
     if (per > 1) {
         items = slots = 0;
         for (int i = first; i < last; ++i) {
             const Count c = count(i);
             parts = parts_of(c);
-            items += items_of(c, parts);
-            slots += slots_of(c, parts);
+            items = min(items + items_of(c, parts), kFindMost);
+            slots = min(slots + slots_of(c, parts), kFindMost);
         }
     }
     const int inc = wave_scan(items), slot_inc = wave_scan(slots);
@@ -99,7 +103,7 @@ __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j
     if (past == 0) return false;
     const int run = __builtin_ctzll(past);
     int left = j - (__builtin_amdgcn_readlane(inc, run) - __builtin_amdgcn_readlane(items, run));
-    int slot = __builtin_amdgcn_readlane(slot_inc, run) - __builtin_amdgcn_readlane(slots, run);
+    long long slot = __builtin_amdgcn_readlane(slot_inc, run) - __builtin_amdgcn_readlane(slots, run);
     int tiles;
     if (per == 1) {
         it.seq = run;
@@ -135,15 +139,18 @@ __device__ __forceinline__ bool paged_find(const PagedParams& p, int lane, int j
         it.part = left % it.parts;
         it.tile = tiles - 1 - left / it.parts;
     }
-    it.slot = slot + it.tile * it.parts + it.part;
-    // (Of starts in no order the sums may wrap: no partial outside the workspace.)
-    return it.parts == 1 || (unsigned)it.slot + (kCut ? it.parts : 1u) <= 2u * (unsigned)p.target;
+    slot += (long long)it.tile * it.parts + it.part;
+    it.slot = (int)slot;
+    // (Of starts in no order there may be more partials than the workspace holds.)
+    return it.parts == 1 || slot + (kCut ? it.parts : 1) <= 2LL * p.target;
 }
 
 // The work of a KV head as a line of units, its sequences one after the other, of which every
 // workgroup has an equal share.  Share j: from unit u0 of the line on to u1; the sequence
 // of u0 and its place among the sequence's units.  By the lanes of a wave; false past the last
-// unit.
+// unit.  (A sequence has at most 2^52 units, rows and keys being ints; of starts in no order a lane's
+// stop at kLineMost, so that 64 of them do not pass 63 bits.)
+constexpr long long kLineMost = 1LL << 56;
 struct LineShare {
     long long u0, u1, share, at;
     int seq;
@@ -169,7 +176,7 @@ template <class UnitsOf>
 __device__ __forceinline__ bool line_find(const PagedParams& p, int lane, int j, LineShare& w, const UnitsOf& units_of) {
     const int per = (p.n_seqs + 63) / 64, first = min(lane * per, p.n_seqs), last = min(first + per, p.n_seqs);
     long long mine = 0;
-    for (int i = first; i < last; ++i) mine += units_of(i);
+    for (int i = first; i < last; ++i) mine = min(mine + units_of(i), kLineMost);
     long long inc = line_scan(mine, lane);
     const long long total = line_lane(inc, 63);
     w.share = max(line_div(total + p.target - 1, p.target), (long long)p.min_share);
@@ -261,8 +268,7 @@ __device__ __forceinline__ void paged_tile(const PagedParams& p, const PagedItem
     const float c = p.scale_log2;
     const int wave = KS > 1 ? wave_id % kRowWaves : wave_id;
     const int kgrp = KS > 1 ? wave_id / kRowWaves : 0;
-    // (Of starts in no order the sums by which the item was found may wrap.)
-    if ((unsigned)it.tile * (unsigned)kRows >= (unsigned)R) return;
+    if ((unsigned)it.tile * (unsigned)kRows >= (unsigned)R) return;   // not reached
     const auto limit = [&](int row) {  // keys that the row sees
         return p.causal ? min(max(klen - sq.qn + row / ratio + 1, 0), klen) : klen;
     };
