@@ -65,8 +65,8 @@ void kf_kv_append_kernel(KvAppendParams p) {
 // ---------------------------------------------------------------------------
 // Eviction.  Sequence b is cut from n keys to m = min(n, budgets[b]); of every KV head the last r =
 // min(recent, m) stay, and of the n - r old ones the k = m - r of largest weight.
-// Attention does not depend on the order of the old keys, so that only those move
-// that have to: the kept ones in places from k on go to the places below k that were
+// Attention does not depend on the order of the keys, so that of the old ones only those
+// move that have to: the kept ones in places from k on go to the places below k that were
 // freed, the i-th to the i-th, and the last r to k .. m - 1, in order.  (Closing
 // the gaps in order would move half a head's keys where one of them goes.)
 //

@@ -212,7 +212,9 @@ __device__ __forceinline__ int line_parts(const LineShare& w, long long in_front
 __device__ __forceinline__ int line_slot(int share, int k) { return k == 0 ? 2 * share - 1 : 2 * (share + k - 1); }
 
 // Attention of tiles of 32 rows: every tile of a sequence has its 32-key stages, and what
-// starting on one costs, as units.
+// starting on one costs, as units (32 contexts of 512 to 8192 keys, 32 / 8 heads of 128, 80 us with
+// none, 74, 69 and 66 with 3, 6 and 12; 64 of 16 to 512 39, 29, 28 and 27; with up to 8 tokens over 64
+// to 1024 33, 28, 26 and 26).
 constexpr int kLineStart = 6;
 __device__ __forceinline__ int line_stages(const PagedSeq& s) { return kLineStart + key_stages(s.kn); }
 __device__ __forceinline__ long long line_units(const PagedParams& p, int i) {
@@ -222,7 +224,8 @@ __device__ __forceinline__ long long line_units(const PagedParams& p, int i) {
 
 // Chunks are bound by the matrix unit and the softmax, which overlap in part only: 4 x 512
 // tokens over 8192 keys, 32 / 8 heads of 128, 327 us, 866 TFLOPS, 2048 over 65536 at D = 256 2100 us,
-// 1064; steps by HBM, 5.4 TB/s for 32 contexts of 512 to 8192 keys.
+// 1064.  Steps wait half of their cycles and read at 5.4 TB/s (32 contexts of 512 to 8192 keys), the
+// matrix unit is busy for 6 %.
 // A workgroup is NW waves of 32 query rows each; with KS > 1 they form KS groups that
 // take the same rows and a share of the keys each, merged through LDS at the end.
 template <int D, int NW, int KS> struct PagedCfg {
@@ -460,9 +463,10 @@ __device__ __forceinline__ void paged_tile(const PagedParams& p, const PagedItem
     };
     if constexpr (kRowWaves == 1) {
         // The wave copies its stages itself and waits for itself alone: K of the stage after the
-        // next as soon as this one's has been read, and V likewise, so that three of four
-        // half stages are on their way (64 contexts of 2048 keys, 32 / 8 heads of 128: 112 us
-        // with one stage, 108 with these).
+        // next as soon as this one's has been read, and V likewise (64 contexts of 2048 keys,
+        // 32 / 8 heads of 128: 112 us with one stage on its way, 108 so).  As compiled, a
+        // stage's first products also wait for q's loads, and page ids for their own, by the
+        // counter that all copies are in, so that fewer than three of four half stages are.
         constexpr int kHalf = 2 * kUnitInstr;             // copies of K or V of a stage
         const auto landed = [](int halves) {              // but for so many younger halves
             asm volatile("" ::: "memory");
@@ -692,9 +696,11 @@ void kf_attn_paged_merge_kernel(PagedParams p) {
 // The work of a KV head is a line of units, 64 rows that meet a block of keys or a
 // run of a step's keys, of which every workgroup has an equal share.  Where a block's
 // units lie in several shares, their sums go through the workspace and a second kernel.
-// Chunks are bound by the VALU, an exponential, a multiply-add and an addition a
-// score, and the products beside it (4 x 512 tokens over 8192 keys, 32 / 8 heads of 128, 197 us),
-// steps by HBM (32 contexts of 512 to 8192 keys 31.6 us, 5.2 TB/s).
+// Chunks keep neither unit busy: of 421K cycles a SIMD the VALU issues for 195K, an exponential, a
+// multiply-add and an addition a score, and the matrix unit works for 136K, while waves, two a
+// SIMD, wait for 31 % of theirs, for stages at the one barrier of each (4 x 512 tokens over 8192
+// keys, 32 / 8 heads of 128, 198 us).  Steps wait for 75 % and read at 5.2 TB/s (32 contexts of 512
+// to 8192 keys 31.5 us).
 // ---------------------------------------------------------------------------
 constexpr int kWeighRows = 64;                                      // query rows of a stage
 template <int D> struct WeighCfg {
@@ -705,8 +711,9 @@ template <int D> struct WeighCfg {
     static constexpr int kKeys = kWaveKeys * kWaves;                // of a block
     static constexpr int kWavesPerSimd = 2;
     // Steps: a run has a tile of 32 keys for every wave, and counts as much as so many
-    // units; channels of an LDS stage and the stages of a wave; tiles whose sums wait
-    // in LDS.
+    // units (steps alone take the same by 1, 2 and 4, 34 us for 32 contexts of 512 to 8192
+    // keys; with 1 to 256 new tokens each 123, 145 and 180); channels of an LDS stage
+    // and the stages of a wave; tiles whose sums wait in LDS.
     static constexpr int kStepKeys = 32 * kWaves, kStepUnits = 2;
     static constexpr int kStepWidth = D < 128 ? D : 128, kRing = D == 64 ? 4 : 2;
     static constexpr int kStepStage = 32 * kStepWidth * 2, kStepSums = 16;

@@ -303,9 +303,8 @@ int launch_rope_dim(const kf::RopeParams& prm, int D, hipStream_t stream) {
 
 // ---- Attention over the paged 16-bit cache. ----
 
-// Rows of a tile and KV groups of the layouts of the paged kernel (PagedCfg).
 struct PagedPlan {
-    int rows, slots;
+    int rows, slots;                      // rows of a tile (PagedCfg)
     long long items, cut_tiles;           // at most, of a KV head
     size_t o_bytes, s_bytes, ws_bytes;
     kf::PagedParams prm;
@@ -335,14 +334,27 @@ int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, 
     if (const int st = check_paged(n_seqs, tokens, H_q, H_kv, D, page_size, max_pages, num_pages, &prm); st != KF_OK)
         return st;
     const long long rows = (long long)tokens * (H_q / H_kv);
+    // By the rows that a sequence has on average.  us with 32, 64 and 128 rows, 32 / 8 heads of 128:
+    //   32 x 4 tokens over 2048 keys 52, 53, 53  x 12 92, 59, 61  x 24 134, 64, 70  x 64 338, 117, 102
+    //   4 x 4 over 8192 36, 36, 36               x 12 50, 45, 46  x 24  69, 42, 48  x 64 129,  64,  65
+    //   32 x 1 over 512 to 8192 69, 73, 67       x 1 to 4 71, 76, 71;  8 x 1 over 512 to 32768 54, 62, 54
+    // and with 32 and 128 rows, 16 / 4 heads of 256,
+    //   32 x 4 over 2048 70, 60                  x 12 102, 69;  4 x 4 over 8192 53, 59  x 12 76, 86
+    //   32 x 1 over 512 to 8192 74, 88           x 1 to 16 94, 105  x 1 to 64 136, 115
+    // At D = 64, 64 rows would be the best up to 96, too (32 x 2 over 2048 33, 29, 34, x 24 67, 40, 42;
+    // 32 x 1 over 512 to 8192 36, 35, 40).  Averages say little of steps beside a prompt or of empty
+    // sequences: 1 x 4096 alone takes 169 us, among 999 empty ones, in tiles of 32, 996.
     const double avg = (double)rows / n_seqs;
     pl->rows = D == 256 ? (avg > 32 ? 128 : 32) : avg > 64 ? 128 : avg > 32 ? 64 : 32;
     if (pl->rows == 32) {
         // Equal shares of a line, for every workgroup that the device holds; no fewer than 8
-        // units each.
+        // units each (one step over 4096 keys, 32 / 8 heads of 128, 17.6, 16.4 and 18.7 us by 4, 8 and
+        // 16; 40 of 1 to 4 tokens over 16 to 300 20, 20 and 23).
         prm.target = std::max(1, current_device_shape().cus * (D == 64 ? 2 : 1) / H_kv);
         prm.min_share = 8;
-        // (Few keys: no second launch.)
+        // Few keys: no second launch (by the table's places: the host knows no lengths).  us without and
+        // with one: 1 step over 256 keys 10.6, 13.3, over 512 14.1, 13.4, over 1024 21.5, 14.0; 32 steps
+        // 12.6, 14.5, 18.3, 20.3, and over 2048 48, 50.
         prm.cut = prm.target > 1 && prm.kv_len > 256 ? 1 : 0;
         pl->items = prm.target;
         pl->cut_tiles = prm.cut ? prm.target - 1 : 0;
@@ -353,10 +365,14 @@ int paged_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, 
     const long long least = (rows + pl->rows - 1) / pl->rows;
     const long long tiles = rows / pl->rows + std::min<long long>(n_seqs, tokens);
     const long long stages = ((long long)prm.kv_len + 31) / 32;
+    // No cuts where tiles fill the device twice, or of few keys (us without and with cuts, 64 tokens: 1 x over
+    // 256 keys 14.0, 15.8, over 512 21.0, 20.0, over 1024 35, 21; 16 x 16.3, 18.4, 23.9, 32.0, 38, 42, and
+    // over 2048 66, 63).
     const int wanted = std::max(1, 2 * current_device_shape().cus / H_kv);
     prm.target = least >= 2 * wanted || stages <= 8 ? 0 : wanted;
     prm.unit_shift = 0;
     while (tiles * ((stages >> prm.unit_shift) + 1) > INT_MAX) ++prm.unit_shift;
+    // (1 x 64 tokens over 2048 keys 33, 26 and 28 us by 4, 8 and 16, 4 x 64 over 512 25, 21, 23.)
     prm.min_share = std::max(1, 8 >> prm.unit_shift);
     pl->items = tiles + prm.target;
     pl->cut_tiles = std::min<long long>(tiles, prm.target);
@@ -430,11 +446,15 @@ int weigh_plan(int n_seqs, int tokens, int H_q, int H_kv, int D, int page_size, 
         return st;
     const int keys = D == 256 ? kf::WeighCfg<256>::kKeys : kf::WeighCfg<128>::kKeys;
     const long long rows = (long long)tokens * (H_q / H_kv);
-    // A share for every workgroup that the device holds.
+    // A share for every workgroup that the device holds, of 4 units at least (us by 2, 4 and 8: 1 x 64
+    // tokens over 8192 keys 29.4, 26.5, 28.9, over 512 16.4, 20.3, 26.9; 32 steps over 512 12.2, 12.1, 14.8).
     prm.target = std::max(1, 2 * current_device_shape().cus / H_kv);
     prm.min_share = 4;
     // Blocks are cut where sequences have, on average, more than a stage of rows; a
-    // batch of steps is spared the second launch.
+    // batch of steps is spared the second launch.  us without and with cuts, 32 / 8 heads of 128: 1 x 32
+    // tokens over 2048 keys 19, 22 |  x 64 17, 21 |  x 128 25, 21 |  x 512 79, 35; 4 x 64 over 8192 45, 48 |
+    // x 128 67, 67 |  x 512 209, 198.  (1 x 1000 alone 32 us; among 63 empty sequences, by the average not
+    // cut, 96.)
     prm.cut = rows / n_seqs > kf::kWeighRows ? 1 : 0;
     pl->ws_bytes = prm.cut ? align_up((size_t)2 * prm.target * H_kv * keys * sizeof(float), kWsAlign) : 0;
     return fits_grid((long long)prm.target * H_kv, 4 * keys) ? KF_OK : KF_ERR_SIZE;
@@ -484,7 +504,9 @@ int evict_plan(int n_seqs, int H_kv, int D, int page_size, int max_pages, int nu
     if (n_seqs <= 0 || H_kv <= 0) return KF_ERR_SIZE;
     if (const int st = paged_geometry(page_size, max_pages, num_pages, &pl->shift, &pl->capacity); st != KF_OK) return st;
     const long long groups = (long long)n_seqs * H_kv;
-    // Up to 32 workgroups a CU that move keys, each with a few rounds at least.
+    // Up to 32 workgroups a CU that move keys, each with a few rounds at least (16 contexts of 4096 to
+    // 32768 keys to half 145, 138 and 137 us by 16, 32 and 64; one key of 32 contexts in tables of 65536
+    // places 28.5, 28.9, 32.8).
     const long long rounds = pl->capacity / 2 / (kf::kMoveThreads * 8 / D * kf::kMoveAhead);
     pl->parts = (int)std::max<long long>(1, std::min(32LL * current_device_shape().cus / groups, rounds / 4));
     if (pl->capacity > kMaxIndex || !fits_grid(groups, kf::kSelectThreads) ||
