@@ -459,7 +459,8 @@ int kf_attn_paged(const void* Q, const int64_t* strides, const void* K_pages, co
  * [tokens, H_q] is the row_max with KF_ATTN_LSE (natural logarithm); a row whose lse
  * is -inf adds nothing, whatever it and the keys hold.  flags: KF_ATTN_CAUSAL, KF_BF16.
  * A NaN or an infinity in another row of Q, or a NaN in its lse, reaches the keys that
- * the row sees and no others, one in a key the key's own weight.  Sequences that share a page race for its weights: they must not.
+ * the row sees and no others, one in a key the key's own weight.  Sequences that share a
+ * page race for its weights: they must not.
  * Workspace: kf_kv_weigh_workspace_bytes() bytes (may be 0, then NULL will do), as
  * kf_attn_paged's. */
 size_t kf_kv_weigh_workspace_bytes(int n_seqs, int tokens, int H_q, int H_kv, int D,
